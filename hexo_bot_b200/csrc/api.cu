@@ -17,48 +17,13 @@
 #include "attention_geo.cuh"
 #include "aux.cuh"
 #include "gemm.cuh"
+#include "host.cuh"
 #include "conv_ts.cuh"
 #include "conv_grid.cuh"
 #include "mlp.cuh"
 
 namespace sb {
 namespace {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-// SHRIMP_B200_SYNC_DEBUG=1: synchronise and log after every launch (debugging
-// aid; never set in serving).
-bool sync_debug() {
-  static const bool v = [] {  // read once (thread-safe static initialisation)
-    const char* e = getenv("SHRIMP_B200_SYNC_DEBUG");
-    return e && e[0] == '1';
-  }();
-  return v;
-}
-
-int check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && sync_debug()) {
-    fprintf(stderr, "[sb] launched %s ...", what);
-    fflush(stderr);
-    e = cudaDeviceSynchronize();
-    fprintf(stderr, " done (%s)\n", cudaGetErrorString(e));
-  }
-  if (e != cudaSuccess) return fail(SB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-  return SB_OK;
-}
-
-inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
 // Programmatic dependent launch inside the forward: every kernel after the
 // first is launched with the programmatic-serialization attribute, so its
@@ -103,7 +68,6 @@ void launch_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   cfg.numAttrs = t_pdl ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);  // errors surface in check_launch
 }
-inline int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
 // N tile for an n-wide GEMM: one tile when n <= 256, else the fewest equal
 // tiles (multiples of 16) of at most 256 columns.
@@ -115,21 +79,6 @@ int choose_bn(int n) {
     if (bn <= 256 && bn % 32 == 0) return bn;
   }
   return -1;
-}
-
-// Raise a kernel's dynamic shared-memory limit once per (device, kernel).
-int ensure_smem(const void* fn, int bytes) {
-  struct Entry { const void* fn; int dev; int bytes; };
-  static thread_local Entry cache[64];
-  static thread_local int used = 0;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  for (int i = 0; i < used; ++i)
-    if (cache[i].fn == fn && cache[i].dev == dev && cache[i].bytes >= bytes) return SB_OK;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(SB_ERR_CUDA, "shared-memory attribute: %s", cudaGetErrorString(e));
-  if (used < 64) cache[used++] = Entry{fn, dev, bytes};
-  return SB_OK;
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -199,21 +148,6 @@ int make_tmap_3d(CUtensorMap* m, const void* ptr, CUtensorMapDataType dt, int es
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled (3D) failed (%d)", (int)r);
   return SB_OK;
-}
-
-int num_sms() {
-  // per device; host threads racing on a first query store the same value
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) dev = 0;
-  int n = cache[dev].load(std::memory_order_relaxed);
-  if (!n) {
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 148;
-    cache[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 template <typename T>
