@@ -44,6 +44,15 @@ EXPORTED = (
     "sb_legal_prefix_softmax",
     "sb_raytap_conv",
     "sb_offset_attention",
+    "sb_axes_rotary",
+    "sb_qk_norm_rotary",
+    "sb_qk_norm_rotary_backward_workspace_bytes",
+    "sb_qk_norm_rotary_backward",
+    "sb_block_means",
+    "sb_block_select",
+    "sb_block_attention_workspace_bytes",
+    "sb_block_attention",
+    "sb_block_attention_backward",
 )
 
 _P = C.c_void_p
@@ -112,6 +121,19 @@ class Group(C.Structure):
     _fields_ = [("start", C.c_int), ("end", C.c_int), ("pad_to", C.c_int)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("data", _P), ("batch_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [
+        ("coords", _P), ("coords_dtype", C.c_int),
+        ("batch_stride", C.c_int64), ("row_stride", C.c_int64), ("axis_stride", C.c_int64),
+        ("prefix", C.c_int), ("axes", C.c_int), ("sections", C.c_int * 4), ("adjacent", C.c_int),
+        ("freqs", _P),
+    ]
+
+
 class NativeError(RuntimeError):
     pass
 
@@ -127,6 +149,8 @@ def lib() -> C.CDLL:
     sz = C.c_size_t
     i32 = C.c_int
     f32 = C.c_float
+    hd = C.POINTER(Heads)
+    ro = C.POINTER(Rotary)
     sig = {
         "sb_abi_version": ([], i32),
         "sb_last_error": ([C.c_char_p, sz], i32),
@@ -152,6 +176,17 @@ def lib() -> C.CDLL:
         "sb_legal_prefix_softmax": ([_P, i32, i32, _P, _P, _P, _P], i32),
         "sb_raytap_conv": ([_P, _P, i32, _P, _P, i32, i32, i32, _P, _P, sz, _P], i32),
         "sb_offset_attention": ([_P, _P, _P, _P, i32, _P, i32, i32, i32, i32, _P, _P], i32),
+        "sb_axes_rotary": ([hd, i32, ro, i32, i32, i32, i32, i32, hd, _P], i32),
+        "sb_qk_norm_rotary": ([hd, hd, i32, _P, _P, i32, f32, ro, i32, i32, i32, i32, i32, hd, hd, _P], i32),
+        "sb_qk_norm_rotary_backward_workspace_bytes": ([i32, C.POINTER(sz)], i32),
+        "sb_qk_norm_rotary_backward": ([hd, hd, hd, hd, i32, _P, _P, i32, f32, ro, i32, i32, i32, i32, i32, hd, hd, _P, _P,
+                                        _P, sz, _P], i32),
+        "sb_block_means": ([hd, i32, _P, i32, i32, i32, i32, i32, _P, _P], i32),
+        "sb_block_select": ([hd, i32, _P, _P, _P] + [i32] * 10 + [_P, _P], i32),
+        "sb_block_attention_workspace_bytes": ([i32] * 9 + [C.POINTER(sz)], i32),
+        "sb_block_attention": ([hd, hd, hd, i32, _P, _P, _P] + [i32] * 8 + [f32, hd, _P, _P, sz, _P], i32),
+        "sb_block_attention_backward": ([hd, hd, hd, hd, hd, _P, i32, _P, _P, _P] + [i32] * 8
+                                        + [f32, hd, hd, hd, _P, sz, _P], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(h, name)

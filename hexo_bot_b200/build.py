@@ -18,8 +18,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_native"
 LIB_NAME = "libshrimp_b200.so"
-SOURCES = ["api.cu"]
-HEADERS = ["host.cuh", "ptx.cuh", "gemm.cuh", "conv_ts.cuh", "conv_grid.cuh", "mlp.cuh", "attention.cuh", "attention_geo.cuh", "aux.cuh"]
+SOURCES = ["api.cu", "attention_ops.cu"]
+HEADERS = ["host.cuh", "ptx.cuh", "gemm.cuh", "conv_ts.cuh", "conv_grid.cuh", "mlp.cuh", "attention.cuh", "attention_geo.cuh", "aux.cuh",
+           "rotary.cuh", "block_select.cuh", "block_attention.cuh"]
 INCLUDE = PKG.parent / "include"
 
 NVCC_FLAGS = [
@@ -27,6 +28,7 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
     "--expt-relaxed-constexpr",
+    "--threads", "0",  # the translation units side by side
 ]
 
 

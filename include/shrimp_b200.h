@@ -256,6 +256,93 @@ int sb_hex_conv_ln_planned(const void* x, const void* plan, size_t plan_bytes, i
 int sb_attn_pair(const void* q, const void* k, const void* v, const uint8_t* pair, const float* table2,
                  const int32_t* seq_lens, int batch, int heads, int seq, int head_dim, void* out, void* stream);
 
+/* ---- long-support attention operators --------------------------------------
+ * For attention layers over supports of many cells (or other long rows) beside
+ * the biased dense ops above: rotary positions, query / key norms, and
+ * attention over key blocks that each query chooses. No counterpart in the
+ * reference. Tensors are (batch, heads, rows, head_dim) views with any
+ * batch / head / row strides (in elements) and unit stride over head_dim, so
+ * the heads of a packed projection (B, S, 3, H, D) are passed where they lie. */
+typedef struct {
+  void* data;            /* element (0, 0, 0, 0); read only where the op says input */
+  int64_t batch_stride, head_stride, row_stride;
+} sb_heads;
+
+/* Rotary positions with several axes: axis a turns sections[a] channel pairs,
+ * axes in order; pair p turns by coord[axis of p] * freqs[p] radians. Half
+ * pairing joins channels (p, P + p), adjacent pairing (2p, 2p + 1), P = all
+ * pairs; channels from 2P on stay. The first `prefix` rows (summary tokens)
+ * have no coordinates and stay; coordinate row r belongs to row prefix + r. */
+typedef struct {
+  const void* coords; int coords_dtype;  /* (B, rows - prefix, axes) i16 / i32 / i64 / f32 */
+  int64_t batch_stride, row_stride, axis_stride;
+  int prefix;
+  int axes;              /* 1 to 4 */
+  int sections[4];       /* pairs of each axis, >= 1 */
+  int adjacent;
+  const double* freqs;   /* (P) radians per coordinate step, on the device */
+} sb_rotary;
+
+/* out = rotated x (inverse != 0: rotated back, which is also the gradient).
+ * x, out (B, H, S, D) f32 / f16 / bf16, D <= 256; out may be x. Angles are
+ * reduced in 64 bits, the rotation is computed in 32 and rounded once. */
+int sb_axes_rotary(const sb_heads* x, int dtype, const sb_rotary* rotary, int inverse, int batch, int heads, int rows,
+                   int head_dim, const sb_heads* out, void* stream);
+/* RMS norm of every query and key head, times a weight per channel, then the
+ * rotation, in one pass: y = R (x (mean(x^2) + eps)^-1/2 w). q (B, Hq, S, D),
+ * k (B, Hk, S, D) or k_heads = 0; weights (D) f32 / f16 / bf16 or NULL (= 1);
+ * rotary NULL = norm alone; q_out / k_out may be q / k. */
+int sb_qk_norm_rotary(const sb_heads* q, const sb_heads* k, int dtype, const void* q_weight, const void* k_weight,
+                      int weight_dtype, float eps, const sb_rotary* rotary, int batch, int q_heads, int k_heads, int rows,
+                      int head_dim, const sb_heads* q_out, const sb_heads* k_out, void* stream);
+/* Its gradients from those of q_out and k_out and the inputs of the forward:
+ * dq, dk (may be dq_out / dk_out), and dq_weight, dk_weight (weight_dtype) or
+ * NULL. The weight gradients are summed in a fixed order. */
+int sb_qk_norm_rotary_backward_workspace_bytes(int head_dim, size_t* bytes);
+int sb_qk_norm_rotary_backward(const sb_heads* dq_out, const sb_heads* dk_out, const sb_heads* q, const sb_heads* k, int dtype,
+                               const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                               const sb_rotary* rotary, int batch, int q_heads, int k_heads, int rows, int head_dim,
+                               const sb_heads* dq, const sb_heads* dk, void* dq_weight, void* dk_weight, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* means (B, Hkv, ceil(kv_rows / block), D) f32 = mean of each block's live
+ * keys (keys t < kv_lens[b]; NULL = all), 0 for a block without any. Summed in
+ * 64 bits, rounded once. k f32 / f16 / bf16, D <= 256, any block >= 1. */
+int sb_block_means(const sb_heads* k, int dtype, const int32_t* kv_lens, int batch, int kv_heads, int kv_rows, int head_dim,
+                   int block, float* means, void* stream);
+/* The key blocks that each query keeps, by score = (sum of the group's query
+ * heads) . mean: index (B, Hkv, Sq, topk) int32, ascending, -1 where a row has
+ * fewer live blocks or is no live query (row >= q_lens[b]). The first
+ * keep_first blocks, and with keep_own the block row / block, are kept before
+ * the others (keep_first + keep_own <= topk). Ties go to the lowest index, NaN
+ * ranks below every number. The choice equals that of 64-bit scores.
+ * topk <= 64, at most 16384 blocks, D <= 256. */
+int sb_block_select(const sb_heads* q, int dtype, const float* means, const int32_t* kv_lens, const int32_t* q_lens, int batch,
+                    int q_heads, int kv_heads, int q_rows, int kv_rows, int head_dim, int block, int topk, int keep_first,
+                    int keep_own, int32_t* index, void* stream);
+/* Softmax attention of each query over the live keys of its blocks:
+ * out (B, Hq, Sq, D) and lse (B, Hq, Sq) f32 = log of the sum of exp(scores).
+ * Query head h reads key head h / (Hq / Hkv). q, k, v, out f16 / bf16, D a
+ * multiple of 8 up to 128, block 32 / 64 / 128, topk <= 64, bases 16-byte
+ * aligned and strides multiples of 8. Index entries below 0 or past the live
+ * blocks are skipped and a block named twice counts once, in any order. A row
+ * without keys, or past q_lens[b], gives zeros and lse = -inf. Results do not
+ * vary from run to run. Few queries (<= 16 rows) need no workspace. */
+int sb_block_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int q_rows, int kv_rows, int head_dim, int block,
+                                       int topk, int backward, size_t* bytes);
+int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, int dtype, const int32_t* index,
+                       const int32_t* kv_lens, const int32_t* q_lens, int batch, int q_heads, int kv_heads, int q_rows,
+                       int kv_rows, int head_dim, int block, int topk, float scale, const sb_heads* out, float* lse,
+                       void* workspace, size_t workspace_bytes, void* stream);
+/* dq, dk, dv from the gradient of out and the forward's operands and results
+ * (the choice of blocks has no gradient). Rows past q_lens / kv_lens get
+ * zeros. q_rows >= 1. */
+int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const sb_heads* k, const sb_heads* v,
+                                const sb_heads* out, const float* lse, int dtype, const int32_t* index,
+                                const int32_t* kv_lens, const int32_t* q_lens, int batch, int q_heads, int kv_heads,
+                                int q_rows, int kv_rows, int head_dim, int block, int topk, float scale, const sb_heads* dq,
+                                const sb_heads* dk, const sb_heads* dv, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 /* ---- weight packing ------------------------------------------------------ */
 /* HexNodeConv weight (taps, Cin, Cout) fp32 -> f16 [Cout][Kpad], Kpad =
  * roundup(taps * cin_pad, 64), channel c >= Cin of each tap zero. */
