@@ -159,6 +159,48 @@ void put(RotArgs* a, int slot, const sb_heads* x, const sb_heads* dy, const sb_h
   }
 }
 
+// ---- block selection ----------------------------------------------------------
+constexpr int kSelFewRows = 8;  // up to so many queries of a sequence take the few-query kernel
+
+template <typename T, int PER>
+int launch_select_per(const SelArgs& a, unsigned grid, cudaStream_t st) {
+  const int smem = sel_smem_bytes(a.tile, a.nb, a.dim);
+  if (int s = ensure_smem(reinterpret_cast<const void*>(block_select_kernel<T, PER>), smem)) return s;
+  block_select_kernel<T, PER><<<grid, kSelThreads, smem, st>>>(a);
+  return check_launch("block_select_kernel");
+}
+template <typename T>
+int launch_select(const SelArgs& a, unsigned grid, cudaStream_t st) {
+  if (a.nb <= 40) return launch_select_per<T, 5>(a, grid, st);
+  if (a.nb <= 64) return launch_select_per<T, 8>(a, grid, st);
+  if (a.nb <= 128) return launch_select_per<T, 16>(a, grid, st);
+  return launch_select_per<T, 0>(a, grid, st);
+}
+template <typename T, int PER>
+int launch_select_few_per(const SelArgs& a, unsigned rows, int cluster, cudaStream_t st) {
+  const int smem = sel_few_smem_bytes(a.nb);
+  if (int s = ensure_smem(reinterpret_cast<const void*>(block_select_few_kernel<T, PER>), smem)) return s;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = rows * cluster;
+  cfg.blockDim = kSelThreads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, block_select_few_kernel<T, PER>, a);  // errors surface in check_launch
+  return check_launch("block_select_few_kernel");
+}
+template <typename T>
+int launch_select_few(const SelArgs& a, unsigned rows, int cluster, cudaStream_t st) {
+  if (a.nb <= 2 * kSelThreads) return launch_select_few_per<T, 2>(a, rows, cluster, st);
+  if (a.nb <= 8 * kSelThreads) return launch_select_few_per<T, 8>(a, rows, cluster, st);
+  return launch_select_few_per<T, 0>(a, rows, cluster, st);
+}
+
 // ---- block-sparse attention ------------------------------------------------------
 // Bytes of parts that a window of rows may hold: they stay in the 126 MB L2
 // between the kernel that writes them and the one that joins them.
@@ -466,15 +508,24 @@ int sb_block_means(const sb_heads* k, int dtype, const int32_t* kv_lens, int bat
   const bool wide = heads_vec(k, e, 16 / e) == 16 / e && head_dim % (16 / e) == 0;
   cudaStream_t st = (cudaStream_t)stream;
   const HeadsView kv = view(k);
+  // a warp a block, or a CTA of four where that leaves SMs without work
+  const bool split = grid < 8ll * num_sms();
+  const int vec = wide ? 16 / e : 1;
+  const int chunk_lanes = 1 << pow2_log2(head_dim / vec < 32 ? head_dim / vec : 32);
+  const unsigned ctas = (unsigned)(split ? grid : cdiv(grid, kMeansThreads / 32));
+#define SB_MEANS_AS(T, V, W)                                                                                      \
+  block_means_kernel<T, V, W><<<ctas, kMeansThreads, 0, st>>>(kv, kv_lens, kv_heads, kv_rows, head_dim, block, nb, grid, \
+                                                              chunk_lanes, means)
 #define SB_MEANS(T, V) \
-  block_means_kernel<T, V><<<(unsigned)grid, kMeansThreads, 0, st>>>(kv, kv_lens, kv_heads, kv_rows, head_dim, block, nb, means)
+  if (split) SB_MEANS_AS(T, V, 4); else SB_MEANS_AS(T, V, 1)
   if (dtype == SB_F32) {
-    if (wide) SB_MEANS(float, 4); else SB_MEANS(float, 1);
+    if (wide) { SB_MEANS(float, 4); } else { SB_MEANS(float, 1); }
   } else if (dtype == SB_F16) {
-    if (wide) SB_MEANS(__half, 8); else SB_MEANS(__half, 1);
+    if (wide) { SB_MEANS(__half, 8); } else { SB_MEANS(__half, 1); }
   } else {
-    if (wide) SB_MEANS(__nv_bfloat16, 8); else SB_MEANS(__nv_bfloat16, 1);
+    if (wide) { SB_MEANS(__nv_bfloat16, 8); } else { SB_MEANS(__nv_bfloat16, 1); }
   }
+#undef SB_MEANS_AS
 #undef SB_MEANS
   return check_launch("block_means_kernel");
 }
@@ -517,6 +568,18 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
   a.topk = topk;
   a.keep_first = keep_first;
   a.keep_own = keep_own != 0;
+  a.q_vec = head_dim % 8 == 0 && heads_vec(q, e, 16 / e) == 16 / e;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (q_rows <= kSelFewRows) {
+    const long long rows = (long long)batch * kv_heads * q_rows;
+    // CTAs of a row: enough that the means are read by every SM, each with some rows to read
+    int cluster = 1;
+    while (cluster < kSelFewCluster && rows * cluster < 2 * num_sms() && nb >= 64 * cluster) cluster *= 2;
+    if (rows * cluster > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
+    if (dtype == SB_F32) return launch_select_few<float>(a, (unsigned)rows, cluster, st);
+    if (dtype == SB_F16) return launch_select_few<__half>(a, (unsigned)rows, cluster, st);
+    return launch_select_few<__nv_bfloat16>(a, (unsigned)rows, cluster, st);
+  }
   // the widest tile whose scores leave room for two CTAs an SM
   int tile = 64;
   while (tile > 2 && (sel_smem_bytes(tile, a.nb, head_dim) > 100 * 1024 || tile / 2 >= q_rows)) tile >>= 1;
@@ -524,18 +587,9 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
   a.tiles = (int)cdiv(q_rows, tile);
   const long long grid = (long long)batch * kv_heads * a.tiles;
   if (grid > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
-  const int smem = sel_smem_bytes(tile, a.nb, head_dim);
-  cudaStream_t st = (cudaStream_t)stream;
-#define SB_SELECT(T)                                                                             \
-  do {                                                                                           \
-    if (int s = ensure_smem(reinterpret_cast<const void*>(block_select_kernel<T>), smem)) return s; \
-    block_select_kernel<T><<<(unsigned)grid, kSelThreads, smem, st>>>(a);                        \
-  } while (0)
-  if (dtype == SB_F32) SB_SELECT(float);
-  else if (dtype == SB_F16) SB_SELECT(__half);
-  else SB_SELECT(__nv_bfloat16);
-#undef SB_SELECT
-  return check_launch("block_select_kernel");
+  if (dtype == SB_F32) return launch_select<float>(a, (unsigned)grid, st);
+  if (dtype == SB_F16) return launch_select<__half>(a, (unsigned)grid, st);
+  return launch_select<__nv_bfloat16>(a, (unsigned)grid, st);
 }
 
 int sb_block_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int q_rows, int kv_rows, int head_dim, int block,

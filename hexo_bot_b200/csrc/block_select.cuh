@@ -6,12 +6,13 @@
 //              scores; ties to the lowest index, NaN below everything
 //
 // The choice is the one 64-bit arithmetic on the given means makes. Scores are
-// computed in 32 bits together with a bound on their error; a row whose last
-// kept and first dropped score lie within that bound of one another (or that
-// holds a score that is not finite) is done again in 64 bits, all others are
-// settled by their 32-bit scores.
+// computed in 32 bits together with a bound on their error. Where the last
+// kept and the first dropped score lie further apart than that, they settle the
+// row; else the few scores near the border are computed again in 64 bits, and
+// the whole row where many are near or one is not finite.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -19,6 +20,7 @@
 #include <cfloat>
 #include <cstdint>
 
+#include "ptx.cuh"
 #include "rotary.cuh"
 
 namespace sb {
@@ -29,6 +31,7 @@ constexpr int kSelMaxBlocks = 16384;
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelChunk = 64;  // blocks of a score chunk
+constexpr float kSelTiny = 1e-40f;  // more than the squares of a row lose to underflow
 
 struct HeadsView {
   const void* p;
@@ -36,47 +39,70 @@ struct HeadsView {
 };
 
 // ---- block means ------------------------------------------------------------
-// One CTA per (batch, head, block). Sums run in 64 bits, so 16-bit keys add up
-// without error and the mean is rounded once.
+// Sums run in 64 bits, so 16-bit keys add up without error and the mean is
+// rounded once. WPU warps make a unit (one block of one head): a lane holds a
+// VEC-wide channel chunk, the lanes of one chunk split the rows and are joined
+// by shuffles, the warps of a unit through shared memory. Bound by HBM (the
+// keys are read once); loads of a lane are issued four rows at a time.
 constexpr int kMeansThreads = 128;
 
-template <typename T, int VEC>
+template <typename T, int VEC, int WPU>
 __global__ __launch_bounds__(kMeansThreads) void block_means_kernel(HeadsView k, const int* __restrict__ kv_lens,
                                                                     int heads, int rows, int dim, int block, int nb,
+                                                                    long long units, int chunk_lanes,
                                                                     float* __restrict__ out) {
-  __shared__ double red[kMeansThreads * VEC];
-  const long long u = blockIdx.x;
+  constexpr int UNITS = kMeansThreads / 32 / WPU;
+  __shared__ double red[WPU > 1 ? WPU : 1][32 * VEC];
+  using V = RotVec<T, VEC>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wu = warp % WPU;
+  const long long u = (long long)blockIdx.x * UNITS + warp / WPU;
+  if (u >= units) return;  // whole units: with WPU > 1 a CTA is one unit
   const int j = (int)(u % nb);
   const long long bh = u / nb;
   const int b = (int)(bh / heads), h = (int)(bh - (long long)b * heads);
   int len = kv_lens ? kv_lens[b] : rows;
   len = len < 0 ? 0 : len > rows ? rows : len;
-  const int n = len - j * block < block ? len - j * block : block;
+  const int n = min(len - j * block, block);
   const int chunks = dim / VEC;
-  using V = RotVec<T, VEC>;
+  const int strands = 32 / chunk_lanes;  // row strands of a warp
+  const int cl = lane % chunk_lanes, step = strands * WPU;
   const T* base = (const T*)k.p + b * k.b + h * k.h + (long long)j * block * k.s;
-  for (int c0 = 0; c0 < chunks; c0 += kMeansThreads) {
-    const int nc = chunks - c0 < kMeansThreads ? chunks - c0 : kMeansThreads;
-    const int strands = kMeansThreads / nc;
-    const int c = threadIdx.x % nc, g = threadIdx.x / nc;
+  for (int c0 = 0; c0 < chunks; c0 += chunk_lanes) {
+    const int c = c0 + cl;
     double acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.0;
-    if (g < strands)
-      for (int r = g; r < n; r += strands) {
-        const V v = *reinterpret_cast<const V*>(base + r * k.s + (c0 + c) * VEC);
+    if (c < chunks) {
+      for (int r0 = wu * strands + lane / chunk_lanes; r0 < n; r0 += 4 * step) {
+        V v[4];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += (double)rot_f32(v.v[e]);
+        for (int x = 0; x < 4; ++x)
+          v[x] = r0 + x * step < n ? *reinterpret_cast<const V*>(base + (r0 + x * step) * k.s + c * VEC) : V{};
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += (double)rot_f32(v[x].v[e]);
       }
-    __syncthreads();
+    }
+    for (int m = chunk_lanes; m < 32; m <<= 1)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) red[e * kMeansThreads + threadIdx.x] = acc[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < nc * VEC; i += kMeansThreads) {
-      const int cc = i / VEC, e = i - cc * VEC;
-      double s = 0.0;
-      for (int g2 = 0; g2 < strands; ++g2) s += red[e * kMeansThreads + g2 * nc + cc];
-      out[(bh * nb + j) * dim + (c0 + cc) * VEC + e] = n > 0 ? (float)(s / n) : 0.f;
+      for (int e = 0; e < VEC; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], m);
+    if (WPU > 1) {
+      __syncthreads();
+      if (lane < chunk_lanes)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) red[wu][lane * VEC + e] = acc[e];
+      __syncthreads();
+      if (wu == 0 && lane < chunk_lanes)
+#pragma unroll
+        for (int w = 1; w < WPU; ++w)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += red[w][lane * VEC + e];
+    }
+    if (wu == 0 && lane < chunk_lanes && c < chunks) {
+      float* o = out + (bh * nb + j) * dim + c * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = n > 0 ? (float)(acc[e] / n) : 0.f;
     }
   }
 }
@@ -91,98 +117,227 @@ struct SelArgs {
   int batch, kv_heads, group, q_rows, kv_rows, dim, nb, block, topk, keep_first, keep_own;
   int tile;            // queries of a CTA
   int tiles;           // tiles of a sequence
+  int q_vec;           // query rows may be read in 16-byte pieces
 };
 
-// Order-preserving image of a float (larger float -> larger integer).
+// One row's choice.
+struct SelRow {
+  int live, topk, own, first, forced;
+  __device__ __forceinline__ SelRow(const SelArgs& a, int row, int live_blocks) {
+    live = live_blocks;
+    topk = a.topk;
+    first = a.keep_first < live ? a.keep_first : live;
+    own = a.keep_own && row / a.block < live ? row / a.block : -1;
+    forced = first + (own >= first ? 1 : 0);
+  }
+  __device__ __forceinline__ bool is_forced(int j) const { return j < first || j == own; }
+  __device__ __forceinline__ int want() const { return topk - forced; }  // among the others
+};
+
+// Order-preserving image of a float (larger float -> larger integer), NaN the
+// lowest (1); 0 marks blocks that do not compete.
 __device__ __forceinline__ uint32_t sel_key(float f) {
   const uint32_t u = __float_as_uint(f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return isnan(f) ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float sel_unkey(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-__device__ __forceinline__ bool sel_forced(int j, int own, int keep_first) { return j < keep_first || j == own; }
-
-// Writes the kept blocks of one row in ascending order, -1 behind them. `kept`
-// tells for a block index whether it is kept; called by a whole warp.
-template <typename F>
-__device__ __forceinline__ void sel_write(int* out, int live, int topk, F kept) {
-  const int lane = threadIdx.x & 31;
-  int n = 0;
-  for (int j0 = 0; j0 < live; j0 += 32) {
-    const int j = j0 + lane;
-    const bool k = j < live && kept(j);
-    const uint32_t m = __ballot_sync(0xffffffffu, k);
-    const int at = n + __popc(m & ((1u << lane) - 1u));
-    if (k && at < topk) out[at] = j;
-    n += __popc(m);
+// Threads that settle a row together: a warp, or a whole CTA.
+struct SelWarp {
+  static constexpr int N = 32;
+  __device__ __forceinline__ int id() const { return threadIdx.x & 31; }
+  __device__ __forceinline__ unsigned add(unsigned v) const { return __reduce_add_sync(0xffffffffu, v); }
+  __device__ __forceinline__ unsigned min(unsigned v) const { return __reduce_min_sync(0xffffffffu, v); }
+  __device__ __forceinline__ unsigned max(unsigned v) const { return __reduce_max_sync(0xffffffffu, v); }
+};
+struct SelCta {
+  static constexpr int N = kSelThreads;
+  unsigned* s;  // shared [2][kSelWarps], used in turn: one barrier a join
+  int turn = 0;
+  __device__ __forceinline__ int id() const { return threadIdx.x; }
+  template <typename F>
+  __device__ __forceinline__ unsigned join(unsigned v, F f) {
+    unsigned* p = s + turn * kSelWarps;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = v;
+    __syncthreads();
+    unsigned r = p[0];
+#pragma unroll
+    for (int w = 1; w < kSelWarps; ++w) r = f(r, p[w]);
+    return r;
   }
-  for (int i = n + lane; i < topk; i += 32) out[i] = -1;
-}
-
-// One row settled by 32-bit scores s[0..live): returns false when the row is
-// too close to call. `err` bounds the error of every score.
-__device__ __forceinline__ bool sel_row_fast(const float* s, int live, int topk, int forced, int own, int keep_first,
-                                             float err, int* out) {
-  const int lane = threadIdx.x & 31;
-  const int want = topk - forced;  // among the blocks that are not forced
-  const int rest = live - forced;
-  if (want >= rest) {
-    sel_write(out, live, topk, [](int) { return true; });
-    return true;
+  __device__ __forceinline__ unsigned add(unsigned v) {
+    return join(__reduce_add_sync(0xffffffffu, v), [](unsigned a, unsigned b) { return a + b; });
   }
+  __device__ __forceinline__ unsigned min(unsigned v) {
+    return join(__reduce_min_sync(0xffffffffu, v), [](unsigned a, unsigned b) { return a < b ? a : b; });
+  }
+  __device__ __forceinline__ unsigned max(unsigned v) {
+    return join(__reduce_max_sync(0xffffffffu, v), [](unsigned a, unsigned b) { return a > b ? a : b; });
+  }
+};
+
+// Keys of a row over its threads: PER in registers, or (PER = 0) images of the
+// scores made anew at each visit. Thread t holds blocks t, t + N, ...
+template <typename G, int PER>
+struct SelKeys {
+  uint32_t k[PER ? PER : 1];
+  const float* s;
+  const SelRow& r;
+  int id;
+  __device__ __forceinline__ uint32_t image(int j) const { return j < r.live && !r.is_forced(j) ? sel_key(s[j]) : 0u; }
+  __device__ __forceinline__ SelKeys(const float* s_, const SelRow& r_, int id_) : s(s_), r(r_), id(id_) {
+    if (PER)
+#pragma unroll
+      for (int x = 0; x < PER; ++x) k[x] = image(id + x * G::N);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if (PER) {
+#pragma unroll
+      for (int x = 0; x < PER; ++x) f(k[x], id + x * G::N);
+    } else {
+      for (int j = id; j < r.live; j += G::N) f(image(j), j);
+    }
+  }
+};
+
+enum SelCase { SEL_DONE, SEL_BAND, SEL_ALL };
+
+// Where a row stands by its 32-bit scores (each within `err` of its 64-bit
+// value). SEL_DONE: kept are the forced blocks and keys >= lo. SEL_BAND: kept
+// for certain are keys > hi, certainly dropped keys < lo; `sure` counts the
+// former, `band` the keys between, from which the rest is chosen in 64 bits.
+// SEL_ALL: a score is not finite or the band is long; everything in 64 bits.
+template <typename G, int PER>
+__device__ __forceinline__ SelCase sel_place(G& g, const SelKeys<G, PER>& keys, const SelRow& r, float err,
+                                             uint32_t& lo, uint32_t& hi, int& sure, int& band) {
+  const int want = r.want();
+  lo = 1;
+  hi = 0xffffffffu;
+  if (want >= r.live - r.forced) return SEL_DONE;
   if (want <= 0) {
-    sel_write(out, live, topk, [&](int j) { return sel_forced(j, own, keep_first); });
-    return true;
+    lo = 0xffffffffu;
+    return SEL_DONE;
   }
-  bool odd = false;
-  for (int j = lane; j < live; j += 32) odd |= !isfinite(s[j]) && !sel_forced(j, own, keep_first);
-  if (__any_sync(0xffffffffu, odd) || !isfinite(err)) return false;
-  // largest threshold that at least `want` scores reach, bit by bit; done as
-  // soon as exactly `want` of them do
-  uint32_t t = 0;
+  uint32_t most = 0, least = 0xffffffffu;
+  keys.each([&](uint32_t k, int) {
+    if (k) {
+      most = k > most ? k : most;
+      least = k < least ? k : least;
+    }
+  });
+  most = g.max(most);
+  least = g.min(least);
+  if (!(most < sel_key(INFINITY) && least > sel_key(-INFINITY)) || !isfinite(err)) return SEL_ALL;
+  // the largest threshold that `want` keys reach, bit by bit below the common
+  // leading bits; done as soon as exactly `want` keys do
+  const int top = 31 - __clz(most ^ least);  // -1: all keys equal
+  uint32_t t = top < 0 ? least : most & ~((2u << top) - 1u);
   bool exact = false;
-  for (int bit = 31; bit >= 0 && !exact; --bit) {
+  for (int bit = top; bit >= 0 && !exact; --bit) {
     const uint32_t cand = t | (1u << bit);
     unsigned c = 0;
-    for (int j = lane; j < live; j += 32) c += !sel_forced(j, own, keep_first) && sel_key(s[j]) >= cand;
-    c = __reduce_add_sync(0xffffffffu, c);
+    keys.each([&](uint32_t k, int) { c += k >= cand; });
+    c = g.add(c);
     if (c >= (unsigned)want) t = cand;
     exact = c == (unsigned)want;
   }
-  // the smallest kept and the largest dropped score
-  uint32_t lo = 0xffffffffu, hi = 0;
+  // the smallest kept and the largest dropped key
+  uint32_t kept = 0xffffffffu, dropped = 0;
   unsigned c = 0;
-  for (int j = lane; j < live; j += 32) {
-    if (sel_forced(j, own, keep_first)) continue;
-    const uint32_t k = sel_key(s[j]);
+  keys.each([&](uint32_t k, int) {
     if (k >= t) {
-      lo = k < lo ? k : lo;
+      kept = k < kept ? k : kept;
       ++c;
     } else {
-      hi = k > hi ? k : hi;
+      dropped = k > dropped ? k : dropped;
     }
+  });
+  kept = g.min(kept);
+  dropped = g.max(dropped);
+  c = g.add(c);
+  const float kf = sel_unkey(kept);
+  if (c == (unsigned)want && kf - sel_unkey(dropped) > 2.f * err) {
+    lo = kept;
+    return SEL_DONE;
   }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  c = __reduce_add_sync(0xffffffffu, c);
-  if (c != (unsigned)want) return false;  // equal scores at the border
-  if (!(sel_unkey(lo) - sel_unkey(hi) > 2.f * err)) return false;
-  sel_write(out, live, topk, [&](int j) { return sel_forced(j, own, keep_first) || sel_key(s[j]) >= t; });
-  return true;
+  // the want-th largest 64-bit score lies within err of kf
+  lo = sel_key(kf - 2.1f * err);
+  hi = sel_key(kf + 2.1f * err);
+  unsigned over = 0, in = 0;
+  keys.each([&](uint32_t k, int) {
+    over += k > hi;
+    in += k >= lo && k <= hi;
+  });
+  sure = (int)g.add(over);
+  band = (int)g.add(in);
+  return band <= 32 ? SEL_BAND : SEL_ALL;
 }
 
-// One row in 64 bits: s holds the scores; a taken block is marked by NaN.
-__device__ __forceinline__ void sel_row_exact(double* s, int live, int topk, int forced, int own, int keep_first,
-                                              int* out) {
+// 64-bit score of block j, by a warp: lanes over the channels.
+template <typename T>
+__device__ __forceinline__ double sel_score64(const SelArgs& a, const T* q, const float* mean) {
+  double s = 0.0;
+  for (int d = threadIdx.x & 31; d < a.dim; d += 32) {
+    double x = 0.0;
+    for (int g = 0; g < a.group; ++g) x += (double)rot_f32(q[g * a.q.h + d]);
+    s += x * (double)mean[d];
+  }
+  for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+  return isnan(s) ? -INFINITY : s;
+}
+
+// SEL_BAND by a warp: `members` (shared, ascending, n of them) hold the band's
+// blocks; returns the mask of those that are kept: the `need` largest 64-bit
+// scores, ties to the lowest index.
+template <typename T>
+__device__ __forceinline__ uint32_t sel_band(const SelArgs& a, const T* q, const float* means, const int* members, int n,
+                                             int need) {
   const int lane = threadIdx.x & 31;
-  const int want = min(topk, live) - forced;
-  for (int r = 0; r < want; ++r) {
+  double mine = 0.0;
+  for (int c = 0; c < n; ++c) {
+    const double s = sel_score64(a, q, means + (long long)members[c] * a.dim);
+    if (lane == c) mine = s;
+  }
+  int rank = 0;
+  for (int c = 0; c < n; ++c) {
+    const double o = __shfl_sync(0xffffffffu, mine, c);
+    rank += o > mine || (o == mine && c < lane);
+  }
+  return __ballot_sync(0xffffffffu, lane < n && rank < need);
+}
+
+// Writes kept blocks among [j0, j1) in ascending order from place n on, by a
+// warp; returns the next place.
+template <typename F>
+__device__ __forceinline__ int sel_write(int* out, int j0, int j1, int n, int topk, F kept) {
+  const int lane = threadIdx.x & 31;
+  for (; j0 < j1; j0 += 32) {
+    const int j = j0 + lane;
+    const bool k = j < j1 && kept(j);
+    const uint32_t m = __ballot_sync(0xffffffffu, k);
+    const int at = n + __popc(m & ((1u << lane) - 1u));
+    if (out && k && at < topk) out[at] = j;
+    n += __popc(m);
+  }
+  return n;
+}
+__device__ __forceinline__ void sel_fill(int* out, int n, int topk) {
+  for (int i = n + (threadIdx.x & 31); i < topk; i += 32) out[i] = -1;
+}
+
+// A row of 64-bit scores s (a taken block is marked by NaN), by a warp.
+__device__ __forceinline__ void sel_row_exact(double* s, const SelRow& r, int* out) {
+  const int lane = threadIdx.x & 31;
+  const int want = min(r.topk, r.live) - r.forced;
+  for (int x = 0; x < want; ++x) {
     double best = 0.0;
     int at = 0x7fffffff;
-    for (int j = lane; j < live; j += 32)
-      if (!sel_forced(j, own, keep_first) && !isnan(s[j]) && (at == 0x7fffffff || s[j] > best)) {
+    for (int j = lane; j < r.live; j += 32)
+      if (!r.is_forced(j) && !isnan(s[j]) && (at == 0x7fffffff || s[j] > best)) {
         best = s[j];
         at = j;
       }
@@ -197,29 +352,180 @@ __device__ __forceinline__ void sel_row_exact(double* s, int live, int topk, int
     if (at != 0x7fffffff && lane == 0) s[at] = __longlong_as_double(0x7ff8000000000000ll);
     __syncwarp();
   }
-  sel_write(out, live, topk, [&](int j) { return sel_forced(j, own, keep_first) || isnan(s[j]); });
+  const int n = sel_write(out, 0, r.live, 0, r.topk, [&](int j) { return r.is_forced(j) || isnan(s[j]); });
+  sel_fill(out, n, r.topk);
 }
 
-// Shared memory: scores [tile][nb] fp32 (later reused as 64-bit scores, one
-// row per warp), the tile's summed queries (rows padded to 16 bytes plus 16) fp32, their 1-norms,
-// a mean chunk with the same rows, the redo list.
+// One row by a warp from its 32-bit scores; false: all of it in 64 bits.
+template <typename T, int PER>
+__device__ __forceinline__ bool sel_row_fast(const SelArgs& a, const float* s, const SelRow& r, float err, const T* q,
+                                             const float* means, int* members, int* out) {
+  SelWarp g;
+  SelKeys<SelWarp, PER> keys(s, r, g.id());
+  uint32_t lo, hi;
+  int sure = 0, band = 0;
+  const SelCase c = sel_place(g, keys, r, err, lo, hi, sure, band);
+  if (c == SEL_ALL) return false;
+  uint32_t won = 0;
+  if (c == SEL_BAND) {
+    sel_write(members, 0, r.live, 0, 32, [&](int j) {
+      const uint32_t k = keys.image(j);
+      return k >= lo && k <= hi;
+    });
+    __syncwarp();
+    won = sel_band(a, q, means, members, band, r.want() - sure);
+    __syncwarp();
+    if (g.id() < band && !(won >> g.id() & 1)) members[g.id()] = -1;
+    __syncwarp();
+  }
+  int seen = 0;  // band members before this lane's chunk: they come in the same ascending order
+  int n = 0;
+  const int lane = g.id();
+  for (int j0 = 0; j0 < r.live; j0 += 32) {
+    const int j = j0 + lane;
+    const uint32_t k = keys.image(j);
+    bool kept = j < r.live && (r.is_forced(j) || (c == SEL_BAND ? k > hi : k >= lo));
+    if (c == SEL_BAND) {
+      const bool in = k >= lo && k <= hi;
+      const uint32_t m = __ballot_sync(0xffffffffu, in);
+      if (in) kept = members[seen + __popc(m & ((1u << lane) - 1u))] >= 0;
+      seen += __popc(m);
+    }
+    const uint32_t m = __ballot_sync(0xffffffffu, kept);
+    const int at = n + __popc(m & ((1u << lane) - 1u));
+    if (kept && at < r.topk) out[at] = j;
+    n += __popc(m);
+  }
+  sel_fill(out, n, r.topk);
+  __syncwarp();
+  return true;
+}
+
+// Four rows by a warp, eight lanes a row, keys in registers (live <= 8 PER).
+// Lanes of a row whose 32-bit scores settle it write it; returns whether this
+// lane's row is settled. `on`: this lane's row exists.
+template <int PER>
+__device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, float err, bool on, int* out) {
+  const int lane = threadIdx.x & 31, id = lane & 7, shift = lane & 24;
+  const int want = r.want();
+  uint32_t k[PER];
+  uint32_t most = 0, least = 0xffffffffu;
+#pragma unroll
+  for (int x = 0; x < PER; ++x) {
+    const int j = id + 8 * x;
+    k[x] = on && j < r.live && !r.is_forced(j) ? sel_key(s[j]) : 0u;
+    most = max(most, k[x]);
+    least = min(least, k[x] ? k[x] : 0xffffffffu);
+  }
+#pragma unroll
+  for (int m = 1; m < 8; m <<= 1) {
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
+    least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
+  }
+  const bool all = want >= r.live - r.forced, none = want <= 0;
+  bool settled = true;
+  uint32_t t = all ? 1u : 0xffffffffu;  // kept: keys >= t
+  const bool search = on && !all && !none;
+  if (search && (!(most < sel_key(INFINITY) && least > sel_key(-INFINITY)) || !isfinite(err))) settled = false;
+  bool busy = search && settled;
+  int bit = 31 - __clz(most ^ least);  // -1: all keys equal
+  if (busy) t = bit < 0 ? least : most & ~((2u << bit) - 1u);
+  while (__any_sync(0xffffffffu, busy && bit >= 0)) {
+    const bool step = busy && bit >= 0;
+    const uint32_t cand = t | (1u << (bit & 31));
+    int c = 0;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) c += k[x] >= cand;
+#pragma unroll
+    for (int m = 1; m < 8; m <<= 1) c += __shfl_xor_sync(0xffffffffu, c, m);
+    if (step) {
+      if (c >= want) t = cand;
+      bit = c == want ? -1 : bit - 1;
+    }
+  }
+  uint32_t kept = 0xffffffffu, dropped = 0;
+  int c = 0;
+#pragma unroll
+  for (int x = 0; x < PER; ++x) {
+    const bool in = k[x] >= t;
+    kept = in ? min(kept, k[x]) : kept;
+    dropped = in ? dropped : max(dropped, k[x]);
+    c += in;
+  }
+#pragma unroll
+  for (int m = 1; m < 8; m <<= 1) {
+    kept = min(kept, __shfl_xor_sync(0xffffffffu, kept, m));
+    dropped = max(dropped, __shfl_xor_sync(0xffffffffu, dropped, m));
+    c += __shfl_xor_sync(0xffffffffu, c, m);
+  }
+  if (busy) settled = c == want && sel_unkey(kept) - sel_unkey(dropped) > 2.f * err;
+  const bool write = on && settled;
+  int n = 0;
+#pragma unroll
+  for (int x = 0; x < PER; ++x) {
+    const int j = id + 8 * x;
+    const bool in = j < r.live && (k[x] ? k[x] >= t : r.is_forced(j));
+    const uint32_t m = __ballot_sync(0xffffffffu, in) >> shift & 0xffu;
+    const int at = n + __popc(m & ((1u << id) - 1u));
+    if (write && in && at < r.topk) out[at] = j;
+    n += __popc(m);
+  }
+  if (write)
+    for (int x = n + id; x < r.topk; x += 8) out[x] = -1;
+  return settled;
+}
+
+// Shared memory of a CTA:
+//   scores [tile][stride] fp32, later 64-bit scores, one row a warp
+//   summed queries [2][tile][dp + 8] and a chunk of means [2][64][dp + 8] as
+//   bf16 pairs (x = hi + mid + rest, |rest| <= 2^-18 |x|), their 2-norms
+//   two lists of rows left to do
+// stride: an odd multiple of 8 (four rows' octets meet distinct banks); rows of
+// dp + 8: an odd number of 16-byte chunks, so ldmatrix meets every bank once.
+__host__ __device__ inline int sel_stride(int nb) { return ((nb + 7) / 8 | 1) * 8; }
+__host__ __device__ inline int sel_dp(int dim) { return (dim + 15) / 16 * 16; }
 __host__ __device__ inline int sel_smem_bytes(int tile, int nb, int dim) {
-  const int scores = tile * (nb + (nb & 1)) * 4;
-  const int ds = (dim + 3) / 4 * 4 + 4;
-  return scores + tile * ds * 4 + kSelChunk * ds * 4 + tile * 8;
+  return tile * sel_stride(nb) * 4 + 2 * (max(tile, 16) + kSelChunk) * (sel_dp(dim) + 8) * 2 + tile * 12;
 }
 
-template <typename T>
+// Error of a 32-bit score, relative to ||q|| ||mean|| (||q||: of the sums of the
+// heads' magnitudes). Matrix form: three products of bf16 pairs lose mid mid and
+// both rests, 3 2^-18 with the rounding of the parts, and the sums of 3 dp / 16
+// steps 2^-22 each. Plain form (few queries): products are added four at a time
+// and the groups in turn, D / 4 + group + 6 roundings. Both with some to spare.
+__device__ __forceinline__ float sel_unit_mma(const SelArgs& a) {
+  return 3.5f * 3.8146973e-6f + (float)(3 * a.dim / 16 + a.group + 16) * 2.3841858e-7f;
+}
+__device__ __forceinline__ float sel_unit(const SelArgs& a) {
+  return (float)(a.dim / 4 + a.group + 12) * 5.9604645e-8f;
+}
+
+// x as bf16 hi + mid, eight channels to 16 bytes each.
+__device__ __forceinline__ void sel_split8(const float (&x)[8], __nv_bfloat16* hi, __nv_bfloat16* mid) {
+  RotVec<__nv_bfloat16, 8> h, m;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    h.v[e] = __float2bfloat16_rn(x[e]);
+    m.v[e] = __float2bfloat16_rn(x[e] - __bfloat162float(h.v[e]));
+  }
+  *reinterpret_cast<RotVec<__nv_bfloat16, 8>*>(hi) = h;
+  *reinterpret_cast<RotVec<__nv_bfloat16, 8>*>(mid) = m;
+}
+
+// PER > 0: rows of up to 8 PER blocks, settled four a warp; 0: a warp a row.
+template <typename T, int PER>
 __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs a) {
   extern __shared__ __align__(16) char sel_smem[];
-  const int D = a.dim, DS = (D + 3) / 4 * 4 + 4, NBS = a.nb + (a.nb & 1), TQ = a.tile;
+  const int D = a.dim, DP = sel_dp(D), RS = DP + 8, NBS = sel_stride(a.nb), TQ = a.tile, TQ16 = max(TQ, 16);
   float* sc = reinterpret_cast<float*>(sel_smem);
-  float* qs = sc + TQ * NBS;
-  float* ms = qs + TQ * DS;
-  float* q1 = ms + kSelChunk * DS;
-  int* redo = reinterpret_cast<int*>(q1 + TQ);
-  __shared__ int redo_n;
+  __nv_bfloat16* qhi = reinterpret_cast<__nv_bfloat16*>(sc + TQ * NBS);
+  __nv_bfloat16 *qmid = qhi + TQ16 * RS, *mhi = qmid + TQ16 * RS, *mmid = mhi + kSelChunk * RS;
+  float* qn = reinterpret_cast<float*>(mmid + kSelChunk * RS);
+  int* todo = reinterpret_cast<int*>(qn + TQ);
+  int* redo = todo + TQ;
+  __shared__ int todo_n, redo_n;
   __shared__ uint32_t mmax_bits;
+  __shared__ int members[kSelWarps][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long u = blockIdx.x;
   const int tile = (int)(u % a.tiles);
@@ -235,95 +541,146 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   int* out = a.out + (bh * a.q_rows + i0) * a.topk;
   const float* means = a.means + bh * a.nb * D;
   if (tid == 0) {
-    redo_n = 0;
+    todo_n = redo_n = 0;
     mmax_bits = 0;
   }
   for (int i = tid; i < (nq - nl) * a.topk; i += kSelThreads) out[(long long)nl * a.topk + i] = -1;
   if (nl == 0) return;
 
-  // the group's summed queries and the 1-norm over all of their terms
+  // the group's summed queries as bf16 pairs, and the 2-norms of the sums of
+  // magnitudes; four or more threads a row, eight channels a step
   const T* qb = (const T*)a.q.p + b * a.q.b + (long long)h * a.group * a.q.h + (long long)i0 * a.q.s;
-  for (int r = warp; r < nl; r += kSelWarps) {
-    float n1 = 0.f;
-    for (int d = lane; d < D; d += 32) {
-      float s = 0.f;
-      for (int g = 0; g < a.group; ++g) {
-        const float v = rot_f32(qb[g * a.q.h + r * a.q.s + d]);
-        s += v;
-        n1 += fabsf(v);
-      }
-      qs[r * DS + d] = s;
+  const bool q_wide = a.q_vec != 0;
+  const int tpr = min(32, kSelThreads / TQ16);
+  for (int r = tid / tpr; r < TQ16; r += kSelThreads / tpr) {
+    float n2 = 0.f;
+    for (int c = (tid % tpr) * 8; c < DP; c += tpr * 8) {
+      float x[8], m[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = m[e] = 0.f;
+      if (r < nl)
+        for (int g = 0; g < a.group; ++g) {
+          const T* src = qb + g * a.q.h + r * a.q.s + c;
+          float v[8];
+          if (q_wide) {  // D is a multiple of 8, rows are 16-byte aligned
+            constexpr int V = 16 / sizeof(T);
+#pragma unroll
+            for (int y = 0; y < 8 / V; ++y) {
+              const RotVec<T, V> w = c < D ? *reinterpret_cast<const RotVec<T, V>*>(src + y * V) : RotVec<T, V>{};
+#pragma unroll
+              for (int e = 0; e < V; ++e) v[y * V + e] = rot_f32(w.v[e]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < D ? rot_f32(src[e]) : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] += v[e];
+            m[e] += fabsf(v[e]);
+          }
+        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n2 += m[e] * m[e];
+      sel_split8(x, qhi + r * RS + c, qmid + r * RS + c);
     }
-    for (int m = 16; m; m >>= 1) n1 += __shfl_xor_sync(0xffffffffu, n1, m);
-    if (lane == 0) q1[r] = n1;
+    for (int m = 1; m < tpr; m <<= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, m);
+    if (tid % tpr == 0 && r < TQ) qn[r] = sqrtf(n2 + kSelTiny);
   }
-  float mm = 0.f;
+  const bool m_wide = D % 4 == 0 && ((uintptr_t)means & 15) == 0;
   for (int j0 = 0; j0 < live; j0 += kSelChunk) {
     const int nj = live - j0 < kSelChunk ? live - j0 : kSelChunk;
     __syncthreads();
-    for (int i = tid; i < nj * D; i += kSelThreads) {
-      const int r = i / D, d = i - r * D;
-      const float v = means[(long long)j0 * D + i];
-      ms[r * DS + d] = v;
-      mm = fmaxf(mm, fabsf(v));
-    }
-    __syncthreads();
-    // 4 queries x 4 blocks a thread: queries ty, ty + 16, ..., blocks tx, tx + 16, ...
-    const int tx = tid & 15, ty = tid >> 4;
-    for (int q0 = 0; q0 < nl; q0 += 64) {
-      float acc[4][4];
+    {
+      const int r = tid >> 2;  // four threads a mean
+      float n2 = 0.f;
+      for (int c = (tid & 3) * 8; c < DP; c += 32) {
+        float x[8];
+        const float* src = means + (long long)(j0 + r) * D + c;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+        for (int y = 0; y < 2; ++y) {
+          if (m_wide) {
+            const float4 v = r < nj && c + 4 * y < D ? *reinterpret_cast<const float4*>(src + 4 * y) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[4 * y] = v.x; x[4 * y + 1] = v.y; x[4 * y + 2] = v.z; x[4 * y + 3] = v.w;
+          } else {
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[x][y] = 0.f;
-      int d = 0;
-      for (; d + 4 <= D; d += 4) {
-        float4 qv[4], mv[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = q0 + ty + 16 * x;
-          qv[x] = *reinterpret_cast<const float4*>(qs + (r < nl ? r : 0) * DS + d);
-          mv[x] = *reinterpret_cast<const float4*>(ms + (tx + 16 * x < nj ? tx + 16 * x : 0) * DS + d);
+            for (int e = 4 * y; e < 4 * y + 4; ++e) x[e] = r < nj && c + e < D ? src[e] : 0.f;
+          }
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            acc[x][y] += qv[x].x * mv[y].x + qv[x].y * mv[y].y + qv[x].z * mv[y].z + qv[x].w * mv[y].w;
+        for (int e = 0; e < 8; ++e) n2 += x[e] * x[e];
+        sel_split8(x, mhi + r * RS + c, mmid + r * RS + c);
       }
-      for (; d < D; ++d)
+      n2 += __shfl_xor_sync(0xffffffffu, n2, 1);
+      n2 += __shfl_xor_sync(0xffffffffu, n2, 2);
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(n2 >= 0.f ? n2 + kSelTiny : INFINITY));
+      if (lane == 0) atomicMax(&mmax_bits, bits);  // values >= 0: bits order as they do
+    }
+    __syncthreads();
+    // units of 16 queries x 32 blocks: hi hi + hi mid + mid hi
+    for (int unit = warp; unit < TQ16 / 16 * 2; unit += kSelWarps) {
+      const int r0 = unit / 2 * 16, c0 = unit % 2 * 32;
+      if (r0 >= nl || c0 >= nj) continue;
+      float acc[4][4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int r = q0 + ty + 16 * x, c = tx + 16 * y;
-            acc[x][y] += qs[(r < nl ? r : 0) * DS + d] * ms[(c < nj ? c : 0) * DS + d];
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+      for (int kk = 0; kk < DP; kk += 16) {
+        uint32_t ah[4], am[4];
+        const int qa = (r0 + (lane & 15)) * RS + kk + (lane >> 4) * 8;
+        ldmatrix_x4(ah, smem_u32(qhi + qa));
+        ldmatrix_x4(am, smem_u32(qmid + qa));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t bh4[4], bm4[4];
+          const int ma = (c0 + 16 * n + (lane & 7) + ((lane >> 4) << 3)) * RS + kk + ((lane >> 3) & 1) * 8;
+          ldmatrix_x4(bh4, smem_u32(mhi + ma));
+          ldmatrix_x4(bm4, smem_u32(mmid + ma));
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t bh2[2] = {bh4[2 * y], bh4[2 * y + 1]}, bm2[2] = {bm4[2 * y], bm4[2 * y + 1]};
+            MmaTraits<__nv_bfloat16>::mma(acc[2 * n + y], am, bh2);
+            MmaTraits<__nv_bfloat16>::mma(acc[2 * n + y], ah, bm2);
+            MmaTraits<__nv_bfloat16>::mma(acc[2 * n + y], ah, bh2);
           }
+        }
+      }
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int r = q0 + ty + 16 * x, c = tx + 16 * y;
-          if (r < nl && c < nj) sc[r * NBS + j0 + c] = acc[x][y];
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + (lane >> 2) + 8 * (e >> 1), c = c0 + 8 * n + 2 * (lane & 3) + (e & 1);
+          if (r < nl && c < nj) sc[r * NBS + j0 + c] = acc[n][e];
         }
     }
   }
-  for (int m = 16; m; m >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, m));
-  if (lane == 0) atomicMax(&mmax_bits, __float_as_uint(mm));  // mm >= 0: bits order as values
   __syncthreads();
-  // |fl(score) - score| <= (D + group + 2) 2^-24 (1 + small) sum |q| |mean|, and
-  // under 1e-40 more where products underflow
-  const float unit = (float)(D + a.group + 8) * 5.9604645e-8f * __uint_as_float(mmax_bits);
-  for (int r = warp; r < nl; r += kSelWarps) {
-    const int own = a.keep_own && (i0 + r) / a.block < live ? (i0 + r) / a.block : -1;
-    const int first = a.keep_first < live ? a.keep_first : live;
-    const int forced = first + (own >= first ? 1 : 0);
-    if (!sel_row_fast(sc + r * NBS, live, a.topk, forced, own, first, unit * q1[r] + 1e-40f, out + (long long)r * a.topk) &&
+  const float mmax = sqrtf(__uint_as_float(mmax_bits)), unit = sel_unit_mma(a) * mmax;
+  // parts below the smallest normal number may be lost: 1e-34 of the norms covers them
+  auto err_of = [&](int r) { return unit * qn[r] + 1e-34f * (mmax + qn[r]) + 1e-40f; };
+  if (PER > 0) {
+    for (int r0 = warp * 4; r0 < nl; r0 += kSelWarps * 4) {
+      const int r = r0 + (lane >> 3);
+      const bool on = r < nl;
+      const int rr = on ? r : 0;
+      const SelRow row(a, i0 + rr, live);
+      const bool done = sel_rows_oct<PER ? PER : 1>(sc + rr * NBS, row, err_of(rr), on, out + (long long)rr * a.topk);
+      if (on && !done && (lane & 7) == 0) todo[atomicAdd(&todo_n, 1)] = r;
+    }
+    __syncthreads();
+  }
+  const int rows = PER > 0 ? todo_n : nl;
+  for (int x = warp; x < rows; x += kSelWarps) {
+    const int r = PER > 0 ? todo[x] : x;
+    const SelRow row(a, i0 + r, live);
+    if (!sel_row_fast<T, 0>(a, sc + r * NBS, row, err_of(r), qb + r * a.q.s, means, members[warp],
+                            out + (long long)r * a.topk) &&
         lane == 0)
       redo[atomicAdd(&redo_n, 1)] = r;
   }
   __syncthreads();
-  // close rows: every score again in 64 bits, one row per warp in the scratch
+  // the remaining rows: every score in 64 bits, one row per warp in the scratch
   // that the 32-bit scores leave (a tile of two rows holds one 64-bit row)
   const int rn = redo_n;
   const int workers = TQ / 2 < kSelWarps ? TQ / 2 : kSelWarps;
@@ -331,24 +688,177 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   double* s64 = reinterpret_cast<double*>(sc) + (long long)warp * NBS;
   for (int x = warp; x < rn; x += workers) {
     const int r = redo[x];
-    for (int j = lane; j < live; j += 32) s64[j] = 0.0;
-    for (int j0 = 0; j0 < live; j0 += 32) {
-      const int j = j0 + lane;
-      double acc = 0.0;
-      for (int d = 0; d < D; ++d) {
-        double qd = 0.0;
-        for (int g = 0; g < a.group; ++g) qd += (double)rot_f32(qb[g * a.q.h + r * a.q.s + d]);
-        if (j < live) acc += qd * (double)means[(long long)j * D + d];
-      }
-      if (j < live) s64[j] = isnan(acc) ? -INFINITY : acc;
+    for (int j = 0; j < live; ++j) {
+      const double s = sel_score64(a, qb + r * a.q.s, means + (long long)j * D);
+      if (lane == 0) s64[j] = s;
     }
     __syncwarp();
-    const int own = a.keep_own && (i0 + r) / a.block < live ? (i0 + r) / a.block : -1;
-    const int first = a.keep_first < live ? a.keep_first : live;
-    const int forced = first + (own >= first ? 1 : 0);
-    sel_row_exact(s64, live, a.topk, forced, own, first, out + (long long)r * a.topk);
+    sel_row_exact(s64, SelRow(a, i0 + r, live), out + (long long)r * a.topk);
     __syncwarp();
   }
+}
+
+// ---- selection, few queries ---------------------------------------------------
+// A cluster of CTAs per row: every CTA scores its share of the blocks straight
+// from global memory (a warp reads whole mean rows, eight in flight) into the
+// shared memory of the cluster's first CTA, which settles the row with all of
+// its threads. Bound by the read of the means.
+constexpr int kSelFewCluster = 8;
+
+__host__ __device__ inline int sel_few_smem_bytes(int nb) { return (nb + (nb & 1)) * 12; }
+
+template <typename T, int PER>
+__global__ __launch_bounds__(kSelThreads) void block_select_few_kernel(const SelArgs a) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ __align__(16) char sel_smem[];
+  float* sc = reinterpret_cast<float*>(sel_smem);                                        // [nb], CTA 0's
+  double* s64 = reinterpret_cast<double*>(sel_smem + (size_t)(a.nb + (a.nb & 1)) * 4);  // [nb], CTA 0's
+  __shared__ __align__(16) float qs[kSelMaxDim];
+  __shared__ unsigned red[2 * kSelWarps];
+  __shared__ uint32_t mmax_bits;  // CTA 0's
+  __shared__ int members[32], counts[kSelWarps];
+  __shared__ uint32_t won_sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const long long u = blockIdx.x / C;
+  const int i = (int)(u % a.q_rows);
+  const long long bh = u / a.q_rows;
+  const int b = (int)(bh / a.kv_heads), h = (int)(bh - (long long)b * a.kv_heads);
+  int kv = a.kv_lens ? a.kv_lens[b] : a.kv_rows;
+  kv = kv < 0 ? 0 : kv > a.kv_rows ? a.kv_rows : kv;
+  const bool on = !a.q_lens || i < a.q_lens[b];
+  const int D = a.dim, live = on ? (kv + a.block - 1) / a.block : 0;
+  const T* q = (const T*)a.q.p + b * a.q.b + (long long)h * a.group * a.q.h + (long long)i * a.q.s;
+  const float* means = a.means + bh * a.nb * D;
+  if (tid == 0) mmax_bits = 0;
+  float n2 = 0.f;
+  for (int d = tid; d < D; d += kSelThreads) {
+    float s = 0.f, m = 0.f;
+    for (int g = 0; g < a.group; ++g) {
+      const float v = rot_f32(q[g * a.q.h + d]);
+      s += v;
+      m += fabsf(v);
+    }
+    qs[d] = s;
+    n2 += m * m;
+  }
+  cluster.sync();  // CTA 0's maximum is set to zero
+  float* sc0 = cluster.map_shared_rank(sc, 0);
+  uint32_t* mm0 = cluster.map_shared_rank(&mmax_bits, 0);
+  float mx = 0.f;
+  if (D % 4 == 0 && ((uintptr_t)means & 15) == 0) {
+    // LB lanes a mean row (16 bytes a lane and step), 32 / LB rows a warp and step
+    int LB = 1;
+    while (LB < 32 && LB * 4 < D) LB <<= 1;
+    const int per = 32 / LB, sub = lane / LB, l = lane % LB;
+    const int stride = C * kSelWarps * per;
+    for (int j0 = (rank * kSelWarps + warp) * per; j0 < live; j0 += 8 * stride) {
+      float dot[8], nn[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) dot[x] = nn[x] = 0.f;
+      for (int d = l * 4; d < D; d += LB * 4) {
+        float4 m[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int j = j0 + sub + x * stride;
+          m[x] = j < live ? *reinterpret_cast<const float4*>(means + (long long)j * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float4 v = *reinterpret_cast<const float4*>(qs + d);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          dot[x] += fmaf(v.w, m[x].w, fmaf(v.z, m[x].z, fmaf(v.y, m[x].y, v.x * m[x].x)));
+          nn[x] += fmaf(m[x].w, m[x].w, fmaf(m[x].z, m[x].z, fmaf(m[x].y, m[x].y, m[x].x * m[x].x)));
+        }
+      }
+      for (int m = 1; m < LB; m <<= 1) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          dot[x] += __shfl_xor_sync(0xffffffffu, dot[x], m);
+          nn[x] += __shfl_xor_sync(0xffffffffu, nn[x], m);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int j = j0 + sub + x * stride;
+        if (l == 0 && j < live) sc0[j] = dot[x];
+        mx = fmaxf(mx, nn[x] >= 0.f ? nn[x] + kSelTiny : INFINITY);
+      }
+    }
+  } else {
+    for (int j = rank * kSelWarps + warp; j < live; j += C * kSelWarps) {
+      float dot = 0.f, nn = 0.f;
+      for (int d = lane; d < D; d += 32) {
+        const float m = means[(long long)j * D + d];
+        dot += qs[d] * m;
+        nn += m * m;
+      }
+      for (int m = 16; m; m >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, m);
+        nn += __shfl_xor_sync(0xffffffffu, nn, m);
+      }
+      if (lane == 0) sc0[j] = dot;
+      mx = fmaxf(mx, nn >= 0.f ? nn + kSelTiny : INFINITY);
+    }
+  }
+  for (int m = 16; m; m >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+  if (lane == 0) atomicMax(mm0, __float_as_uint(mx));
+  cluster.sync();
+  if (rank != 0) return;
+
+  SelCta g{red};
+  for (int m = 16; m; m >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, m);
+  n2 = __uint_as_float(g.join(__float_as_uint(n2), [](unsigned x, unsigned y) {
+    return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+  }));
+  const float err = sel_unit(a) * sqrtf(__uint_as_float(mmax_bits)) * sqrtf(n2 + kSelTiny) + 1e-40f;
+  const SelRow row(a, i, live);
+  int* out = a.out + (bh * a.q_rows + i) * a.topk;
+  SelKeys<SelCta, PER> keys(sc, row, tid);
+  uint32_t lo, hi;
+  int sure = 0, band = 0;
+  const SelCase c = sel_place(g, keys, row, err, lo, hi, sure, band);
+  if (c == SEL_ALL) {
+    for (int j = warp; j < live; j += kSelWarps) {
+      const double s = sel_score64(a, q, means + (long long)j * D);
+      if (lane == 0) s64[j] = s;
+    }
+    __syncthreads();
+    if (warp == 0) sel_row_exact(s64, row, out);
+    return;
+  }
+  // each warp writes a range of blocks; the warps' counts give the places
+  const int span = ((live + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int j0 = min(live, warp * span), j1 = min(live, j0 + span);
+  if (c == SEL_BAND) {
+    if (warp == 0) {
+      sel_write(members, 0, live, 0, 32, [&](int j) {
+        const uint32_t k = keys.image(j);
+        return k >= lo && k <= hi;
+      });
+      __syncwarp();
+      const uint32_t won = sel_band(a, q, means, members, band, row.want() - sure);
+      if (lane == 0) won_sh = won;
+    }
+    __syncthreads();
+  }
+  auto kept = [&](int j) {
+    if (row.is_forced(j)) return true;
+    const uint32_t k = keys.image(j);
+    if (c != SEL_BAND) return k >= lo;
+    if (k > hi) return true;
+    if (k < lo) return false;
+    for (int x = 0; x < band; ++x)
+      if (members[x] == j) return (won_sh >> x & 1) != 0;
+    return false;
+  };
+  const int mine = sel_write(nullptr, j0, j1, 0, a.topk, kept);
+  if (lane == 0) counts[warp] = mine;
+  __syncthreads();
+  int n = 0;
+  for (int w = 0; w < warp; ++w) n += counts[w];
+  n = sel_write(out, j0, j1, n, a.topk, kept);
+  if (warp == kSelWarps - 1) sel_fill(out, n, a.topk);
 }
 
 }  // namespace sb
