@@ -580,9 +580,11 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
     if (dtype == SB_F16) return launch_select_few<__half>(a, (unsigned)rows, cluster, st);
     return launch_select_few<__nv_bfloat16>(a, (unsigned)rows, cluster, st);
   }
-  // the widest tile whose scores leave room for two CTAs an SM
-  int tile = 64;
-  while (tile > 2 && (sel_smem_bytes(tile, a.nb, head_dim) > 100 * 1024 || tile / 2 >= q_rows)) tile >>= 1;
+  // the widest tile whose scores leave room for two CTAs an SM (four where short
+  // rows make a row's own work small against the CTA's), no wider than the rows
+  int tile = 128;
+  while (tile > 64 && (sel_smem_bytes(tile, a.nb, head_dim) > 56 * 1024 || tile / 2 >= q_rows)) tile >>= 1;
+  while (tile > 2 && (sel_smem_bytes(tile, a.nb, head_dim) > 112 * 1024 || tile / 2 >= q_rows)) tile >>= 1;
   a.tile = tile;
   a.tiles = (int)cdiv(q_rows, tile);
   const long long grid = (long long)batch * kv_heads * a.tiles;

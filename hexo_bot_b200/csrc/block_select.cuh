@@ -232,11 +232,24 @@ __device__ __forceinline__ SelCase sel_place(G& g, const SelKeys<G, PER>& keys, 
   most = g.max(most);
   least = g.min(least);
   if (!(most < sel_key(INFINITY) && least > sel_key(-INFINITY)) || !isfinite(err)) return SEL_ALL;
-  // the largest threshold that `want` keys reach, bit by bit below the common
-  // leading bits; done as soon as exactly `want` keys do
+  // a threshold that exactly `want` keys reach, by halving the range of the
+  // scores; where that fails (scores that agree in most of their bits) the
+  // largest one that at least `want` keys reach, bit by bit
   const int top = 31 - __clz(most ^ least);  // -1: all keys equal
   uint32_t t = top < 0 ? least : most & ~((2u << top) - 1u);
   bool exact = false;
+  float f0 = sel_unkey(least), f1 = sel_unkey(most);
+  for (int step = 0; step < 16 && !exact; ++step) {
+    const float mid = 0.5f * f0 + 0.5f * f1;
+    const uint32_t cand = sel_key(mid);
+    unsigned c = 0;
+    keys.each([&](uint32_t k, int) { c += k >= cand; });
+    c = g.add(c);
+    exact = c == (unsigned)want;
+    if (exact) t = cand;
+    if (c > (unsigned)want) f0 = mid;
+    else f1 = mid;
+  }
   for (int bit = top; bit >= 0 && !exact; --bit) {
     const uint32_t cand = t | (1u << bit);
     unsigned c = 0;
@@ -277,17 +290,43 @@ __device__ __forceinline__ SelCase sel_place(G& g, const SelKeys<G, PER>& keys, 
   return band <= 32 ? SEL_BAND : SEL_ALL;
 }
 
-// 64-bit score of block j, by a warp: lanes over the channels.
+// 64-bit scores of up to four blocks, by a warp: lanes over the channels.
 template <typename T>
-__device__ __forceinline__ double sel_score64(const SelArgs& a, const T* q, const float* mean) {
-  double s = 0.0;
+__device__ __forceinline__ void sel_score64(const SelArgs& a, const T* q, const float* (&mean)[4], double (&s)[4]) {
+#pragma unroll
+  for (int y = 0; y < 4; ++y) s[y] = 0.0;
+#pragma unroll 4
   for (int d = threadIdx.x & 31; d < a.dim; d += 32) {
+    float m[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) m[y] = mean[y] ? mean[y][d] : 0.f;
     double x = 0.0;
+#pragma unroll 4
     for (int g = 0; g < a.group; ++g) x += (double)rot_f32(q[g * a.q.h + d]);
-    s += x * (double)mean[d];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) s[y] += x * (double)m[y];
   }
-  for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-  return isnan(s) ? -INFINITY : s;
+  for (int m = 16; m; m >>= 1)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) s[y] += __shfl_xor_sync(0xffffffffu, s[y], m);
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    if (isnan(s[y])) s[y] = -INFINITY;
+}
+// All of a row's 64-bit scores, blocks j0, j0 + 4 step, ... to s, by a warp.
+template <typename T>
+__device__ __forceinline__ void sel_scores64(const SelArgs& a, const T* q, const float* means, int j0, int step, int live,
+                                             double* s) {
+  for (; j0 < live; j0 += 4 * step) {
+    const float* mean[4];
+    double v[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) mean[y] = j0 + y * step < live ? means + (long long)(j0 + y * step) * a.dim : nullptr;
+    sel_score64(a, q, mean, v);
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (mean[y] && (threadIdx.x & 31) == 0) s[j0 + y * step] = v[y];
+  }
 }
 
 // SEL_BAND by a warp: `members` (shared, ascending, n of them) hold the band's
@@ -298,9 +337,15 @@ __device__ __forceinline__ uint32_t sel_band(const SelArgs& a, const T* q, const
                                              int need) {
   const int lane = threadIdx.x & 31;
   double mine = 0.0;
-  for (int c = 0; c < n; ++c) {
-    const double s = sel_score64(a, q, means + (long long)members[c] * a.dim);
-    if (lane == c) mine = s;
+  for (int c = 0; c < n; c += 4) {
+    const float* mean[4];
+    double v[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) mean[y] = c + y < n ? means + (long long)members[c + y] * a.dim : nullptr;
+    sel_score64(a, q, mean, v);
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (lane == c + y) mine = v[y];
   }
   int rank = 0;
   for (int c = 0; c < n; ++c) {
@@ -401,70 +446,76 @@ __device__ __forceinline__ bool sel_row_fast(const SelArgs& a, const float* s, c
   return true;
 }
 
-// Four rows by a warp, eight lanes a row, keys in registers (live <= 8 PER).
+// Four rows by a warp, eight lanes a row, scores in registers (live <= 8 PER).
 // Lanes of a row whose 32-bit scores settle it write it; returns whether this
-// lane's row is settled. `on`: this lane's row exists.
+// lane's row is settled. `on`: this lane's row exists. The border is looked for
+// by halving the range of the scores until as many as wanted lie above.
 template <int PER>
 __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, float err, bool on, int* out) {
   const int lane = threadIdx.x & 31, id = lane & 7, shift = lane & 24;
   const int want = r.want();
-  uint32_t k[PER];
-  uint32_t most = 0, least = 0xffffffffu;
+  float v[PER];
+  float most = -INFINITY, least = INFINITY;
+  bool odd = !(err < INFINITY);
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
     const int j = id + 8 * x;
-    k[x] = on && j < r.live && !r.is_forced(j) ? sel_key(s[j]) : 0u;
-    most = max(most, k[x]);
-    least = min(least, k[x] ? k[x] : 0xffffffffu);
-  }
-#pragma unroll
-  for (int m = 1; m < 8; m <<= 1) {
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
-  }
-  const bool all = want >= r.live - r.forced, none = want <= 0;
-  bool settled = true;
-  uint32_t t = all ? 1u : 0xffffffffu;  // kept: keys >= t
-  const bool search = on && !all && !none;
-  if (search && (!(most < sel_key(INFINITY) && least > sel_key(-INFINITY)) || !isfinite(err))) settled = false;
-  bool busy = search && settled;
-  int bit = 31 - __clz(most ^ least);  // -1: all keys equal
-  if (busy) t = bit < 0 ? least : most & ~((2u << bit) - 1u);
-  while (__any_sync(0xffffffffu, busy && bit >= 0)) {
-    const bool step = busy && bit >= 0;
-    const uint32_t cand = t | (1u << (bit & 31));
-    int c = 0;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) c += k[x] >= cand;
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) c += __shfl_xor_sync(0xffffffffu, c, m);
-    if (step) {
-      if (c >= want) t = cand;
-      bit = c == want ? -1 : bit - 1;
+    v[x] = -INFINITY;  // blocks that do not compete are never above the border
+    if (j < r.live && !r.is_forced(j)) {
+      v[x] = s[j];
+      odd |= !(fabsf(v[x]) < INFINITY);
+      most = fmaxf(most, v[x]);
+      least = fminf(least, v[x]);
     }
   }
-  uint32_t kept = 0xffffffffu, dropped = 0;
-  int c = 0;
+  odd = (__ballot_sync(0xffffffffu, odd) >> shift & 0xffu) != 0;
+#pragma unroll
+  for (int m = 1; m < 8; m <<= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, m));
+  }
+  const bool all = want >= r.live - r.forced, search = on && !all && want > 0;
+  bool busy = search && !odd;
+  float t = 0.f;
+  bool exact = false;
+#pragma unroll 1
+  for (int step = 0; step < 26 && __any_sync(0xffffffffu, busy); ++step) {
+    const float mid = 0.5f * least + 0.5f * most;
+    int c = 0;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) c += v[x] >= mid;
+#pragma unroll
+    for (int m = 1; m < 8; m <<= 1) c += __shfl_xor_sync(0xffffffffu, c, m);
+    if (busy) {
+      if (c == want) {
+        exact = true;
+        busy = false;
+        t = mid;
+      }
+      if (c > want) least = mid;
+      else most = mid;
+    }
+  }
+  // the smallest kept and the largest dropped score
+  float kept = INFINITY, dropped = -INFINITY;
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
-    const bool in = k[x] >= t;
-    kept = in ? min(kept, k[x]) : kept;
-    dropped = in ? dropped : max(dropped, k[x]);
-    c += in;
+    const bool in = v[x] >= t;
+    kept = in ? fminf(kept, v[x]) : kept;
+    dropped = in ? dropped : fmaxf(dropped, v[x]);
   }
 #pragma unroll
   for (int m = 1; m < 8; m <<= 1) {
-    kept = min(kept, __shfl_xor_sync(0xffffffffu, kept, m));
-    dropped = max(dropped, __shfl_xor_sync(0xffffffffu, dropped, m));
-    c += __shfl_xor_sync(0xffffffffu, c, m);
+    kept = fminf(kept, __shfl_xor_sync(0xffffffffu, kept, m));
+    dropped = fmaxf(dropped, __shfl_xor_sync(0xffffffffu, dropped, m));
   }
-  if (busy) settled = c == want && sel_unkey(kept) - sel_unkey(dropped) > 2.f * err;
+  const bool settled = !search || (exact && kept - dropped > 2.f * err);
   const bool write = on && settled;
   int n = 0;
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
     const int j = id + 8 * x;
-    const bool in = j < r.live && (k[x] ? k[x] >= t : r.is_forced(j));
+    const bool in = j < r.live && (all || r.is_forced(j) || (search && v[x] >= t));
     const uint32_t m = __ballot_sync(0xffffffffu, in) >> shift & 0xffu;
     const int at = n + __popc(m & ((1u << id) - 1u));
     if (write && in && at < r.topk) out[at] = j;
@@ -478,7 +529,7 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
 // Shared memory of a CTA:
 //   scores [tile][stride] fp32, later 64-bit scores, one row a warp
 //   summed queries [2][tile][dp + 8] and a chunk of means [2][64][dp + 8] as
-//   bf16 pairs (x = hi + mid + rest, |rest| <= 2^-18 |x|), their 2-norms
+//   bf16 pairs (x = hi + mid + rest, |rest| <= 2^-18 |x|), the rows' squares
 //   two lists of rows left to do
 // stride: an odd multiple of 8 (four rows' octets meet distinct banks); rows of
 // dp + 8: an odd number of 16-byte chunks, so ldmatrix meets every bank once.
@@ -527,10 +578,9 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   __shared__ uint32_t mmax_bits;
   __shared__ int members[kSelWarps][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long u = blockIdx.x;
-  const int tile = (int)(u % a.tiles);
-  const long long bh = u / a.tiles;
-  const int b = (int)(bh / a.kv_heads), h = (int)(bh - (long long)b * a.kv_heads);
+  const int bh32 = blockIdx.x / a.tiles, tile = blockIdx.x - bh32 * a.tiles;
+  const long long bh = bh32;
+  const int b = bh32 / a.kv_heads, h = bh32 - b * a.kv_heads;
   const int i0 = tile * TQ;
   int kv = a.kv_lens ? a.kv_lens[b] : a.kv_rows, ql = a.q_lens ? a.q_lens[b] : a.q_rows;
   kv = kv < 0 ? 0 : kv > a.kv_rows ? a.kv_rows : kv;
@@ -547,75 +597,105 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   for (int i = tid; i < (nq - nl) * a.topk; i += kSelThreads) out[(long long)nl * a.topk + i] = -1;
   if (nl == 0) return;
 
-  // the group's summed queries as bf16 pairs, and the 2-norms of the sums of
-  // magnitudes; four or more threads a row, eight channels a step
+  // the group's summed queries as bf16 pairs, and the squares of the sums of
+  // magnitudes; items of eight channels, two a thread and step so that several
+  // loads are in flight; 2^cl lanes a row, joined by shuffles
   const T* qb = (const T*)a.q.p + b * a.q.b + (long long)h * a.group * a.q.h + (long long)i0 * a.q.s;
   const bool q_wide = a.q_vec != 0;
-  const int tpr = min(32, kSelThreads / TQ16);
-  for (int r = tid / tpr; r < TQ16; r += kSelThreads / tpr) {
-    float n2 = 0.f;
-    for (int c = (tid % tpr) * 8; c < DP; c += tpr * 8) {
-      float x[8], m[8];
+  const int cl = 32 - __clz(DP / 8 - 1);
+  for (int it0 = tid; it0 < TQ16 << cl; it0 += 2 * kSelThreads) {
+    float x[2][8], m[2][8];
+    int rr[2], cc[2];
+    bool on[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = m[e] = 0.f;
-      if (r < nl)
-        for (int g = 0; g < a.group; ++g) {
-          const T* src = qb + g * a.q.h + r * a.q.s + c;
-          float v[8];
-          if (q_wide) {  // D is a multiple of 8, rows are 16-byte aligned
-            constexpr int V = 16 / sizeof(T);
+    for (int y = 0; y < 2; ++y) {
+      const int it = it0 + y * kSelThreads;
+      rr[y] = it >> cl;
+      cc[y] = (it - (rr[y] << cl)) * 8;
+      on[y] = rr[y] < nl;
 #pragma unroll
-            for (int y = 0; y < 8 / V; ++y) {
-              const RotVec<T, V> w = c < D ? *reinterpret_cast<const RotVec<T, V>*>(src + y * V) : RotVec<T, V>{};
+      for (int e = 0; e < 8; ++e) x[y][e] = m[y][e] = 0.f;
+    }
+    if (q_wide) {  // D is a multiple of 8, rows are 16-byte aligned
+      constexpr int V = 16 / sizeof(T), NV = 8 / V;
+#pragma unroll 4
+      for (int g = 0; g < a.group; ++g) {
+        RotVec<T, V> w[2][NV];
 #pragma unroll
-              for (int e = 0; e < V; ++e) v[y * V + e] = rot_f32(w.v[e]);
-            }
-          } else {
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < D ? rot_f32(src[e]) : 0.f;
-          }
+          for (int z = 0; z < NV; ++z)
+            w[y][z] = on[y] && cc[y] < D
+                          ? *reinterpret_cast<const RotVec<T, V>*>(qb + g * a.q.h + rr[y] * a.q.s + cc[y] + z * V)
+                          : RotVec<T, V>{};
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            x[e] += v[e];
-            m[e] += fabsf(v[e]);
+            const float v = rot_f32(w[y][e / V].v[e % V]);
+            x[y][e] += v;
+            m[y][e] += fabsf(v);
           }
-        }
+      }
+    } else {
+      for (int g = 0; g < a.group; ++g)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) n2 += m[e] * m[e];
-      sel_split8(x, qhi + r * RS + c, qmid + r * RS + c);
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = on[y] && cc[y] + e < D ? rot_f32(qb[g * a.q.h + rr[y] * a.q.s + cc[y] + e]) : 0.f;
+            x[y][e] += v;
+            m[y][e] += fabsf(v);
+          }
     }
-    for (int m = 1; m < tpr; m <<= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, m);
-    if (tid % tpr == 0 && r < TQ) qn[r] = sqrtf(n2 + kSelTiny);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      float n2 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n2 += m[y][e] * m[y][e];
+      for (int z = 1; z < 1 << cl; z <<= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, z);
+      if (cc[y] == 0 && rr[y] < TQ) qn[rr[y]] = n2 + kSelTiny;
+      if (rr[y] < TQ16 && cc[y] < DP) sel_split8(x[y], qhi + rr[y] * RS + cc[y], qmid + rr[y] * RS + cc[y]);
+    }
   }
   const bool m_wide = D % 4 == 0 && ((uintptr_t)means & 15) == 0;
   for (int j0 = 0; j0 < live; j0 += kSelChunk) {
     const int nj = live - j0 < kSelChunk ? live - j0 : kSelChunk;
     __syncthreads();
-    {
-      const int r = tid >> 2;  // four threads a mean
-      float n2 = 0.f;
-      for (int c = (tid & 3) * 8; c < DP; c += 32) {
-        float x[8];
-        const float* src = means + (long long)(j0 + r) * D + c;
+    float most = 0.f;
+    for (int it0 = tid; it0 < kSelChunk << cl; it0 += 2 * kSelThreads) {
+      float x[2][8];
+      int rr[2], cc[2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < 2; ++y) {
+        const int it = it0 + y * kSelThreads;
+        rr[y] = it >> cl;
+        cc[y] = (it - (rr[y] << cl)) * 8;
+        const bool on = rr[y] < nj;
+        const float* src = means + (long long)(j0 + rr[y]) * D + cc[y];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
           if (m_wide) {
-            const float4 v = r < nj && c + 4 * y < D ? *reinterpret_cast<const float4*>(src + 4 * y) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[4 * y] = v.x; x[4 * y + 1] = v.y; x[4 * y + 2] = v.z; x[4 * y + 3] = v.w;
+            const float4 v = on && cc[y] + 4 * z < D ? *reinterpret_cast<const float4*>(src + 4 * z) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[y][4 * z] = v.x; x[y][4 * z + 1] = v.y; x[y][4 * z + 2] = v.z; x[y][4 * z + 3] = v.w;
           } else {
 #pragma unroll
-            for (int e = 4 * y; e < 4 * y + 4; ++e) x[e] = r < nj && c + e < D ? src[e] : 0.f;
+            for (int e = 4 * z; e < 4 * z + 4; ++e) x[y][e] = on && cc[y] + e < D ? src[e] : 0.f;
           }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) n2 += x[e] * x[e];
-        sel_split8(x, mhi + r * RS + c, mmid + r * RS + c);
       }
-      n2 += __shfl_xor_sync(0xffffffffu, n2, 1);
-      n2 += __shfl_xor_sync(0xffffffffu, n2, 2);
-      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(n2 >= 0.f ? n2 + kSelTiny : INFINITY));
-      if (lane == 0) atomicMax(&mmax_bits, bits);  // values >= 0: bits order as they do
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float n2 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n2 += x[y][e] * x[y][e];
+        for (int z = 1; z < 1 << cl; z <<= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, z);
+        most = fmaxf(most, n2 >= 0.f ? n2 + kSelTiny : INFINITY);
+        if (rr[y] < kSelChunk && cc[y] < DP) sel_split8(x[y], mhi + rr[y] * RS + cc[y], mmid + rr[y] * RS + cc[y]);
+      }
     }
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if (lane == 0) atomicMax(&mmax_bits, bits);  // values >= 0: bits order as they do
     __syncthreads();
     // units of 16 queries x 32 blocks: hi hi + hi mid + mid hi
     for (int unit = warp; unit < TQ16 / 16 * 2; unit += kSelWarps) {
@@ -658,7 +738,10 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   __syncthreads();
   const float mmax = sqrtf(__uint_as_float(mmax_bits)), unit = sel_unit_mma(a) * mmax;
   // parts below the smallest normal number may be lost: 1e-34 of the norms covers them
-  auto err_of = [&](int r) { return unit * qn[r] + 1e-34f * (mmax + qn[r]) + 1e-40f; };
+  auto err_of = [&](int r) {
+    const float q = sqrtf(qn[r]);
+    return unit * q + 1e-34f * (mmax + q) + 1e-40f;
+  };
   if (PER > 0) {
     for (int r0 = warp * 4; r0 < nl; r0 += kSelWarps * 4) {
       const int r = r0 + (lane >> 3);
@@ -688,10 +771,7 @@ __global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs
   double* s64 = reinterpret_cast<double*>(sc) + (long long)warp * NBS;
   for (int x = warp; x < rn; x += workers) {
     const int r = redo[x];
-    for (int j = 0; j < live; ++j) {
-      const double s = sel_score64(a, qb + r * a.q.s, means + (long long)j * D);
-      if (lane == 0) s64[j] = s;
-    }
+    sel_scores64(a, qb + r * a.q.s, means, 0, 1, live, s64);
     __syncwarp();
     sel_row_exact(s64, SelRow(a, i0 + r, live), out + (long long)r * a.topk);
     __syncwarp();
@@ -819,10 +899,7 @@ __global__ __launch_bounds__(kSelThreads) void block_select_few_kernel(const Sel
   int sure = 0, band = 0;
   const SelCase c = sel_place(g, keys, row, err, lo, hi, sure, band);
   if (c == SEL_ALL) {
-    for (int j = warp; j < live; j += kSelWarps) {
-      const double s = sel_score64(a, q, means + (long long)j * D);
-      if (lane == 0) s64[j] = s;
-    }
+    sel_scores64(a, q, means, warp, kSelWarps, live, s64);
     __syncthreads();
     if (warp == 0) sel_row_exact(s64, row, out);
     return;
