@@ -52,18 +52,33 @@ inline int check_launch(const char* what) {
 inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 inline int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
-// Raise a kernel's dynamic shared-memory limit once per (device, kernel).
+// Raise a kernel's dynamic shared-memory limit to `bytes` on the current device
+// unless it is that high already. The limit belongs to the device's kernel, not
+// to the calling thread: one table serves all host threads and never lowers it.
 inline int ensure_smem(const void* fn, int bytes) {
   struct Entry { const void* fn; int dev; int bytes; };
-  static thread_local Entry cache[128];
-  static thread_local int used = 0;
+  constexpr int kEntries = 1024;  // open addressing; more than the library has kernels
+  static Entry table[kEntries];
+  static std::atomic_flag lock = ATOMIC_FLAG_INIT;
   int dev = 0;
   cudaGetDevice(&dev);
-  for (int i = 0; i < used; ++i)
-    if (cache[i].fn == fn && cache[i].dev == dev && cache[i].bytes >= bytes) return SB_OK;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(SB_ERR_CUDA, "shared-memory attribute: %s", cudaGetErrorString(e));
-  if (used < 128) cache[used++] = Entry{fn, dev, bytes};
+  unsigned at = (unsigned)(((uintptr_t)fn >> 4) * 2654435761u + (unsigned)dev) % kEntries;
+  while (lock.test_and_set(std::memory_order_acquire)) {
+  }
+  Entry* e = nullptr;
+  for (int i = 0; i < kEntries && !e; ++i, at = (at + 1) % kEntries)
+    if (!table[at].fn || (table[at].fn == fn && table[at].dev == dev)) e = &table[at];
+  cudaError_t err = cudaSuccess;
+  if (!e || e->fn != fn || e->bytes < bytes) {
+    cudaFuncAttributes now{};
+    err = cudaFuncGetAttributes(&now, fn);
+    if (err == cudaSuccess && now.maxDynamicSharedSizeBytes < bytes)
+      err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == cudaSuccess && e)
+      *e = Entry{fn, dev, bytes > now.maxDynamicSharedSizeBytes ? bytes : now.maxDynamicSharedSizeBytes};
+  }
+  lock.clear(std::memory_order_release);
+  if (err != cudaSuccess) return fail(SB_ERR_CUDA, "shared-memory attribute: %s", cudaGetErrorString(err));
   return SB_OK;
 }
 
