@@ -202,16 +202,28 @@ int launch_select_few(const SelArgs& a, unsigned rows, int cluster, cudaStream_t
 }
 
 // ---- block-sparse attention ------------------------------------------------------
-// Bytes of parts that a window of rows may hold: they stay in the 126 MB L2
-// between the kernel that writes them and the one that joins them.
-constexpr long long kBaWindowBytes = 64ll << 20;
+// Bytes of parts that a window of rows may hold. Windows that fit the 126 MB L2
+// keep the parts off HBM but leave the SMs short of work at every launch's end:
+// 8192 rows, 8 heads of 64, 16 of 128 blocks, forward: 335 us with windows of
+// 64 MB, 278 with 100, 255 with 200, 234 with one of 277 MB.
+constexpr long long kBaWindowBytes = 1ll << 30;
 constexpr int kBaFewRows = 16;      // up to so many queries take the few-query kernel
-constexpr int kBaFwdTarget = 128;   // listed rows per CTA that a segment aims at
-constexpr int kBaBwdTarget = 256;
+// Listed rows per CTA that a segment aims at. Forward, the same case / 16 x 2440
+// rows of 16 over 39 blocks: 229 / 187 us at 128, 219 / 170 at 256, 228 / 157 at
+// 512; backward, the same case: 510 us at 128, 441 at 256, 425 at 512.
+constexpr int kBaFwdTarget = 384;
+constexpr int kBaBwdTarget = 512;
+
+// Segments of `seg` list groups over all windows of wq rows.
+int ba_segments(int q_rows, int wq, int seg) {
+  long long n = 0;
+  for (long long w0 = 0; w0 < q_rows; w0 += wq) n += cdiv(cdiv(q_rows - w0 < wq ? q_rows - w0 : wq, kBaMark), seg);
+  return (int)n;
+}
 
 struct BaPlan {
   int marks, bh_step, wq, seg;
-  size_t bits, slots, part, ml, delta, kv_part, total;
+  size_t entries, spans, slots, part, ml, delta, kv_part, total;
 };
 
 BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, int topk, bool backward) {
@@ -228,17 +240,18 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
     const long long w = kBaWindowBytes / row_bytes / kBaMark * kBaMark;
     p.wq = (int)(w < kBaMark ? kBaMark : w);
   }
+  // a segment: as many groups as give a CTA its target of listed rows on average
   const long long target = backward ? kBaBwdTarget : kBaFwdTarget;
-  long long seg = cdiv(target * nb, (long long)topk * group);
-  seg = cdiv(seg, kBaMark) * kBaMark;
-  if (seg < kBaMark) seg = kBaMark;
-  if (seg > kBaMaxSeg) seg = kBaMaxSeg;
-  if (seg > cdiv(p.wq, kBaMark) * kBaMark) seg = cdiv(p.wq, kBaMark) * kBaMark;
+  long long seg = cdiv(target * nb, (long long)topk * group * kBaMark);
+  if (seg < 1) seg = 1;
+  if (seg > cdiv(p.wq, kBaMark)) seg = cdiv(p.wq, kBaMark);
   p.seg = (int)seg;
   const long long rows = (long long)p.bh_step * p.wq * group;
   size_t at = 0;
-  p.bits = at;
-  at += align256((size_t)bh * p.marks * nb * 32);
+  p.entries = at;
+  at += align256((size_t)bh * p.marks * kBaMark * topk * 2);
+  p.spans = at;
+  at += align256((size_t)bh * nb * p.marks * 4);
   p.slots = at;
   at += align256((size_t)bh * q_rows * 8);
   p.part = at;
@@ -249,8 +262,7 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   if (backward) at += align256((size_t)bh * q_rows * group * 4);
   p.kv_part = at;
   if (backward) {
-    int nseg = 0;
-    for (int w0 = 0; w0 < q_rows; w0 += p.wq) nseg += (int)cdiv(q_rows - w0 < p.wq ? q_rows - w0 : p.wq, p.seg);
+    const long long nseg = ba_segments(q_rows, p.wq, p.seg);
     if (nseg > 1) at += align256((size_t)bh * nb * nseg * 2 * block * dim * 4);
   }
   p.total = at;
@@ -263,6 +275,7 @@ int check_ba(const char* what, int dtype, int batch, int q_heads, int kv_heads, 
   if (batch < 0 || q_rows < 0 || kv_rows < 0 || q_heads < 1 || kv_heads < 1)
     return fail(SB_ERR_INVALID_ARG, "%s: bad sizes", what);
   if (q_heads % kv_heads) return fail(SB_ERR_INVALID_ARG, "%s: %d query heads over %d key heads", what, q_heads, kv_heads);
+  if (q_rows > 1 << 26) return fail(SB_ERR_UNSUPPORTED, "%s: %d rows (at most 2^26)", what, q_rows);
   if (q_heads > 65535 || q_heads / kv_heads > 1024 || (long long)batch * kv_heads > 0x7fffffffll)
     return fail(SB_ERR_UNSUPPORTED, "%s: too many heads", what);
   if (dim < 8 || dim > kBaMaxDim || dim % 8)
@@ -321,7 +334,8 @@ struct LaunchFwd {
                           ba_fwd_smem<DP, BK>(), a, st))
       return s;
     return launch_ba(block_attn_join_kernel<T>, "block_attn_join_kernel",
-                     cdiv((long long)a.nbh * a.wq * a.group * (a.dim / 8), 256), 256, 0, a, st);
+                     cdiv((long long)a.nbh * a.wq * a.group, kBaJoinThreads >> ba_join_lanes(a.dim, a.topk)),
+                     kBaJoinThreads, 0, a, st);
   }
 };
 struct LaunchBwd {
@@ -333,7 +347,8 @@ struct LaunchBwd {
                           ba_bwd_smem<DP, BK>(), a, st))
       return s;
     return launch_ba(block_attn_dq_kernel<T>, "block_attn_dq_kernel",
-                     cdiv((long long)a.nbh * a.wq * a.group * (a.dim / 8), 256), 256, 0, a, st);
+                     cdiv((long long)a.nbh * a.wq * a.group, kBaJoinThreads >> ba_join_lanes(a.dim, a.topk)),
+                     kBaJoinThreads, 0, a, st);
   }
 };
 
@@ -368,7 +383,7 @@ int ba_windows(BaArgs& a, const BaPlan& p, F f) {
     for (a.w0 = 0; a.w0 < a.q_rows; a.w0 += p.wq) {
       a.wq = a.q_rows - a.w0 < p.wq ? a.q_rows - a.w0 : p.wq;
       a.seg = p.seg;
-      a.nseg = (int)cdiv(a.wq, p.seg);
+      a.nseg = (int)cdiv(cdiv(a.wq, kBaMark), p.seg);
       if (int s = f()) return s;
       a.seg0 += a.nseg;
     }
@@ -639,11 +654,13 @@ int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, 
     return fail(SB_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", what, p.total);
   char* ws = (char*)workspace;
   a.marks = p.marks;
-  a.bits = (uint32_t*)(ws + p.bits);
+  a.entries = (uint16_t*)(ws + p.entries);
+  a.spans = (uint32_t*)(ws + p.spans);
   a.slots = (unsigned long long*)(ws + p.slots);
   a.part = (float*)(ws + p.part);
   a.ml = (float2*)(ws + p.ml);
-  if (int s = launch_ba(block_mark_kernel, "block_mark_kernel", (long long)batch * kv_heads * p.marks, kBaMark, 0, a, st))
+  if (int s = launch_ba(block_list_kernel, "block_list_kernel", (long long)batch * kv_heads * p.marks, kBaMark,
+                        ba_list_smem(topk), a, st))
     return s;
   return ba_windows(a, p, [&] { return ba_dispatch(dtype, head_dim, block, LaunchFwd{a, st}); });
 }
@@ -689,14 +706,15 @@ int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const s
     return fail(SB_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", what, p.total);
   char* ws = (char*)workspace;
   a.marks = p.marks;
-  a.bits = (uint32_t*)(ws + p.bits);
+  a.entries = (uint16_t*)(ws + p.entries);
+  a.spans = (uint32_t*)(ws + p.spans);
   a.slots = (unsigned long long*)(ws + p.slots);
   a.part = (float*)(ws + p.part);
   a.delta = (float*)(ws + p.delta);
   a.kv_part = (float*)(ws + p.kv_part);
-  for (int w0 = 0; w0 < q_rows; w0 += p.wq) a.nseg_all += (int)cdiv(q_rows - w0 < p.wq ? q_rows - w0 : p.wq, p.seg);
+  a.nseg_all = ba_segments(q_rows, p.wq, p.seg);
   cudaStream_t st = (cudaStream_t)stream;
-  if (int s = launch_ba(block_mark_kernel, "block_mark_kernel", bh * p.marks, kBaMark, 0, a, st)) return s;
+  if (int s = launch_ba(block_list_kernel, "block_list_kernel", bh * p.marks, kBaMark, ba_list_smem(topk), a, st)) return s;
   const int chunks = 1 << pow2_log2(head_dim / 8);
   const long long dgrid = cdiv(bh * q_rows * a.group * chunks, 256);
   const bool f16 = dtype == SB_F16;

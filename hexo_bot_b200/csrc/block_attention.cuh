@@ -14,10 +14,9 @@
 // block in the query's list; a second kernel joins a row's parts. Nothing is
 // added up in an order that varies: results are the same from run to run.
 //
-// A part is written and read once (8 D bytes a pair against 4 D block flops),
-// so for D >= 32 the traffic of the parts is the cost. The host therefore runs
-// windows of rows whose parts fit the L2 cache, the buffer of the window
-// before being written over while it is still cached.
+// A part is written and read once: 8 D bytes a pair against 4 D block flops,
+// which at D = 64 and block 64 is as long at HBM's rate as the products at that
+// of mma.sync.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -33,8 +32,9 @@ namespace sb {
 
 constexpr int kBaMaxTopk = 64;
 constexpr int kBaMaxDim = 128;
-constexpr int kBaMark = 256;     // queries of a mark word group (8 words)
-constexpr int kBaMaxSeg = 4096;  // queries of a segment
+constexpr int kBaMark = 256;    // queries of a list group
+constexpr int kBaChunk = 1024;  // listed queries that a CTA holds at once
+constexpr int kBaJoinThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -44,7 +44,8 @@ struct BaArgs {
   const int* idx;         // (B, Hkv, Sq, topk)
   const int* kv_lens;
   const int* q_lens;
-  uint32_t* bits;         // (B Hkv, marks, nb, 8): bit i of a block's words = query i of the group chose it
+  uint16_t* entries;      // (B Hkv, marks, kBaMark topk): per group, by block: place in the row's list << 8 | query
+  uint32_t* spans;        // (B Hkv, nb, marks): first entry of the group's queries that chose the block | count << 16
   unsigned long long* slots;  // (B Hkv, Sq): bit s = entry s of the row's list counts
   float* part;            // window's parts: [row][topk][dim], row = (local bh * wq + local i) * group + g
   float2* ml;             // forward: [row][topk] (max in log2 units, sum)
@@ -53,7 +54,7 @@ struct BaArgs {
   int batch, kv_heads, group, q_rows, kv_rows, dim, nb, block, topk, marks;
   int bh0, nbh;           // window: first (batch, kv head) pair and their count
   int w0, wq;             // window: first query and count (w0 a multiple of kBaMark)
-  int seg, nseg;          // queries of a segment, segments of the window
+  int seg, nseg;          // list groups of a segment, segments of the window
   int seg0, nseg_all;     // backward: index of the window's first segment, segments in all
   float scale, scale_log2;
   uint32_t group_magic;   // ceil(2^32 / group), 0 for group 1
@@ -69,34 +70,89 @@ __device__ __forceinline__ int ba_q_len(const BaArgs& a, int b) {
 }
 
 // ---- who chose what -----------------------------------------------------------
-// One CTA per 256 queries of a (batch, kv head): a bit per (block, query), and
-// per query the entries of its list that count (in range, not a repetition).
-constexpr int kBaMarkWindow = 1024;  // blocks whose bits are in shared memory at once
+// One CTA per 256 queries of a (batch, kv head) turns their lists round: for
+// every block the queries that chose it, ascending, with the place of the block
+// in each query's list. A bit per (block, query) in shared memory counts and
+// orders them (a counting sort whose result no scheduling changes) and shows
+// repeated entries: `slots` marks the entries that count.
+constexpr int kBaListWindow = 1024;  // blocks whose bits are in shared memory at once
 
-__global__ __launch_bounds__(kBaMark) void block_mark_kernel(const BaArgs a) {
-  __shared__ uint32_t sm[kBaMarkWindow * 8];
-  const int mark = blockIdx.x % a.marks, bh = blockIdx.x / a.marks;
-  const int b = bh / a.kv_heads;
-  const int i = mark * kBaMark + threadIdx.x;
+__host__ __device__ inline int ba_list_smem(int topk) {
+  return kBaListWindow * 8 * 4 + kBaListWindow * 4 + kBaMark * (topk | 1) * 4;
+}
+
+__global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
+  extern __shared__ __align__(16) char list_smem[];
+  uint32_t* bits = reinterpret_cast<uint32_t*>(list_smem);  // [window][8]
+  uint32_t* offs = bits + kBaListWindow * 8;                // [window]
+  int* rows = reinterpret_cast<int*>(offs + kBaListWindow);  // [256][topk | 1]: odd rows meet distinct banks
+  __shared__ uint32_t warp_sum[kBaMark / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bh = blockIdx.x / a.marks, mark = blockIdx.x - bh * a.marks;
+  const int b = bh / a.kv_heads, K = a.topk, KS = K | 1;
+  const int i = mark * kBaMark + tid;
   const int live = (ba_kv_len(a, b) + a.block - 1) / a.block;
   const bool on = i < ba_q_len(a, b);
-  const int* row = a.idx + ((long long)bh * a.q_rows + i) * a.topk;
+  const int have = min(kBaMark, a.q_rows - mark * kBaMark) * K;
+  const int* src = a.idx + ((long long)bh * a.q_rows + (long long)mark * kBaMark) * K;
+  for (int x = tid; x < have; x += kBaMark) rows[x / K * KS + x % K] = src[x];
   unsigned long long counts = 0;
-  for (int j0 = 0; j0 < a.nb; j0 += kBaMarkWindow) {
-    const int n = a.nb - j0 < kBaMarkWindow ? a.nb - j0 : kBaMarkWindow;
-    for (int x = threadIdx.x; x < n * 8; x += kBaMark) sm[x] = 0;
+  uint32_t base = 0;
+  uint16_t* entries = a.entries + ((long long)bh * a.marks + mark) * kBaMark * K;
+  for (int j0 = 0; j0 < a.nb; j0 += kBaListWindow) {
+    const int n = min(a.nb - j0, kBaListWindow);
+    for (int x = tid; x < n * 8; x += kBaMark) bits[x] = 0;
     __syncthreads();
+    const uint32_t bit = 1u << lane;
     if (on)
-      for (int s = 0; s < a.topk; ++s) {
-        const int j = row[s];
+      for (int s = 0; s < K; ++s) {
+        const int j = rows[tid * KS + s];
         if (j < j0 || j >= j0 + n || j >= live) continue;
-        const uint32_t bit = 1u << (threadIdx.x & 31);
         // this thread alone touches its bit, so the old value tells of a repetition
-        if (!(atomicOr(&sm[(j - j0) * 8 + (threadIdx.x >> 5)], bit) & bit)) counts |= 1ull << s;
+        if (!(atomicOr(&bits[(j - j0) * 8 + warp], bit) & bit)) counts |= 1ull << s;
       }
     __syncthreads();
-    uint32_t* dst = a.bits + (((long long)bh * a.marks + mark) * a.nb + j0) * 8;
-    for (int x = threadIdx.x; x < n * 8; x += kBaMark) dst[x] = sm[x];
+    // four blocks a thread: counts, and their exclusive sums over the window
+    uint32_t c[4], sum = 0;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      c[y] = 0;
+      if (tid * 4 + y < n)
+#pragma unroll
+        for (int w = 0; w < 8; ++w) c[y] += __popc(bits[(tid * 4 + y) * 8 + w]);
+      sum += c[y];
+    }
+    uint32_t pre = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, pre, d);
+      if (lane >= d) pre += o;
+    }
+    if (lane == 31) warp_sum[warp] = pre;
+    __syncthreads();
+    uint32_t at = base + pre - sum;
+#pragma unroll
+    for (int w = 0; w < kBaMark / 32; ++w) {
+      if (w < warp) at += warp_sum[w];
+      base += warp_sum[w];
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (tid * 4 + y < n) {
+        offs[tid * 4 + y] = at;
+        a.spans[((long long)bh * a.nb + j0 + tid * 4 + y) * a.marks + mark] = at | c[y] << 16;
+      }
+      at += c[y];
+    }
+    __syncthreads();
+    if (on)
+      for (int s = 0; s < K; ++s) {
+        const int j = rows[tid * KS + s] - j0;
+        if (!(counts >> s & 1) || j < 0 || j >= n) continue;
+        uint32_t p = offs[j] + __popc(bits[j * 8 + warp] & (bit - 1));
+        for (int w = 0; w < warp; ++w) p += __popc(bits[j * 8 + w]);
+        entries[p] = (uint16_t)(s << 8 | tid);
+      }
     __syncthreads();
   }
   if (i < a.q_rows) a.slots[(long long)bh * a.q_rows + i] = counts;
@@ -125,46 +181,53 @@ __device__ __forceinline__ void ba_load_rows(uint32_t dst, const T* src, long lo
   }
 }
 
-// The listed queries of a segment: ascending indices into list[], returns their
-// count. Every thread of the CTA calls it; it ends with a barrier.
+// The queries that chose block j in the list groups from g on (up to `end`), as
+// many whole groups as fit kBaChunk: list[] gets query << 6 | place in its list,
+// ascending. Moves g past the groups taken; returns the number listed. Every
+// thread of the CTA calls it; it begins and ends with a barrier.
 template <int THREADS>
-__device__ __forceinline__ int ba_list(const BaArgs& a, int bh, int j, int q_first, int q_count, uint16_t* list) {
-  __shared__ int warp_sum[THREADS / 32];
-  const int words = (q_count + 31) / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t* bits = a.bits + (((long long)bh * a.marks + q_first / kBaMark) * a.nb + j) * 8;
-  int total = 0;
-  for (int w0 = 0; w0 < words; w0 += THREADS) {
-    const int w = w0 + threadIdx.x;
-    uint32_t m = 0;
-    if (w < words) m = bits[(long long)(w >> 3) * a.nb * 8 + (w & 7)];
-    const int mine = __popc(m);
-    int pre = mine;
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, pre, d);
-      if (lane >= d) pre += o;
-    }
-    if (lane == 31) warp_sum[warp] = pre;
-    __syncthreads();
-    int at = total + pre - mine;
-    int all = 0;
-    for (int x = 0; x < THREADS / 32; ++x) {
-      if (x < warp) at += warp_sum[x];
-      all += warp_sum[x];
-    }
-    for (; m; m &= m - 1) list[at++] = (uint16_t)(w * 32 + __ffs(m) - 1);
-    total += all;
-    __syncthreads();
+__device__ __forceinline__ int ba_fill(const BaArgs& a, int bh, int j, int& g, int end, uint32_t* list) {
+  __shared__ uint32_t pos[THREADS + 1], first[THREADS];
+  __shared__ uint32_t warp_sum[THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool in = g + tid < end;
+  const uint32_t sp = in ? a.spans[((long long)bh * a.nb + j) * a.marks + g + tid] : 0u;
+  const uint32_t cnt = sp >> 16;
+  uint32_t pre = cnt;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, pre, d);
+    if (lane >= d) pre += o;
   }
-  return total;
+  __syncthreads();  // the list and these arrays may still be in use
+  if (lane == 31) warp_sum[warp] = pre;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) pre += warp_sum[w];
+  pos[tid + 1] = pre;
+  first[tid] = sp & 0xffffu;
+  if (tid == 0) pos[0] = 0;
+  const int taken = __syncthreads_count(in && pre <= kBaChunk);
+  const int n = (int)pos[taken];
+  for (int e = tid; e < n; e += THREADS) {
+    int lo = 0, hi = taken - 1;  // the group that holds entry e
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pos[mid] <= (uint32_t)e) lo = mid;
+      else hi = mid - 1;
+    }
+    const uint32_t x =
+        a.entries[((long long)bh * a.marks + g + lo) * kBaMark * a.topk + first[lo] + (e - pos[lo])];
+    list[e] = (uint32_t)((g + lo) * kBaMark + (x & 255)) << 6 | x >> 8;
+  }
+  g += taken;
+  __syncthreads();
+  return n;
 }
 
-// Place of block j in a row's list: its first entry that counts.
-__device__ __forceinline__ int ba_slot(const BaArgs& a, long long row, int j) {
-  const int* p = a.idx + row * a.topk;
-  for (int s = 0; s < a.topk; ++s)
-    if (p[s] == j) return s;
-  return 0;
+__device__ __forceinline__ float ba_exp2(float x) {  // 2^x, relative error 2^-22, 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ int ba_div_group(const BaArgs& a, int x) {
@@ -199,14 +262,21 @@ struct BaTile {
         MmaTraits<T>::mma(s[2 * n + 1], fa, b1);
       }
     }
+    if (scale_log2 < 0.f) {
+#pragma unroll
+      for (int n = 0; n < BK / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = -s[n][e];
+    }
+    const float sc = fmaxf(fabsf(scale_log2), 1e-38f);  // not 0: masked scores stay -inf
+    if (live_keys < BK) {
+#pragma unroll
+      for (int n = 0; n < BK / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n * 8 + 2 * (lane & 3) + (e & 1) >= live_keys) s[n][e] = -INFINITY;
+    }
     m[0] = m[1] = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < BK / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] *= scale_log2;
-        if (n * 8 + 2 * (lane & 3) + (e & 1) >= live_keys) s[n][e] = -INFINITY;
-      }
 #pragma unroll
     for (int n = 0; n < BK / 8; ++n)
 #pragma unroll
@@ -215,15 +285,16 @@ struct BaTile {
     for (int r = 0; r < 2; ++r) {
       m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
       m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2));
+      // -inf (no score above it: the row keeps weight 0) or the maximum in log2 units
+      m[r] = m[r] == -INFINITY ? m[r] : m[r] * sc;
       l[r] = 0.f;
     }
-    // a row of nothing but -inf scores keeps weight 0
     const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
     for (int n = 0; n < BK / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = exp2f(s[n][e] - (e >> 1 ? m1 : m0));
+        s[n][e] = ba_exp2(fmaf(s[n][e], sc, e >> 1 ? -m1 : -m0));
         l[e >> 1] += s[n][e];
       }
 #pragma unroll
@@ -261,7 +332,7 @@ constexpr int kBaFwdWarps = kBaFwdThreads / 32;
 
 template <int DP, int BK>
 constexpr int ba_fwd_smem() {
-  return 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2 + kBaMaxSeg * 2;
+  return 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2 + kBaChunk * 4;
 }
 
 template <typename T, int DP, int BK>
@@ -270,120 +341,181 @@ __global__ __launch_bounds__(kBaFwdThreads) void block_attn_kernel(const BaArgs 
   const uint32_t ks = smem_u32(ba_smem), vs = ks + BK * DP * 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t qs = vs + BK * DP * 2 + warp * (2 * 16 * DP * 2);
-  uint16_t* list = reinterpret_cast<uint16_t*>(ba_smem + 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2);
-  const long long u = blockIdx.x;
-  const int sg = (int)(u % a.nseg);
-  const int j = (int)((u / a.nseg) % a.nb);
-  const int lbh = (int)(u / a.nseg / a.nb), bh = a.bh0 + lbh;
+  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2);
+  const uint32_t u = blockIdx.x;
+  const int sg = (int)(u % (uint32_t)a.nseg);
+  const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
+  const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const int q_first = a.w0 + sg * a.seg;
-  const int q_count = min(a.seg, a.w0 + a.wq - q_first);
+  int g = a.w0 / kBaMark + sg * a.seg;
+  const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
   const int have = min(BK, ba_kv_len(a, b) - j * BK);
   if (have <= 0) return;
-  const int n = ba_list<kBaFwdThreads>(a, bh, j, q_first, q_count, list);
-  if (n == 0) return;
   const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s;
   const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s;
-  ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
-  ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
-  cp_async_commit();
-
-  const int rows = n * a.group;
   const int G = a.group;
   const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
   constexpr int CH = DP / 8;
-  auto load_q = [&](int tile, uint32_t dst) {
-    for (int x = lane; x < 16 * CH; x += 32) {
-      const int r = x / CH, c = x - r * CH;
-      const int row = tile * 16 + r;
-      const bool ok = row < rows && c * 8 < a.dim;
-      const T* src = qp;
-      if (ok) {
-        const int li = ba_div_group(a, row), g = row - li * G;
-        src = qp + g * a.q.h + (long long)(q_first + list[li]) * a.q.s + c * 8;
-      }
-      cp_async16(ba_at<DP>(dst, r, c), src, ok ? 16 : 0);
+  bool loaded = false;
+  while (g < end) {
+    const int n = ba_fill<kBaFwdThreads>(a, bh, j, g, end, list);
+    if (n == 0) continue;
+    if (!loaded) {
+      ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
+      ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
     }
-  };
-  const int tiles = (rows + 15) / 16;
-  if (warp < tiles) load_q(warp, qs);
-  cp_async_commit();
-  cp_async_wait<1>();
-  __syncthreads();
-  int buf = 0;
-  for (int t = warp; t < tiles; t += kBaFwdWarps, buf ^= 1) {
-    const uint32_t qt = qs + buf * (16 * DP * 2);
-    if (t + kBaFwdWarps < tiles) load_q(t + kBaFwdWarps, qs + (buf ^ 1) * (16 * DP * 2));
     cp_async_commit();
-    // this lane's two rows: where their parts go
-    long long at[2];
-    bool ok[2];
+    const int rows = n * G;
+    auto load_q = [&](int tile, uint32_t dst) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = t * 16 + (lane >> 2) + 8 * r;
-      ok[r] = row < rows;
-      at[r] = 0;
-      if (ok[r]) {
-        const int li = ba_div_group(a, row), g = row - li * G;
-        const int i = q_first + list[li];
-        const int slot = ba_slot(a, (long long)bh * a.q_rows + i, j);
-        at[r] = (((long long)lbh * a.wq + (i - a.w0)) * G + g) * a.topk + slot;
+      for (int x0 = 0; x0 < 16 * CH; x0 += 32) {
+        const int x = x0 + lane;
+        const int r = x / CH, c = x % CH;
+        const int row = tile * 16 + r;
+        const bool ok = row < rows && c * 8 < a.dim;
+        const T* src = qp;
+        if (ok) {
+          const int li = ba_div_group(a, row), gr = row - li * G;
+          src = qp + gr * a.q.h + (long long)(list[li] >> 6) * a.q.s + c * 8;
+        }
+        cp_async16(ba_at<DP>(dst, r, c), src, ok ? 16 : 0);
       }
+    };
+    const int tiles = (rows + 15) / 16;
+    if (warp < tiles) load_q(warp, qs);
+    cp_async_commit();
+    if (!loaded) {
+      cp_async_wait<1>();
+      __syncthreads();
+      loaded = true;
     }
-    cp_async_wait<1>();
-    __syncwarp();
-    BaTile<T, DP, BK> tile;
-    tile.run(qt, ks, vs, have, a.scale_log2);
-    __syncwarp();  // the buffer is free for the tile after next
+    int buf = 0;
+    for (int t = warp; t < tiles; t += kBaFwdWarps, buf ^= 1) {
+      const uint32_t qt = qs + buf * (16 * DP * 2);
+      if (t + kBaFwdWarps < tiles) load_q(t + kBaFwdWarps, qs + (buf ^ 1) * (16 * DP * 2));
+      cp_async_commit();
+      // this lane's two rows: where their parts go
+      long long at[2];
+      bool ok[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (!ok[r]) continue;
-      if ((lane & 3) == 0) a.ml[at[r]] = make_float2(tile.m[r], tile.l[r]);
-      float* p = a.part + at[r] * a.dim;
+      for (int r = 0; r < 2; ++r) {
+        const int row = t * 16 + (lane >> 2) + 8 * r;
+        ok[r] = row < rows;
+        const int li = ok[r] ? ba_div_group(a, row) : 0, gr = row - li * G;
+        const uint32_t e = list[li];
+        at[r] = (((long long)lbh * a.wq + ((int)(e >> 6) - a.w0)) * G + gr) * a.topk + (e & 63);
+      }
+      cp_async_wait<1>();
+      __syncwarp();
+      BaTile<T, DP, BK> tile;
+      tile.run(qt, ks, vs, have, a.scale_log2);
+      __syncwarp();  // the buffer is free for the tile after next
 #pragma unroll
-      for (int nn = 0; nn < DP / 8; ++nn)
-        if (nn * 8 < a.dim)
-          *reinterpret_cast<float2*>(p + nn * 8 + 2 * (lane & 3)) = make_float2(tile.o[nn][2 * r], tile.o[nn][2 * r + 1]);
+      for (int r = 0; r < 2; ++r) {
+        if (!ok[r]) continue;
+        if ((lane & 3) == 0) a.ml[at[r]] = make_float2(tile.m[r], tile.l[r]);
+        float* p = a.part + at[r] * a.dim;
+#pragma unroll
+        for (int nn = 0; nn < DP / 8; ++nn)
+          if (nn * 8 < a.dim)
+            *reinterpret_cast<float2*>(p + nn * 8 + 2 * (lane & 3)) =
+                make_float2(tile.o[nn][2 * r], tile.o[nn][2 * r + 1]);
+      }
     }
   }
 }
 
-// Joins the parts of each row: 8 channels a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void block_attn_join_kernel(const BaArgs a) {
-  const int chunks = a.dim / 8;
-  const long long total = (long long)a.nbh * a.wq * a.group * chunks;
-  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (x >= total) return;
-  const long long row = x / chunks;
-  const int c = (int)(x - row * chunks);
-  const long long iq = row / a.group;
-  const int g = (int)(row - iq * a.group);
-  const int lbh = (int)(iq / a.wq), i = a.w0 + (int)(iq - (long long)lbh * a.wq);
-  const int bh = a.bh0 + lbh, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + g;
-  const unsigned long long slots = a.slots[(long long)bh * a.q_rows + i];
-  const float2* ml = a.ml + row * a.topk;
-  float top = -INFINITY;
-  for (unsigned long long m = slots; m; m &= m - 1) top = fmaxf(top, ml[__ffsll(m) - 1].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (unsigned long long m = slots; m; m &= m - 1) {
-    const int s = __ffsll(m) - 1;
-    const float2 p = ml[s];
-    const float w = exp2f(p.x - ref);
-    sum += w * p.y;
-    const float4* src = reinterpret_cast<const float4*>(a.part + (row * a.topk + s) * a.dim + c * 8);
-    const float4 u = src[0], v = src[1];
-    acc[0] += w * u.x; acc[1] += w * u.y; acc[2] += w * u.z; acc[3] += w * u.w;
-    acc[4] += w * v.x; acc[5] += w * v.y; acc[6] += w * v.z; acc[7] += w * v.w;
+// A row's place in the window, for the kernels that join parts: 2^cl lanes of
+// eight channels each, times strands of lanes that take up to four parts each
+// (where a warp has them); a warp holds as many rows as fit.
+__host__ __device__ inline int ba_join_log2(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+__host__ __device__ inline int ba_join_lanes(int dim, int topk) {  // log2 of a row's lanes
+  const int l = ba_join_log2(dim / 8) + ba_join_log2((topk + 3) / 4);
+  return l < 5 ? l : 5;
+}
+struct BaRow {
+  long long row;  // of the window
+  int lbh, i, g, c, strand, strands, chunks;
+  __device__ __forceinline__ BaRow(const BaArgs& a) {
+    const int cl = ba_join_log2(a.dim / 8), rl = ba_join_lanes(a.dim, a.topk);
+    const int lane = threadIdx.x & ((1 << rl) - 1);
+    row = (long long)blockIdx.x * (kBaJoinThreads >> rl) + (threadIdx.x >> rl);
+    c = (lane & ((1 << cl) - 1)) * 8;
+    strand = lane >> cl;
+    strands = 1 << (rl - cl);
+    chunks = 1 << cl;
+    const int iq = (int)(row / a.group);
+    g = (int)(row - (long long)iq * a.group);
+    lbh = iq / a.wq;
+    i = a.w0 + iq - lbh * a.wq;
   }
+};
+// Sum over a row's strands.
+__device__ __forceinline__ void ba_strand_sum(float (&acc)[8], const BaRow& r) {
+  for (int m = r.chunks; m < r.chunks * r.strands; m <<= 1)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], m);
+}
+
+// Joins the parts of each row, four parts a lane in flight.
+template <typename T>
+__global__ __launch_bounds__(kBaJoinThreads) void block_attn_join_kernel(const BaArgs a) {
+  const BaRow r(a);
+  const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
+  const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
+  const unsigned long long slots = there ? a.slots[(long long)bh * a.q_rows + r.i] : 0ull;
+  const float2* ml = a.ml + r.row * a.topk;
+  const float* part = a.part + r.row * a.topk * a.dim + r.c;
+  const bool on = r.c < a.dim;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, sum = 0.f;
+  for (int s0 = r.strand; s0 < a.topk; s0 += 4 * r.strands) {
+    float2 p[4];
+    float4 u[4], v[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int s = s0 + y * r.strands;
+      const bool in = s < a.topk && (slots >> s & 1);
+      p[y] = in ? ml[s] : make_float2(-INFINITY, 0.f);
+      const float4* src = reinterpret_cast<const float4*>(part + (long long)s * a.dim);
+      u[y] = in && on ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[y] = in && on ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const float t = fmaxf(fmaxf(fmaxf(p[0].x, p[1].x), fmaxf(p[2].x, p[3].x)), top);
+    const float ref = t == -INFINITY ? 0.f : t;
+    const float w0 = ba_exp2(top - ref);
+    top = t;
+    sum *= w0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= w0;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float w = ba_exp2(p[y].x - ref);
+      sum += w * p[y].y;
+      acc[0] += w * u[y].x; acc[1] += w * u[y].y; acc[2] += w * u[y].z; acc[3] += w * u[y].w;
+      acc[4] += w * v[y].x; acc[5] += w * v[y].y; acc[6] += w * v[y].z; acc[7] += w * v[y].w;
+    }
+  }
+  float all = top;
+  for (int m = r.chunks; m < r.chunks * r.strands; m <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, m));
+  const float ref = all == -INFINITY ? 0.f : all;
+  const float w = ba_exp2(top - ref);
+  sum *= w;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] *= w;
+  for (int m = r.chunks; m < r.chunks * r.strands; m <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  ba_strand_sum(acc, r);
+  if (r.strand != 0 || !there) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   RotVec<T, 8> y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y.v[e] = rot_cast<T>(acc[e] * inv);
-  *reinterpret_cast<RotVec<T, 8>*>((T*)a.o.p + b * a.o.b + h * a.o.h + i * a.o.s + c * 8) = y;
-  if (c == 0) a.lse[((long long)b * a.kv_heads * a.group + h) * a.q_rows + i] = (ref + log2f(sum)) * kLn2;
+  if (on) *reinterpret_cast<RotVec<T, 8>*>((T*)a.o.p + b * a.o.b + h * a.o.h + r.i * a.o.s + r.c) = y;
+  if (r.c == 0) a.lse[((long long)b * a.kv_heads * a.group + h) * a.q_rows + r.i] = (ref + log2f(sum)) * kLn2;
 }
 
 // ---- forward, few queries --------------------------------------------------------
@@ -464,7 +596,7 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
     for (int r = 0; r < 2; ++r) {
       const float t = fmaxf(top[r], tile.m[r]);
       const float ref = t == -INFINITY ? 0.f : t;
-      const float wo = exp2f(top[r] - ref), wn = exp2f(tile.m[r] - ref);
+      const float wo = ba_exp2(top[r] - ref), wn = ba_exp2(tile.m[r] - ref);
       top[r] = t;
       sum[r] = sum[r] * wo + tile.l[r] * wn;
 #pragma unroll
@@ -494,7 +626,7 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
     const float ref = t == -INFINITY ? 0.f : t;
     float acc = 0.f, s = 0.f;
     for (int w = 0; w < W; ++w) {
-      const float f = exp2f(sml[w][row].x - ref);
+      const float f = ba_exp2(sml[w][row].x - ref);
       s += f * sml[w][row].y;
       acc += f * all[w * (16 * DP) + row * DP + d];
     }
@@ -546,7 +678,7 @@ constexpr int ba_bwd_rows() {
 template <int DP, int BK>
 constexpr int ba_bwd_smem() {
   constexpr int TR = ba_bwd_rows<DP>();
-  return 2 * BK * DP * 2 + 2 * 2 * TR * DP * 2 + BK * TR * 2 + 2 * TR * 16 + kBaMaxSeg * 2;
+  return 2 * BK * DP * 2 + 2 * 2 * TR * DP * 2 + BK * TR * 2 + 2 * TR * 16 + kBaChunk * 4;
 }
 
 template <typename T, int DP, int BK>
@@ -562,25 +694,20 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
   // per row of a tile: (lse in log2 units, delta) and where its dq part goes
   float2* stat = reinterpret_cast<float2*>(tail);                    // [2][TR]
   long long* dst = reinterpret_cast<long long*>(tail + 2 * TR * 8);  // [2][TR]
-  uint16_t* list = reinterpret_cast<uint16_t*>(tail + 2 * TR * 16);
+  uint32_t* list = reinterpret_cast<uint32_t*>(tail + 2 * TR * 16);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long u = blockIdx.x;
-  const int sg = (int)(u % a.nseg);
-  const int j = (int)((u / a.nseg) % a.nb);
-  const int lbh = (int)(u / a.nseg / a.nb), bh = a.bh0 + lbh;
+  const uint32_t u = blockIdx.x;
+  const int sg = (int)(u % (uint32_t)a.nseg);
+  const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
+  const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  const int q_first = a.w0 + sg * a.seg;
-  const int q_count = min(a.seg, a.w0 + a.wq - q_first);
+  int first_group = a.w0 / kBaMark + sg * a.seg;
+  const int end = min(first_group + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
   const int G = a.group;
   const int have = max(0, min(BK, ba_kv_len(a, b) - j * BK));
-  const int n = ba_list<THREADS>(a, bh, j, q_first, q_count, list);
-  const int rows = n * G;
+  int rows = 0;  // of the chunk at hand
   const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s;
   const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s;
-  if (n > 0) {
-    ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, THREADS);
-    ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, THREADS);
-  }
   const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
   const T* gp = (const T*)a.go.p + b * a.go.b + (long long)h * G * a.go.h;
   constexpr int CH = DP / 8;
@@ -592,7 +719,7 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
       const T *sq = qp, *sgr = gp;
       if (ok) {
         const int li = ba_div_group(a, row), g = row - li * G;
-        const long long i = q_first + list[li];
+        const long long i = list[li] >> 6;
         sq = qp + g * a.q.h + i * a.q.s + c * 8;
         sgr = gp + g * a.go.h + i * a.go.s + c * 8;
       }
@@ -605,12 +732,13 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
       long long to = -1;
       if (row < rows) {
         const int li = ba_div_group(a, row), g = row - li * G;
-        const int i = q_first + list[li];
+        const uint32_t e = list[li];
+        const int i = (int)(e >> 6);
         const long long qrow = (long long)bh * a.q_rows + i;
         // a row all of whose scores are -inf has no weights
         const float l = a.lse[((long long)b * a.kv_heads * G + h * G + g) * a.q_rows + i];
         st = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, a.delta[qrow * G + g]);
-        to = (((long long)lbh * a.wq + (i - a.w0)) * G + g) * a.topk + ba_slot(a, qrow, j);
+        to = (((long long)lbh * a.wq + (i - a.w0)) * G + g) * a.topk + (e & 63);
       }
       stat[buf * TR + r] = st;
       dst[buf * TR + r] = to;
@@ -621,112 +749,122 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
   for (int x = 0; x < DP / 8; ++x)
 #pragma unroll
     for (int e = 0; e < 4; ++e) dk[x][e] = dv[x][e] = 0.f;
-  const int tiles = (rows + TR - 1) / TR;
-  if (tiles > 0) load_tile(0, 0);
-  cp_async_commit();
   const int k0 = warp * 16;
   const bool live0 = k0 + (lane >> 2) < have, live1 = k0 + (lane >> 2) + 8 < have;
-  for (int t = 0; t < tiles; ++t) {
-    const int buf = t & 1;
-    if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
+  bool loaded = false;
+  for (int gq = have > 0 ? first_group : end; gq < end;) {
+    rows = ba_fill<THREADS>(a, bh, j, gq, end, list) * G;
+    if (rows == 0) continue;
+    if (!loaded) {
+      ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, THREADS);
+      ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, THREADS);
+      loaded = true;
+    }
+    const int tiles = (rows + TR - 1) / TR;
+    load_tile(0, 0);
     cp_async_commit();
-    cp_async_wait<1>();
-    __syncthreads();
-    const uint32_t qt = qs + buf * TILE, gt = gs + buf * TILE;
-    float s[TR / 8][4], dp[TR / 8][4];
+    for (int t = 0; t < tiles; ++t) {
+      const int buf = t & 1;
+      if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+      __syncthreads();
+      const uint32_t qt = qs + buf * TILE, gt = gs + buf * TILE;
+      float s[TR / 8][4], dp[TR / 8][4];
 #pragma unroll
-    for (int x = 0; x < TR / 8; ++x)
+      for (int x = 0; x < TR / 8; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[x][e] = dp[x][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[x][e] = dp[x][e] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      uint32_t fk[4], fv[4];
-      ldmatrix_x4(fk, ba_at<DP>(ks, k0 + (lane & 15), 2 * kk + (lane >> 4)));
-      ldmatrix_x4(fv, ba_at<DP>(vs, k0 + (lane & 15), 2 * kk + (lane >> 4)));
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t fk[4], fv[4];
+        ldmatrix_x4(fk, ba_at<DP>(ks, k0 + (lane & 15), 2 * kk + (lane >> 4)));
+        ldmatrix_x4(fv, ba_at<DP>(vs, k0 + (lane & 15), 2 * kk + (lane >> 4)));
+#pragma unroll
+        for (int x = 0; x < TR / 16; ++x) {
+          uint32_t f[4];
+          ldmatrix_x4(f, ba_at<DP>(qt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+          const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
+          MmaTraits<T>::mma(s[2 * x], fk, b0);
+          MmaTraits<T>::mma(s[2 * x + 1], fk, b1);
+          ldmatrix_x4(f, ba_at<DP>(gt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+          const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
+          MmaTraits<T>::mma(dp[2 * x], fv, c0);
+          MmaTraits<T>::mma(dp[2 * x + 1], fv, c1);
+        }
+      }
+      // p = 2^(s - lse), ds = p (dp - delta): columns are rows of the tile
+#pragma unroll
+      for (int x = 0; x < TR / 8; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 st = stat[buf * TR + 8 * x + 2 * (lane & 3) + (e & 1)];
+          const bool live = e >> 1 ? live1 : live0;
+          s[x][e] = live ? ba_exp2(fmaf(s[x][e], a.scale_log2, -st.x)) : 0.f;
+          dp[x][e] = live ? s[x][e] * (dp[x][e] - st.y) : 0.f;
+        }
+      // p and ds are rounded to the inputs' type for the matrix unit (as the
+      // forward rounds p); their products are added in 32 bits
+      uint32_t fp[TR / 16][4], fd[TR / 16][4];
 #pragma unroll
       for (int x = 0; x < TR / 16; ++x) {
-        uint32_t f[4];
-        ldmatrix_x4(f, ba_at<DP>(qt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-        const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
-        MmaTraits<T>::mma(s[2 * x], fk, b0);
-        MmaTraits<T>::mma(s[2 * x + 1], fk, b1);
-        ldmatrix_x4(f, ba_at<DP>(gt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-        const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
-        MmaTraits<T>::mma(dp[2 * x], fv, c0);
-        MmaTraits<T>::mma(dp[2 * x + 1], fv, c1);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          fp[x][2 * hf] = MmaTraits<T>::pack(s[2 * x + hf][0], s[2 * x + hf][1]);
+          fp[x][2 * hf + 1] = MmaTraits<T>::pack(s[2 * x + hf][2], s[2 * x + hf][3]);
+          fd[x][2 * hf] = MmaTraits<T>::pack(dp[2 * x + hf][0], dp[2 * x + hf][1]);
+          fd[x][2 * hf + 1] = MmaTraits<T>::pack(dp[2 * x + hf][2], dp[2 * x + hf][3]);
+          // ds to shared memory as [key][row]
+          const uint32_t a0 = ba_at<TR>(ds, k0 + (lane >> 2), 2 * x + hf) + 4 * (lane & 3);
+          const uint32_t a1 = ba_at<TR>(ds, k0 + (lane >> 2) + 8, 2 * x + hf) + 4 * (lane & 3);
+          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a0), "r"(fd[x][2 * hf]) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a1), "r"(fd[x][2 * hf + 1]) : "memory");
+        }
       }
+#pragma unroll
+      for (int x = 0; x < TR / 16; ++x)
+#pragma unroll
+        for (int nn = 0; nn < DP / 16; ++nn) {
+          uint32_t f[4];
+          ldmatrix_x4_trans(f, ba_at<DP>(gt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
+          const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
+          MmaTraits<T>::mma(dv[2 * nn], fp[x], b0);
+          MmaTraits<T>::mma(dv[2 * nn + 1], fp[x], b1);
+          ldmatrix_x4_trans(f, ba_at<DP>(qt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
+          const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
+          MmaTraits<T>::mma(dk[2 * nn], fd[x], c0);
+          MmaTraits<T>::mma(dk[2 * nn + 1], fd[x], c1);
+        }
+      __syncthreads();
+      // dq parts: units of 16 rows x 16 channels, spread over the warps
+      for (int unit = warp; unit < (TR / 16) * (DP / 16); unit += NW) {
+        const int mt = unit % (TR / 16), nt = unit / (TR / 16);
+        if (nt * 16 >= a.dim || t * TR + mt * 16 >= rows) continue;
+        float acc[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          uint32_t fa[4], fb[4];
+          ldmatrix_x4_trans(fa, ba_at<TR>(ds, 16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
+          ldmatrix_x4_trans(fb, ba_at<DP>(ks, 16 * kk + (lane & 15), 2 * nt + (lane >> 4)));
+          const uint32_t b0[2] = {fb[0], fb[1]}, b1[2] = {fb[2], fb[3]};
+          MmaTraits<T>::mma(acc[0], fa, b0);
+          MmaTraits<T>::mma(acc[1], fa, b1);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const long long to = dst[buf * TR + mt * 16 + (lane >> 2) + 8 * r];
+          if (to < 0) continue;
+          float* p = a.part + to * a.dim + nt * 16 + 2 * (lane & 3);
+          *reinterpret_cast<float2*>(p) = make_float2(acc[0][2 * r], acc[0][2 * r + 1]);
+          if (nt * 16 + 8 < a.dim) *reinterpret_cast<float2*>(p + 8) = make_float2(acc[1][2 * r], acc[1][2 * r + 1]);
+        }
+      }
+      __syncthreads();  // ds, the tile and its stats are written over from here on
     }
-    // p = 2^(s - lse), ds = p (dp - delta): columns are rows of the tile
-#pragma unroll
-    for (int x = 0; x < TR / 8; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 st = stat[buf * TR + 8 * x + 2 * (lane & 3) + (e & 1)];
-        const bool live = e >> 1 ? live1 : live0;
-        s[x][e] = live ? exp2f(s[x][e] * a.scale_log2 - st.x) : 0.f;
-        dp[x][e] = live ? s[x][e] * (dp[x][e] - st.y) : 0.f;
-      }
-    // p and ds are rounded to the inputs' type for the matrix unit (as the
-    // forward rounds p); their products are added in 32 bits
-    uint32_t fp[TR / 16][4], fd[TR / 16][4];
-#pragma unroll
-    for (int x = 0; x < TR / 16; ++x) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        fp[x][2 * hf] = MmaTraits<T>::pack(s[2 * x + hf][0], s[2 * x + hf][1]);
-        fp[x][2 * hf + 1] = MmaTraits<T>::pack(s[2 * x + hf][2], s[2 * x + hf][3]);
-        fd[x][2 * hf] = MmaTraits<T>::pack(dp[2 * x + hf][0], dp[2 * x + hf][1]);
-        fd[x][2 * hf + 1] = MmaTraits<T>::pack(dp[2 * x + hf][2], dp[2 * x + hf][3]);
-        // ds to shared memory as [key][row]
-        const uint32_t a0 = ba_at<TR>(ds, k0 + (lane >> 2), 2 * x + hf) + 4 * (lane & 3);
-        const uint32_t a1 = ba_at<TR>(ds, k0 + (lane >> 2) + 8, 2 * x + hf) + 4 * (lane & 3);
-        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a0), "r"(fd[x][2 * hf]) : "memory");
-        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a1), "r"(fd[x][2 * hf + 1]) : "memory");
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < TR / 16; ++x)
-#pragma unroll
-      for (int nn = 0; nn < DP / 16; ++nn) {
-        uint32_t f[4];
-        ldmatrix_x4_trans(f, ba_at<DP>(gt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
-        const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
-        MmaTraits<T>::mma(dv[2 * nn], fp[x], b0);
-        MmaTraits<T>::mma(dv[2 * nn + 1], fp[x], b1);
-        ldmatrix_x4_trans(f, ba_at<DP>(qt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
-        const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
-        MmaTraits<T>::mma(dk[2 * nn], fd[x], c0);
-        MmaTraits<T>::mma(dk[2 * nn + 1], fd[x], c1);
-      }
-    __syncthreads();
-    // dq parts: units of 16 rows x 16 channels, spread over the warps
-    for (int unit = warp; unit < (TR / 16) * (DP / 16); unit += NW) {
-      const int mt = unit % (TR / 16), nt = unit / (TR / 16);
-      if (nt * 16 >= a.dim || t * TR + mt * 16 >= rows) continue;
-      float acc[2][4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) {
-        uint32_t fa[4], fb[4];
-        ldmatrix_x4_trans(fa, ba_at<TR>(ds, 16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
-        ldmatrix_x4_trans(fb, ba_at<DP>(ks, 16 * kk + (lane & 15), 2 * nt + (lane >> 4)));
-        const uint32_t b0[2] = {fb[0], fb[1]}, b1[2] = {fb[2], fb[3]};
-        MmaTraits<T>::mma(acc[0], fa, b0);
-        MmaTraits<T>::mma(acc[1], fa, b1);
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const long long to = dst[buf * TR + mt * 16 + (lane >> 2) + 8 * r];
-        if (to < 0) continue;
-        float* p = a.part + to * a.dim + nt * 16 + 2 * (lane & 3);
-        *reinterpret_cast<float2*>(p) = make_float2(acc[0][2 * r], acc[0][2 * r + 1]);
-        if (nt * 16 + 8 < a.dim) *reinterpret_cast<float2*>(p + 8) = make_float2(acc[1][2 * r], acc[1][2 * r + 1]);
-      }
-    }
-    __syncthreads();  // ds, the tile and its stats are written over from here on
   }
   cp_async_wait_all();
   // keys of this block: final rows, or this segment's part
@@ -758,28 +896,35 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
 
 // dq of the window: the sum of each row's parts.
 template <typename T>
-__global__ __launch_bounds__(256) void block_attn_dq_kernel(const BaArgs a) {
-  const int chunks = a.dim / 8;
-  const long long total = (long long)a.nbh * a.wq * a.group * chunks;
-  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (x >= total) return;
-  const long long row = x / chunks;
-  const int c = (int)(x - row * chunks);
-  const long long iq = row / a.group;
-  const int g = (int)(row - iq * a.group);
-  const int lbh = (int)(iq / a.wq), i = a.w0 + (int)(iq - (long long)lbh * a.wq);
-  const int bh = a.bh0 + lbh, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + g;
+__global__ __launch_bounds__(kBaJoinThreads) void block_attn_dq_kernel(const BaArgs a) {
+  const BaRow r(a);
+  const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
+  const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
+  const unsigned long long slots = there ? a.slots[(long long)bh * a.q_rows + r.i] : 0ull;
+  const float* part = a.part + r.row * a.topk * a.dim + r.c;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (unsigned long long m = a.slots[(long long)bh * a.q_rows + i]; m; m &= m - 1) {
-    const float4* src = reinterpret_cast<const float4*>(a.part + (row * a.topk + __ffsll(m) - 1) * a.dim + c * 8);
-    const float4 u = src[0], v = src[1];
-    acc[0] += u.x; acc[1] += u.y; acc[2] += u.z; acc[3] += u.w;
-    acc[4] += v.x; acc[5] += v.y; acc[6] += v.z; acc[7] += v.w;
+  for (int s0 = r.strand; s0 < a.topk; s0 += 4 * r.strands) {
+    float4 u[4], v[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int s = s0 + y * r.strands;
+      const bool in = s < a.topk && (slots >> s & 1) && r.c < a.dim;
+      const float4* src = reinterpret_cast<const float4*>(part + (long long)s * a.dim);
+      u[y] = in ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[y] = in ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      acc[0] += u[y].x; acc[1] += u[y].y; acc[2] += u[y].z; acc[3] += u[y].w;
+      acc[4] += v[y].x; acc[5] += v[y].y; acc[6] += v[y].z; acc[7] += v[y].w;
+    }
   }
+  ba_strand_sum(acc, r);
+  if (r.strand != 0 || r.c >= a.dim || !there) return;
   RotVec<T, 8> y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y.v[e] = rot_cast<T>(acc[e] * a.scale);
-  *reinterpret_cast<RotVec<T, 8>*>((T*)a.dq.p + b * a.dq.b + h * a.dq.h + i * a.dq.s + c * 8) = y;
+  *reinterpret_cast<RotVec<T, 8>*>((T*)a.dq.p + b * a.dq.b + h * a.dq.h + r.i * a.dq.s + r.c) = y;
 }
 
 // dk, dv: the sum of the segments' parts, in segment order.

@@ -655,6 +655,24 @@ def test_rows_past_two_to_the_32():
     assert torch.equal(ops._qk(packed, packed, w, w, coords, freqs, (8,), False, 1e-6)[0], pq[0])
 
 
+def test_calls_from_several_host_threads():
+    """A kernel's shared-memory limit is the device's: a thread that asks for less must not take it
+    from one that asked for more."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    g = gen(91)
+    q, k, v = (randn(g, 1, 1, 300, 16, dtype=F16) for _ in range(3))
+    index = torch.randint(0, 5, (1, 1, 300, 64), generator=g, device=DEV, dtype=torch.int32)
+    wide = lambda: ops.block_attention(q, k, v, index, 64)[0]  # noqa: E731
+    slim = lambda: ops.block_attention(q, k, v, index[..., :1].contiguous(), 64)[0]  # noqa: E731
+    want = wide(), slim()
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(lambda i: (wide, slim)[i % 2](), range(40)))
+    torch.cuda.synchronize()
+    assert torch.equal(wide(), want[0])
+    assert all(torch.equal(t, want[i % 2]) for i, t in enumerate(got))
+
+
 def test_python_refusals_on_the_gpu():
     x = torch.zeros(1, 2, 20, 16, device=DEV, dtype=F16)
     index = torch.zeros(1, 2, 20, 1, device=DEV, dtype=torch.int32)
