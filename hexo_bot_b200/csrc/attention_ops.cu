@@ -223,7 +223,7 @@ int ba_segments(int q_rows, int wq, int seg) {
 
 struct BaPlan {
   int marks, bh_step, wq, seg;
-  size_t entries, spans, slots, part, ml, delta, kv_part, total;
+  size_t ticket, entries, spans, slots, part, ml, delta, kv_part, total;
 };
 
 BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, int topk, bool backward) {
@@ -248,6 +248,8 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   p.seg = (int)seg;
   const long long rows = (long long)p.bh_step * p.wq * group;
   size_t at = 0;
+  p.ticket = at;
+  at += 256;
   p.entries = at;
   at += align256((size_t)bh * p.marks * kBaMark * topk * 2);
   p.spans = at;
@@ -330,7 +332,9 @@ struct LaunchFwd {
   cudaStream_t st;
   template <typename T, int DP, int BK>
   int operator()() const {
-    if (int s = launch_ba(block_attn_kernel<T, DP, BK>, "block_attn_kernel", (long long)a.nbh * a.nb * a.nseg, kBaFwdThreads,
+    const long long items = (long long)a.nbh * a.nb * a.nseg, most = (long long)num_sms() * ba_fwd_ctas<DP, BK>();
+    if (items > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "block_attention: too many blocks for one launch");
+    if (int s = launch_ba(block_attn_kernel<T, DP, BK>, "block_attn_kernel", items < most ? items : most, kBaFwdThreads,
                           ba_fwd_smem<DP, BK>(), a, st))
       return s;
     return launch_ba(block_attn_join_kernel<T>, "block_attn_join_kernel",
@@ -659,6 +663,7 @@ int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, 
   a.slots = (unsigned long long*)(ws + p.slots);
   a.part = (float*)(ws + p.part);
   a.ml = (float2*)(ws + p.ml);
+  a.ticket = (uint32_t*)(ws + p.ticket);
   if (int s = launch_ba(block_list_kernel, "block_list_kernel", (long long)batch * kv_heads * p.marks, kBaMark,
                         ba_list_smem(topk), a, st))
     return s;

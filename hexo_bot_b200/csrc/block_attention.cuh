@@ -24,6 +24,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "block_select.cuh"
 #include "ptx.cuh"
@@ -46,6 +47,7 @@ struct BaArgs {
   const int* q_lens;
   uint16_t* entries;      // (B Hkv, marks, kBaMark topk): per group, by block: place in the row's list << 8 | query
   uint32_t* spans;        // (B Hkv, nb, marks): first entry of the group's queries that chose the block | count << 16
+  uint32_t* ticket;       // work items of the forward's CTAs that have been taken; 0 before each launch
   unsigned long long* slots;  // (B Hkv, Sq): bit s = entry s of the row's list counts
   float* part;            // window's parts: [row][topk][dim], row = (local bh * wq + local i) * group + g
   float2* ml;             // forward: [row][topk] (max in log2 units, sum)
@@ -78,14 +80,14 @@ __device__ __forceinline__ int ba_q_len(const BaArgs& a, int b) {
 constexpr int kBaListWindow = 1024;  // blocks whose bits are in shared memory at once
 
 __host__ __device__ inline int ba_list_smem(int topk) {
-  return kBaListWindow * 8 * 4 + kBaListWindow * 4 + kBaMark * (topk | 1) * 4;
+  return kBaListWindow * 8 * 4 + kBaListWindow * 8 * 2 + kBaMark * (topk | 1) * 4;
 }
 
 __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
   extern __shared__ __align__(16) char list_smem[];
-  uint32_t* bits = reinterpret_cast<uint32_t*>(list_smem);  // [window][8]
-  uint32_t* offs = bits + kBaListWindow * 8;                // [window]
-  int* rows = reinterpret_cast<int*>(offs + kBaListWindow);  // [256][topk | 1]: odd rows meet distinct banks
+  uint32_t* bits = reinterpret_cast<uint32_t*>(list_smem);                    // [8][window]
+  uint16_t* offs = reinterpret_cast<uint16_t*>(bits + kBaListWindow * 8);     // [8][window]: first entry of a word's queries
+  int* rows = reinterpret_cast<int*>(offs + kBaListWindow * 8);  // [256][topk | 1]: odd rows meet distinct banks
   __shared__ uint32_t warp_sum[kBaMark / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.x / a.marks, mark = blockIdx.x - bh * a.marks;
@@ -95,34 +97,57 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
   const bool on = i < ba_q_len(a, b);
   const int have = min(kBaMark, a.q_rows - mark * kBaMark) * K;
   const int* src = a.idx + ((long long)bh * a.q_rows + (long long)mark * kBaMark) * K;
-  for (int x = tid; x < have; x += kBaMark) rows[x / K * KS + x % K] = src[x];
+  for (int x0 = tid; x0 < have; x0 += 8 * kBaMark) {  // eight loads in flight
+    int v[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) v[y] = x0 + y * kBaMark < have ? src[x0 + y * kBaMark] : 0;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      const int x = x0 + y * kBaMark;
+      if (x < have) rows[x / K * KS + x % K] = v[y];
+    }
+  }
+  __syncthreads();
+  // entries that count: in range, and not named before (lists as block_select
+  // writes them ascend, so the comparison with all before is rarely needed)
+  const int* mine = rows + tid * KS;
   unsigned long long counts = 0;
+  if (on) {
+    int last = -1;
+    for (int s = 0; s < K; ++s) {
+      const int j = mine[s];
+      if (j < 0 || j >= live) continue;
+      bool fresh = true;
+      if (j <= last)
+        for (int e = 0; e < s; ++e) fresh &= mine[e] != j;
+      last = max(last, j);
+      if (fresh) counts |= 1ull << s;
+    }
+  }
   uint32_t base = 0;
+  const uint32_t bit = 1u << lane;
   uint16_t* entries = a.entries + ((long long)bh * a.marks + mark) * kBaMark * K;
   for (int j0 = 0; j0 < a.nb; j0 += kBaListWindow) {
-    const int n = min(a.nb - j0, kBaListWindow);
-    for (int x = tid; x < n * 8; x += kBaMark) bits[x] = 0;
+    const int n = min(a.nb - j0, kBaListWindow), n4 = (n + 3) / 4;
+    for (int x = tid; x < 8 * n4; x += kBaMark) reinterpret_cast<uint4*>(bits + x / n4 * kBaListWindow)[x % n4] = uint4{};
     __syncthreads();
-    const uint32_t bit = 1u << lane;
-    if (on)
-      for (int s = 0; s < K; ++s) {
-        const int j = rows[tid * KS + s];
-        if (j < j0 || j >= j0 + n || j >= live) continue;
-        // this thread alone touches its bit, so the old value tells of a repetition
-        if (!(atomicOr(&bits[(j - j0) * 8 + warp], bit) & bit)) counts |= 1ull << s;
-      }
+    for (unsigned long long m = counts; m; m &= m - 1) {
+      const int j = mine[__ffsll(m) - 1] - j0;
+      if (j >= 0 && j < n) atomicOr(&bits[warp * kBaListWindow + j], bit);
+    }
     __syncthreads();
     // four blocks a thread: counts, and their exclusive sums over the window
-    uint32_t c[4], sum = 0;
+    uint32_t c[8][4], sum[4] = {0, 0, 0, 0}, total = 0;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      c[y] = 0;
-      if (tid * 4 + y < n)
+    for (int w = 0; w < 8; ++w) {
+      const uint4 v = tid < n4 ? reinterpret_cast<const uint4*>(bits + w * kBaListWindow)[tid] : uint4{};
+      c[w][0] = __popc(v.x); c[w][1] = __popc(v.y); c[w][2] = __popc(v.z); c[w][3] = __popc(v.w);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) c[y] += __popc(bits[(tid * 4 + y) * 8 + w]);
-      sum += c[y];
+      for (int y = 0; y < 4; ++y) sum[y] += c[w][y];
     }
-    uint32_t pre = sum;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) total += sum[y];
+    uint32_t pre = total;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t o = __shfl_up_sync(0xffffffffu, pre, d);
@@ -130,7 +155,7 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
     }
     if (lane == 31) warp_sum[warp] = pre;
     __syncthreads();
-    uint32_t at = base + pre - sum;
+    uint32_t at = base + pre - total;
 #pragma unroll
     for (int w = 0; w < kBaMark / 32; ++w) {
       if (w < warp) at += warp_sum[w];
@@ -138,24 +163,25 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      if (tid * 4 + y < n) {
-        offs[tid * 4 + y] = at;
-        a.spans[((long long)bh * a.nb + j0 + tid * 4 + y) * a.marks + mark] = at | c[y] << 16;
+      const int j = tid * 4 + y;
+      if (j < n) a.spans[((long long)bh * a.nb + j0 + j) * a.marks + mark] = at | sum[y] << 16;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (j < n) offs[w * kBaListWindow + j] = (uint16_t)at;
+        at += c[w][y];
       }
-      at += c[y];
     }
     __syncthreads();
-    if (on)
-      for (int s = 0; s < K; ++s) {
-        const int j = rows[tid * KS + s] - j0;
-        if (!(counts >> s & 1) || j < 0 || j >= n) continue;
-        uint32_t p = offs[j] + __popc(bits[j * 8 + warp] & (bit - 1));
-        for (int w = 0; w < warp; ++w) p += __popc(bits[j * 8 + w]);
-        entries[p] = (uint16_t)(s << 8 | tid);
-      }
+    for (unsigned long long m = counts; m; m &= m - 1) {
+      const int s = __ffsll(m) - 1, j = mine[s] - j0;
+      if (j < 0 || j >= n) continue;
+      const int p = offs[warp * kBaListWindow + j] + __popc(bits[warp * kBaListWindow + j] & (bit - 1));
+      entries[p] = (uint16_t)(s << 8 | tid);
+    }
     __syncthreads();
   }
   if (i < a.q_rows) a.slots[(long long)bh * a.q_rows + i] = counts;
+  if (blockIdx.x == 0 && tid == 0 && a.ticket) *a.ticket = 0;
 }
 
 // ---- shared-memory tiles ---------------------------------------------------------
@@ -208,16 +234,25 @@ __device__ __forceinline__ int ba_fill(const BaArgs& a, int bh, int j, int& g, i
   if (tid == 0) pos[0] = 0;
   const int taken = __syncthreads_count(in && pre <= kBaChunk);
   const int n = (int)pos[taken];
-  for (int e = tid; e < n; e += THREADS) {
-    int lo = 0, hi = taken - 1;  // the group that holds entry e
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pos[mid] <= (uint32_t)e) lo = mid;
-      else hi = mid - 1;
+  const uint16_t* entries = a.entries + ((long long)bh * a.marks + g) * kBaMark * a.topk;
+  for (int e0 = tid; e0 < n; e0 += 4 * THREADS) {  // four entries in flight
+    int lo[4];
+    uint32_t x[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int e = min(e0 + y * THREADS, n - 1);
+      int l = 0, hi = taken - 1;  // the group that holds entry e
+      while (l < hi) {
+        const int mid = (l + hi + 1) >> 1;
+        if (pos[mid] <= (uint32_t)e) l = mid;
+        else hi = mid - 1;
+      }
+      lo[y] = l;
+      x[y] = entries[(long long)l * kBaMark * a.topk + first[l] + (e - pos[l])];
     }
-    const uint32_t x =
-        a.entries[((long long)bh * a.marks + g + lo) * kBaMark * a.topk + first[lo] + (e - pos[lo])];
-    list[e] = (uint32_t)((g + lo) * kBaMark + (x & 255)) << 6 | x >> 8;
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (e0 + y * THREADS < n) list[e0 + y * THREADS] = (uint32_t)((g + lo[y]) * kBaMark + (x[y] & 255)) << 6 | x[y] >> 8;
   }
   g += taken;
   __syncthreads();
@@ -326,103 +361,322 @@ struct BaTile {
   }
 };
 
-// ---- forward, many queries -----------------------------------------------------
-constexpr int kBaFwdThreads = 128;
-constexpr int kBaFwdWarps = kBaFwdThreads / 32;
+// Writes row r (0 / 1) of an accumulator group (channels 16 n2 ... of two 8-wide
+// tiles) as 16-byte pieces: lane pairs swap halves so that even lanes hold four
+// channels of the first tile, odd lanes of the second.
+__device__ __forceinline__ void ba_store16(float* p, const float (&t0)[4], const float (&t1)[4], int r, int n2, int dim,
+                                           bool ok) {
+  const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1;
+  const float s0 = odd ? t0[2 * r] : t1[2 * r], s1 = odd ? t0[2 * r + 1] : t1[2 * r + 1];
+  const float g0 = __shfl_xor_sync(0xffffffffu, s0, 1), g1 = __shfl_xor_sync(0xffffffffu, s1, 1);
+  const int c = 16 * n2 + (odd ? 8 : 0) + 2 * (lane & 2);
+  const float4 v = odd ? make_float4(g0, g1, t1[2 * r], t1[2 * r + 1]) : make_float4(t0[2 * r], t0[2 * r + 1], g0, g1);
+  if (ok && c < dim) *reinterpret_cast<float4*>(p + c) = v;
+}
 
+// ---- forward, many queries -----------------------------------------------------
+// Tiles of 128 listed rows on the fifth-generation tensor cores, one row a
+// thread: S = Q K^T into TMEM; each thread reads its row of S, takes maximum,
+// exponentials and sum without any exchange and writes the 16-bit weights back
+// over S; O = P V with P as the TMEM operand; O leaves through the tile's own Q
+// buffer (transposed there, so that a part goes out in whole 128-byte lines).
+// Four CTAs an SM (128 TMEM columns each at D = 64) cover one another's waits.
+// An mma.sync form of this kernel, 16 rows a warp, took 134 us where this one
+// takes @@ (8192 rows, 8 heads of 64, 16 of 128 blocks): it issued 48
+// instructions a row and read every key and value fragment from shared memory
+// once per 16 rows (74 % of that pipe).
+//
+// Shared memory, rows of 128 bytes (64 channels; DP = 128: two panels) in the
+// 128-byte swizzle: K, V [panels][BK], Q [2][panels][128]. As a left or right
+// operand whose rows run over channels (Q, K) they are K-major; V, whose rows
+// run over keys of the sum, is an N-major operand of the same bytes.
+constexpr int kBaFwdThreads = 128;
+constexpr int kBaFwdRows = 128;
+
+__host__ __device__ constexpr int ba_panels(int dp) { return dp > 64 ? 2 : 1; }
+template <int DP, int BK>
+constexpr int ba_fwd_tmem() {
+  return BK + DP <= 64 ? 64 : BK + DP <= 128 ? 128 : 256;
+}
 template <int DP, int BK>
 constexpr int ba_fwd_smem() {
-  return 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2 + kBaChunk * 4;
+  constexpr int need = 1024 + ba_panels(DP) * (2 * BK + 2 * kBaFwdRows) * 128 + kBaChunk * 4 + kBaFwdRows * 12;
+  // no more CTAs on an SM than its 512 TMEM columns serve: an allocation never waits
+  constexpr int least = 232448 / (512 / ba_fwd_tmem<DP, BK>() + 1) + 1;
+  return need > least ? need : least;
+}
+__device__ __forceinline__ uint32_t ba_panel_at(uint32_t base, int rows, int row, int chunk) {
+  return base + (chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+// cp.async of key rows into panels (zero past `have` rows and past dim).
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void ba_load_panels(uint32_t dst, const T* src, long long stride, int have, int dim) {
+  constexpr int CH = DP / 8;
+#pragma unroll
+  for (int x0 = 0; x0 < ROWS * CH; x0 += kBaFwdThreads) {
+    const int x = x0 + threadIdx.x, r = x / CH, c = x % CH;
+    if (ROWS * CH % kBaFwdThreads && x >= ROWS * CH) break;
+    const bool ok = r < have && c * 8 < dim;
+    cp_async16(ba_panel_at(dst, ROWS, r, c), ok ? src + r * stride + c * 8 : src, ok ? 16 : 0);
+  }
+}
+// N columns of this thread's TMEM lane.
+template <int N>
+__device__ __forceinline__ void ba_tmem_ld(uint32_t taddr, float* v) {
+  static_assert(N == 16 || N == 32, "");
+  uint32_t r[N];
+  __syncwarp();
+  if constexpr (N == 32) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ba_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Descriptor of an operand whose rows of 64 elements run along M or N (swizzled
+// 128-byte rows, one row per K index): 8 K rows every 1024 bytes, further 64
+// elements of M / N `panel` bytes on.
+__device__ __forceinline__ uint64_t ba_mn_desc(uint32_t addr, uint32_t panel) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((panel >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+constexpr uint32_t kIdescBMn = 1u << 16;  // right operand N-major
+
+template <int DP, int BK>
+constexpr int ba_fwd_ctas() {  // of an SM: by TMEM columns, and by its 228 KB (2 KB a CTA beside the dynamic part)
+  constexpr int t = 512 / ba_fwd_tmem<DP, BK>(), m = 233472 / (ba_fwd_smem<DP, BK>() + 2048);
+  return t < m ? t : m;
 }
 
 template <typename T, int DP, int BK>
-__global__ __launch_bounds__(kBaFwdThreads) void block_attn_kernel(const BaArgs a) {
-  extern __shared__ __align__(128) char ba_smem[];
-  const uint32_t ks = smem_u32(ba_smem), vs = ks + BK * DP * 2;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t qs = vs + BK * DP * 2 + warp * (2 * 16 * DP * 2);
-  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * BK * DP * 2 + kBaFwdWarps * 2 * 16 * DP * 2);
-  const uint32_t u = blockIdx.x;
-  const int sg = (int)(u % (uint32_t)a.nseg);
-  const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
-  const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  int g = a.w0 / kBaMark + sg * a.seg;
-  const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
-  const int have = min(BK, ba_kv_len(a, b) - j * BK);
-  if (have <= 0) return;
-  const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s;
-  const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s;
+__global__ __launch_bounds__(kBaFwdThreads, ba_fwd_ctas<DP, BK>()) void block_attn_kernel(const BaArgs a) {
+  constexpr int PAN = ba_panels(DP), CH = DP / 8, ROWS = kBaFwdRows;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t KB = PAN * BK * 128, QB = PAN * ROWS * 128;
+  constexpr int SH = BK < 64 ? BK : 64;  // scores a thread holds at a time
+  constexpr int OW = DP < 32 ? DP : 32;  // output channels staged at a time
+  extern __shared__ char ba_smem_raw[];
+  char* ba_smem = ba_smem_raw + (1024 - (smem_u32(ba_smem_raw) & 1023)) % 1024;
+  const uint32_t ks = smem_u32(ba_smem), vs = ks + KB, qs = vs + KB;
+  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB);
+  long long* qoff = reinterpret_cast<long long*>(list + kBaChunk);  // [128]: rows of the tile being loaded
+  int* dst = reinterpret_cast<int*>(qoff + ROWS);                    // [128]: parts of the tile being stored
+  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ uint32_t tmem_slot;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ uint32_t next_item;
+  const uint32_t items = (uint32_t)a.nbh * (uint32_t)a.nb * (uint32_t)a.nseg;
   const int G = a.group;
-  const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
-  constexpr int CH = DP / 8;
-  bool loaded = false;
-  while (g < end) {
-    const int n = ba_fill<kBaFwdThreads>(a, bh, j, g, end, list);
-    if (n == 0) continue;
-    if (!loaded) {
-      ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
-      ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, kBaFwdThreads);
-    }
-    cp_async_commit();
-    const int rows = n * G;
-    auto load_q = [&](int tile, uint32_t dst) {
-#pragma unroll
-      for (int x0 = 0; x0 < 16 * CH; x0 += 32) {
-        const int x = x0 + lane;
-        const int r = x / CH, c = x % CH;
-        const int row = tile * 16 + r;
-        const bool ok = row < rows && c * 8 < a.dim;
-        const T* src = qp;
-        if (ok) {
-          const int li = ba_div_group(a, row), gr = row - li * G;
-          src = qp + gr * a.q.h + (long long)(list[li] >> 6) * a.q.s + c * 8;
-        }
-        cp_async16(ba_at<DP>(dst, r, c), src, ok ? 16 : 0);
-      }
-    };
-    const int tiles = (rows + 15) / 16;
-    if (warp < tiles) load_q(warp, qs);
-    cp_async_commit();
-    if (!loaded) {
-      cp_async_wait<1>();
-      __syncthreads();
-      loaded = true;
-    }
-    int buf = 0;
-    for (int t = warp; t < tiles; t += kBaFwdWarps, buf ^= 1) {
-      const uint32_t qt = qs + buf * (16 * DP * 2);
-      if (t + kBaFwdWarps < tiles) load_q(t + kBaFwdWarps, qs + (buf ^ 1) * (16 * DP * 2));
-      cp_async_commit();
-      // this lane's two rows: where their parts go
-      long long at[2];
-      bool ok[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = t * 16 + (lane >> 2) + 8 * r;
-        ok[r] = row < rows;
-        const int li = ok[r] ? ba_div_group(a, row) : 0, gr = row - li * G;
-        const uint32_t e = list[li];
-        at[r] = (((long long)lbh * a.wq + ((int)(e >> 6) - a.w0)) * G + gr) * a.topk + (e & 63);
-      }
-      cp_async_wait<1>();
-      __syncwarp();
-      BaTile<T, DP, BK> tile;
-      tile.run(qt, ks, vs, have, a.scale_log2);
-      __syncwarp();  // the buffer is free for the tile after next
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (!ok[r]) continue;
-        if ((lane & 3) == 0) a.ml[at[r]] = make_float2(tile.m[r], tile.l[r]);
-        float* p = a.part + at[r] * a.dim;
-#pragma unroll
-        for (int nn = 0; nn < DP / 8; ++nn)
-          if (nn * 8 < a.dim)
-            *reinterpret_cast<float2*>(p + nn * 8 + 2 * (lane & 3)) =
-                make_float2(tile.o[nn][2 * r], tile.o[nn][2 * r + 1]);
-      }
-    }
+  const uint32_t bar_s = smem_u32(&bars[0]), bar_o = smem_u32(&bars[1]);
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), ba_fwd_tmem<DP, BK>());
+    tmem_relinquish();
   }
+  if (tid == 0) {
+    mbar_init(bar_s, 1);
+    mbar_init(bar_o, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+  uint32_t phase = 0;
+  for (uint32_t u = blockIdx.x; u < items;) {
+    const int sg = (int)(u % (uint32_t)a.nseg);
+    const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
+    const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
+    const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+    int g = a.w0 / kBaMark + sg * a.seg;
+    const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
+    const int have = min(BK, ba_kv_len(a, b) - j * BK);
+    __syncthreads();  // the item before is done with the keys, and its successor has been read
+    if (tid == 0) next_item = gridDim.x + atomicAdd(a.ticket, 1u);
+    if (have <= 0) g = end;
+    const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
+    // on their way while the list is made
+    if (have > 0) {
+    ba_load_panels<T, DP, BK>(ks, (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s, a.k.s, have, a.dim);
+    ba_load_panels<T, DP, BK>(vs, (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s, a.v.s, have, a.dim);
+    }
+    while (g < end) {
+      const int n = ba_fill<kBaFwdThreads>(a, bh, j, g, end, list);
+      if (n == 0) continue;
+      const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
+      // a warp loads the 32 rows whose offsets its lanes worked out
+      auto load_q = [&](int tile, uint32_t to) {
+        const int row = tile * ROWS + tid;
+        long long off = -1;
+        if (row < rows) {
+          const int li = ba_div_group(a, row);
+          off = (row - li * G) * a.q.h + (long long)(list[li] >> 6) * a.q.s;
+        }
+        qoff[tid] = off;
+        __syncwarp();
+#pragma unroll
+        for (int x0 = 0; x0 < 32 * CH; x0 += 32) {
+          const int r = warp * 32 + (x0 + lane) / CH, c = (x0 + lane) % CH;
+          const long long o = qoff[r];
+          const bool in = o >= 0 && c * 8 < a.dim;
+          cp_async16(ba_panel_at(to, ROWS, r, c), in ? qp + o + c * 8 : qp, in ? 16 : 0);
+        }
+        __syncwarp();
+      };
+      load_q(0, qs);
+      cp_async_commit();
+      for (int t = 0; t < tiles; ++t) {
+        const uint32_t qt = qs + (t & 1) * QB;
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();  // Q of this tile is there; every thread has read the O of the one before
+        tc_fence_after();
+        const uint32_t s_tm = tmem, o_tm = tmem + BK, lanes = (uint32_t)(warp * 32) << 16;
+        if (tid == 0) {
+          constexpr uint32_t id = mma_idesc(BK, BF);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            tc_mma_f16(s_tm, sw128_desc(qt + kk / 4 * ROWS * 128 + kk % 4 * 32), sw128_desc(ks + kk / 4 * BK * 128 + kk % 4 * 32),
+                       id, kk > 0);
+          tc_commit(bar_s);
+        }
+        if (t + 1 < tiles) load_q(t + 1, qs + ((t + 1) & 1) * QB);
+        cp_async_commit();
+        ok = ok && mbar_wait(bar_s, phase);
+        tc_fence_after();
+        // this thread's row: maximum, weights, sum
+        const float sc = fmaxf(fabsf(a.scale_log2), 1e-38f);  // not 0: masked scores stay -inf
+        const bool flip = a.scale_log2 < 0.f;
+        float s[SH], m = -INFINITY, l = 0.f;
+        auto load_s = [&](int c0) {
+#pragma unroll
+          for (int x = 0; x < SH; x += 32) ba_tmem_ld<32>(s_tm + lanes + c0 + x, s + x);
+          if (flip) {
+#pragma unroll
+            for (int x = 0; x < SH; ++x) s[x] = -s[x];
+          }
+          if (have < BK) {
+#pragma unroll
+            for (int x = 0; x < SH; ++x)
+              if (c0 + x >= have) s[x] = -INFINITY;
+          }
+        };
+#pragma unroll
+        for (int c0 = 0; c0 < BK; c0 += SH) {
+          load_s(c0);
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int x = 0; x < SH; ++x) m4[x & 3] = fmaxf(m4[x & 3], s[x]);
+          m = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        }
+        // -inf (no score above it: the row keeps weight 0) or the maximum in log2 units
+        const float ref = m == -INFINITY ? 0.f : m * sc;
+        m = m == -INFINITY ? m : ref;
+#pragma unroll
+        for (int c0 = 0; c0 < BK; c0 += SH) {
+          if (BK > SH) load_s(c0);
+          // weights go to the matrix unit in the inputs' 16-bit type (half a step of
+          // rounding each, averaged over the keys); their sum l stays in 32 bits
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < SH; c += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float p0 = ba_exp2(fmaf(s[c + 2 * x], sc, -ref)), p1 = ba_exp2(fmaf(s[c + 2 * x + 1], sc, -ref));
+              l4[x & 3] += p0 + p1;
+              w[x] = MmaTraits<T>::pack(p0, p1);
+            }
+            ba_tmem_st16(s_tm + lanes + (c0 + c) / 2, w);
+          }
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          constexpr uint32_t id = mma_idesc(DP, BF) | kIdescBMn;
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            tc_mma_f16_ts(o_tm, s_tm + kk * 8, ba_mn_desc(vs + kk * 2048, BK * 128), id, kk > 0);
+          tc_commit(bar_o);
+        }
+        // where this row's part goes (a window's parts number less than 2^31)
+        const int row = t * ROWS + tid;
+        int at = -1;
+        if (row < rows) {
+          const int li = ba_div_group(a, row);
+          const uint32_t e = list[li];
+          at = ((lbh * a.wq + ((int)(e >> 6) - a.w0)) * G + (row - li * G)) * a.topk + (int)(e & 63);
+          // a wait that gave up leaves no number behind
+          a.ml[at] = ok ? make_float2(m, l) : make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+        }
+        dst[tid] = at;
+        ok = ok && mbar_wait(bar_o, phase);
+        phase ^= 1;
+        tc_fence_after();
+        // O to its parts: a warp's 32 rows through the Q tile's bytes (S is done with them)
+        const uint32_t stage = qt + warp * 32 * 128;
+#pragma unroll
+        for (int c0 = 0; c0 < DP; c0 += OW) {
+          float o[OW];
+          ba_tmem_ld<OW>(o_tm + lanes + c0, o);
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < OW; x += 4)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + lane * 128 + (((x / 4) ^ (lane & 7)) << 4)),
+                         "f"(o[x]), "f"(o[x + 1]), "f"(o[x + 2]), "f"(o[x + 3])
+                         : "memory");
+          __syncwarp();
+          constexpr int LR = OW / 4;  // lanes of a row
+#pragma unroll
+          for (int x = 0; x < LR; ++x) {
+            const int r = x * (32 / LR) + lane / LR, c = lane % LR;
+            const uint4 v = lds128(stage + r * 128 + ((c ^ (r & 7)) << 4));
+            const int to = dst[warp * 32 + r];
+            if (to >= 0 && c0 + c * 4 < a.dim)
+              *reinterpret_cast<uint4*>(a.part + (long long)to * a.dim + c0 + c * 4) = v;
+          }
+        }
+      }
+    }
+    cp_async_wait_all();  // keys of an item that nobody chose
+    __syncthreads();
+    u = next_item;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, ba_fwd_tmem<DP, BK>());
 }
 
 // A row's place in the window, for the kernels that join parts: 2^cl lanes of
@@ -464,6 +718,7 @@ __device__ __forceinline__ void ba_strand_sum(float (&acc)[8], const BaRow& r) {
 // Joins the parts of each row, four parts a lane in flight.
 template <typename T>
 __global__ __launch_bounds__(kBaJoinThreads) void block_attn_join_kernel(const BaArgs a) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;  // for the next window
   const BaRow r(a);
   const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
   const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
@@ -693,7 +948,7 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
   char* tail = ba_smem + 2 * BK * DP * 2 + 4 * TILE + BK * TR * 2;
   // per row of a tile: (lse in log2 units, delta) and where its dq part goes
   float2* stat = reinterpret_cast<float2*>(tail);                    // [2][TR]
-  long long* dst = reinterpret_cast<long long*>(tail + 2 * TR * 8);  // [2][TR]
+  int* dst = reinterpret_cast<int*>(tail + 2 * TR * 8);              // [2][TR]
   uint32_t* list = reinterpret_cast<uint32_t*>(tail + 2 * TR * 16);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t u = blockIdx.x;
@@ -729,7 +984,7 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
     for (int r = threadIdx.x; r < TR; r += THREADS) {
       const int row = t * TR + r;
       float2 st = make_float2(INFINITY, 0.f);  // rows that are not there: weight 0
-      long long to = -1;
+      int to = -1;
       if (row < rows) {
         const int li = ba_div_group(a, row), g = row - li * G;
         const uint32_t e = list[li];
@@ -738,7 +993,7 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
         // a row all of whose scores are -inf has no weights
         const float l = a.lse[((long long)b * a.kv_heads * G + h * G + g) * a.q_rows + i];
         st = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, a.delta[qrow * G + g]);
-        to = (((long long)lbh * a.wq + (i - a.w0)) * G + g) * a.topk + (e & 63);
+        to = ((lbh * a.wq + (i - a.w0)) * G + g) * a.topk + (int)(e & 63);
       }
       stat[buf * TR + r] = st;
       dst[buf * TR + r] = to;
@@ -856,11 +1111,8 @@ __global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) 
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const long long to = dst[buf * TR + mt * 16 + (lane >> 2) + 8 * r];
-          if (to < 0) continue;
-          float* p = a.part + to * a.dim + nt * 16 + 2 * (lane & 3);
-          *reinterpret_cast<float2*>(p) = make_float2(acc[0][2 * r], acc[0][2 * r + 1]);
-          if (nt * 16 + 8 < a.dim) *reinterpret_cast<float2*>(p + 8) = make_float2(acc[1][2 * r], acc[1][2 * r + 1]);
+          const int to = dst[buf * TR + mt * 16 + (lane >> 2) + 8 * r];
+          ba_store16(a.part + (long long)to * a.dim, acc[0], acc[1], r, nt, a.dim, to >= 0);
         }
       }
       __syncthreads();  // ds, the tile and its stats are written over from here on

@@ -565,7 +565,7 @@ __device__ __forceinline__ void sel_split8(const float (&x)[8], __nv_bfloat16* h
 
 // PER > 0: rows of up to 8 PER blocks, settled four a warp; 0: a warp a row.
 template <typename T, int PER>
-__global__ __launch_bounds__(kSelThreads) void block_select_kernel(const SelArgs a) {
+__global__ __launch_bounds__(kSelThreads, 3) void block_select_kernel(const SelArgs a) {
   extern __shared__ __align__(16) char sel_smem[];
   const int D = a.dim, DP = sel_dp(D), RS = DP + 8, NBS = sel_stride(a.nb), TQ = a.tile, TQ16 = max(TQ, 16);
   float* sc = reinterpret_cast<float*>(sel_smem);
