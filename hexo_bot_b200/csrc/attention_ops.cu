@@ -208,11 +208,11 @@ int launch_select_few(const SelArgs& a, unsigned rows, int cluster, cudaStream_t
 // 64 MB, 278 with 100, 255 with 200, 234 with one of 277 MB.
 constexpr long long kBaWindowBytes = 1ll << 30;
 constexpr int kBaFewRows = 16;      // up to so many queries take the few-query kernel
-// Listed rows per CTA that a segment aims at. Forward, the same case / 16 x 2440
-// rows of 16 over 39 blocks: 229 / 187 us at 128, 219 / 170 at 256, 228 / 157 at
-// 512; backward, the same case: 510 us at 128, 441 at 256, 425 at 512.
-constexpr int kBaFwdTarget = 384;
-constexpr int kBaBwdTarget = 512;
+// Work items an SM and window, and the listed rows that an item may hold: fewer
+// items leave SMs idle behind popular blocks (8192 rows, 8 heads of 64, 16 of 128
+// blocks, forward: 211 us with 8 an SM, 201 with 16 to 32; backward 404 / 410 /
+// 423 us with 8 / 16 / 24), smaller ones repeat the listing and the key loads.
+constexpr int kBaItems = 16, kBaMinTarget = 256, kBaMaxTarget = 1024;
 
 // Segments of `seg` list groups over all windows of wq rows.
 int ba_segments(int q_rows, int wq, int seg) {
@@ -240,12 +240,15 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
     const long long w = kBaWindowBytes / row_bytes / kBaMark * kBaMark;
     p.wq = (int)(w < kBaMark ? kBaMark : w);
   }
-  // a segment: as many groups as give a CTA its target of listed rows on average
-  const long long target = backward ? kBaBwdTarget : kBaFwdTarget;
+  // a segment: as many groups as give a work item its target of listed rows on
+  // average (several items a CTA, to even out popular blocks), evenly split
+  const long long pairs = (long long)p.bh_step * p.wq * topk * group;
+  long long target = pairs / (kBaItems * num_sms());
+  target = target < kBaMinTarget ? kBaMinTarget : target > kBaMaxTarget ? kBaMaxTarget : target;
+  const long long groups = cdiv(p.wq, kBaMark);
   long long seg = cdiv(target * nb, (long long)topk * group * kBaMark);
-  if (seg < 1) seg = 1;
-  if (seg > cdiv(p.wq, kBaMark)) seg = cdiv(p.wq, kBaMark);
-  p.seg = (int)seg;
+  seg = seg < 1 ? 1 : seg > groups ? groups : seg;
+  p.seg = (int)cdiv(groups, cdiv(groups, seg));
   const long long rows = (long long)p.bh_step * p.wq * group;
   size_t at = 0;
   p.ticket = at;
@@ -317,6 +320,13 @@ int launch_ba(K kern, const char* name, long long grid, int threads, int smem, c
   return check_launch(name);
 }
 
+int launch_list(const BaArgs& a, cudaStream_t st) {
+  const long long grid = (long long)a.batch * a.kv_heads * a.marks;
+  const int smem = ba_list_smem(a.nb, a.topk);
+  if (a.topk <= 8) return launch_ba(block_list_kernel<8>, "block_list_kernel", grid, kBaMark, smem, a, st);
+  if (a.topk <= 16) return launch_ba(block_list_kernel<16>, "block_list_kernel", grid, kBaMark, smem, a, st);
+  return launch_ba(block_list_kernel<kBaMaxTopk>, "block_list_kernel", grid, kBaMark, smem, a, st);
+}
 struct LaunchFew {
   const BaArgs& a;
   cudaStream_t st;
@@ -664,9 +674,7 @@ int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, 
   a.part = (float*)(ws + p.part);
   a.ml = (float2*)(ws + p.ml);
   a.ticket = (uint32_t*)(ws + p.ticket);
-  if (int s = launch_ba(block_list_kernel, "block_list_kernel", (long long)batch * kv_heads * p.marks, kBaMark,
-                        ba_list_smem(topk), a, st))
-    return s;
+  if (int s = launch_list(a, st)) return s;
   return ba_windows(a, p, [&] { return ba_dispatch(dtype, head_dim, block, LaunchFwd{a, st}); });
 }
 
@@ -719,7 +727,7 @@ int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const s
   a.kv_part = (float*)(ws + p.kv_part);
   a.nseg_all = ba_segments(q_rows, p.wq, p.seg);
   cudaStream_t st = (cudaStream_t)stream;
-  if (int s = launch_ba(block_list_kernel, "block_list_kernel", bh * p.marks, kBaMark, ba_list_smem(topk), a, st)) return s;
+  if (int s = launch_list(a, st)) return s;
   const int chunks = 1 << pow2_log2(head_dim / 8);
   const long long dgrid = cdiv(bh * q_rows * a.group * chunks, 256);
   const bool f16 = dtype == SB_F16;

@@ -79,68 +79,64 @@ __device__ __forceinline__ int ba_q_len(const BaArgs& a, int b) {
 // repeated entries: `slots` marks the entries that count.
 constexpr int kBaListWindow = 1024;  // blocks whose bits are in shared memory at once
 
-__host__ __device__ inline int ba_list_smem(int topk) {
-  return kBaListWindow * 8 * 4 + kBaListWindow * 8 * 2 + kBaMark * (topk | 1) * 4;
+__host__ __device__ inline int ba_list_window(int nb) { return nb < kBaListWindow ? (nb + 3) / 4 * 4 : kBaListWindow; }
+__host__ __device__ inline int ba_list_smem(int nb, int topk) {
+  return ba_list_window(nb) * 8 * (4 + 2) + kBaMark * topk * 2;
 }
 
+// KR: entries of a list that a thread holds in registers (topk <= KR).
+template <int KR>
 __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
   extern __shared__ __align__(16) char list_smem[];
-  uint32_t* bits = reinterpret_cast<uint32_t*>(list_smem);                    // [8][window]
-  uint16_t* offs = reinterpret_cast<uint16_t*>(bits + kBaListWindow * 8);     // [8][window]: first entry of a word's queries
-  int* rows = reinterpret_cast<int*>(offs + kBaListWindow * 8);  // [256][topk | 1]: odd rows meet distinct banks
+  const int W = ba_list_window(a.nb), K = a.topk;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(list_smem);       // [8][W]
+  uint16_t* offs = reinterpret_cast<uint16_t*>(bits + 8 * W);    // [8][W]: first entry of a word's queries
+  uint16_t* sorted = offs + 8 * W;                               // [256 topk]
   __shared__ uint32_t warp_sum[kBaMark / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.x / a.marks, mark = blockIdx.x - bh * a.marks;
-  const int b = bh / a.kv_heads, K = a.topk, KS = K | 1;
+  const int b = bh / a.kv_heads;
   const int i = mark * kBaMark + tid;
-  const int live = (ba_kv_len(a, b) + a.block - 1) / a.block;
-  const bool on = i < ba_q_len(a, b);
-  const int have = min(kBaMark, a.q_rows - mark * kBaMark) * K;
-  const int* src = a.idx + ((long long)bh * a.q_rows + (long long)mark * kBaMark) * K;
-  for (int x0 = tid; x0 < have; x0 += 8 * kBaMark) {  // eight loads in flight
-    int v[8];
+  const bool on = i < a.q_rows;
+  const int* src = a.idx + ((long long)bh * a.q_rows + i) * K;
+  int e[KR];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) v[y] = x0 + y * kBaMark < have ? src[x0 + y * kBaMark] : 0;
+  for (int s = 0; s < KR; ++s) e[s] = on && s < K ? src[s] : -1;
+  const int live = i < ba_q_len(a, b) ? (ba_kv_len(a, b) + a.block - 1) / a.block : 0;
+  // lists as block_select writes them ascend; in any other a block may be named twice
+  bool ascends = true;
+  int last = -1;
 #pragma unroll
-    for (int y = 0; y < 8; ++y) {
-      const int x = x0 + y * kBaMark;
-      if (x < have) rows[x / K * KS + x % K] = v[y];
-    }
-  }
-  __syncthreads();
-  // entries that count: in range, and not named before (lists as block_select
-  // writes them ascend, so the comparison with all before is rarely needed)
-  const int* mine = rows + tid * KS;
-  unsigned long long counts = 0;
-  if (on) {
-    int last = -1;
-    for (int s = 0; s < K; ++s) {
-      const int j = mine[s];
-      if (j < 0 || j >= live) continue;
-      bool fresh = true;
-      if (j <= last)
-        for (int e = 0; e < s; ++e) fresh &= mine[e] != j;
-      last = max(last, j);
-      if (fresh) counts |= 1ull << s;
+  for (int s = 0; s < KR; ++s) {
+    if (e[s] < 0 || e[s] >= live) {
+      e[s] = -1;
+    } else {
+      ascends = ascends && e[s] > last;
+      last = e[s];
     }
   }
   uint32_t base = 0;
   const uint32_t bit = 1u << lane;
-  uint16_t* entries = a.entries + ((long long)bh * a.marks + mark) * kBaMark * K;
-  for (int j0 = 0; j0 < a.nb; j0 += kBaListWindow) {
-    const int n = min(a.nb - j0, kBaListWindow), n4 = (n + 3) / 4;
-    for (int x = tid; x < 8 * n4; x += kBaMark) reinterpret_cast<uint4*>(bits + x / n4 * kBaListWindow)[x % n4] = uint4{};
+  for (int j0 = 0; j0 < a.nb; j0 += W) {
+    const int n = min(a.nb - j0, W), n4 = W / 4;
+    for (int x = tid; x < 8 * n4; x += kBaMark) reinterpret_cast<uint4*>(bits)[x] = uint4{};
     __syncthreads();
-    for (unsigned long long m = counts; m; m &= m - 1) {
-      const int j = mine[__ffsll(m) - 1] - j0;
-      if (j >= 0 && j < n) atomicOr(&bits[warp * kBaListWindow + j], bit);
+    if (ascends) {
+#pragma unroll
+      for (int s = 0; s < KR; ++s)
+        if (e[s] >= j0 && e[s] < j0 + n) atomicOr(&bits[warp * W + e[s] - j0], bit);
+    } else {
+      // this thread alone touches its bit, so the old value tells of a repetition
+#pragma unroll
+      for (int s = 0; s < KR; ++s)
+        if (e[s] >= j0 && e[s] < j0 + n && (atomicOr(&bits[warp * W + e[s] - j0], bit) & bit)) e[s] = -1;
     }
     __syncthreads();
     // four blocks a thread: counts, and their exclusive sums over the window
     uint32_t c[8][4], sum[4] = {0, 0, 0, 0}, total = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const uint4 v = tid < n4 ? reinterpret_cast<const uint4*>(bits + w * kBaListWindow)[tid] : uint4{};
+      const uint4 v = tid < n4 ? reinterpret_cast<const uint4*>(bits + w * W)[tid] : uint4{};
       c[w][0] = __popc(v.x); c[w][1] = __popc(v.y); c[w][2] = __popc(v.z); c[w][3] = __popc(v.w);
 #pragma unroll
       for (int y = 0; y < 4; ++y) sum[y] += c[w][y];
@@ -167,20 +163,26 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
       if (j < n) a.spans[((long long)bh * a.nb + j0 + j) * a.marks + mark] = at | sum[y] << 16;
 #pragma unroll
       for (int w = 0; w < 8; ++w) {
-        if (j < n) offs[w * kBaListWindow + j] = (uint16_t)at;
+        if (j < n) offs[w * W + j] = (uint16_t)at;
         at += c[w][y];
       }
     }
     __syncthreads();
-    for (unsigned long long m = counts; m; m &= m - 1) {
-      const int s = __ffsll(m) - 1, j = mine[s] - j0;
-      if (j < 0 || j >= n) continue;
-      const int p = offs[warp * kBaListWindow + j] + __popc(bits[warp * kBaListWindow + j] & (bit - 1));
-      entries[p] = (uint16_t)(s << 8 | tid);
+#pragma unroll
+    for (int s = 0; s < KR; ++s) {
+      const int j = e[s] - j0;
+      if (e[s] >= 0 && j >= 0 && j < n)
+        sorted[offs[warp * W + j] + __popc(bits[warp * W + j] & (bit - 1))] = (uint16_t)(s << 8 | tid);
     }
     __syncthreads();
   }
-  if (i < a.q_rows) a.slots[(long long)bh * a.q_rows + i] = counts;
+  // out in 16-byte pieces (the group's place holds 256 topk entries)
+  uint4* dst = reinterpret_cast<uint4*>(a.entries + ((long long)bh * a.marks + mark) * kBaMark * K);
+  for (int x = tid; x < ((int)base + 7) / 8; x += kBaMark) dst[x] = reinterpret_cast<const uint4*>(sorted)[x];
+  unsigned long long counts = 0;
+#pragma unroll
+  for (int s = 0; s < KR; ++s) counts |= (unsigned long long)(e[s] >= 0) << s;
+  if (on) a.slots[(long long)bh * a.q_rows + i] = counts;
   if (blockIdx.x == 0 && tid == 0 && a.ticket) *a.ticket = 0;
 }
 
