@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
@@ -44,7 +45,7 @@ def _check(t: torch.Tensor, name: str, like: torch.Tensor, shape: Sequence[int],
         raise ValueError(f"{name} must be a tensor on {like.device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -84,23 +85,17 @@ def _lens(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> Optional[
     return t.data_ptr()
 
 
-class _On:
-    """The tensors' device as the current one for a call, and its stream."""
-
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-        self.stream = torch.cuda.current_stream(t.device).cuda_stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(t: torch.Tensor, what: str, fn, *args) -> None:
+    """fn(*args, stream) on t's device and its current stream; raises on a refusal."""
+    index = t.device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, what)
 
 
 def _wants_grad(*ts) -> bool:
@@ -120,12 +115,17 @@ def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, device="cuda")
     return torch.tensor(table, dtype=torch.float64, device=device)
 
 
-def _rotary(x, coords, freqs, sections, adjacent) -> Optional[_lib.Rotary]:
-    b, _, s, d = x.shape
-    sections = tuple(int(n) for n in sections)
+@lru_cache(maxsize=64)
+def _sections(sections):
+    """Pairs in all and the C array of checked section sizes."""
     if not 1 <= len(sections) <= 4 or min(sections) < 1:
         raise ValueError(f"sections must be 1 to 4 positive pair counts, got {sections}")
-    pairs = sum(sections)
+    return sum(sections), (C.c_int * 4)(*sections)
+
+
+def _rotary(x, coords, freqs, sections, adjacent) -> Optional[_lib.Rotary]:
+    b, _, s, d = x.shape
+    pairs, parts = _sections(tuple(sections))
     if 2 * pairs > d:
         raise ValueError(f"{pairs} pairs do not fit head_dim {d}")
     if not isinstance(coords, torch.Tensor) or coords.dim() != 3 or coords.dtype not in _COORDS:
@@ -138,8 +138,8 @@ def _rotary(x, coords, freqs, sections, adjacent) -> Optional[_lib.Rotary]:
     if not freqs.is_contiguous():
         raise ValueError("freqs must be contiguous")
     st = coords.stride()
-    return _lib.Rotary(coords.data_ptr(), _COORDS[coords.dtype], st[0], st[1], st[2], s - n, len(sections),
-                       (C.c_int * 4)(*sections), int(adjacent), freqs.data_ptr())
+    return _lib.Rotary(coords.data_ptr(), _COORDS[coords.dtype], st[0], st[1], st[2], s - n, len(sections), parts,
+                       adjacent, freqs.data_ptr())
 
 
 def _turn(x, coords, freqs, sections, adjacent, inverse, out=None):
@@ -147,8 +147,7 @@ def _turn(x, coords, freqs, sections, adjacent, inverse, out=None):
     rot = _rotary(x, coords, freqs, sections, adjacent)
     y = torch.empty_like(x) if out is None else _check(out, "out", x, x.shape, x.dtype)
     hx, hy = _heads(x, "x"), _heads(y, "out")
-    with _On(x) as st:
-        _lib.check(_lib.lib().sb_axes_rotary(hx, _FLOATS[x.dtype], rot, int(inverse), b, h, s, d, hy, st), "axes_rotary")
+    _call(x, "axes_rotary", _lib.lib().sb_axes_rotary, hx, _FLOATS[x.dtype], rot, inverse, b, h, s, d, hy)
     return y
 
 
@@ -216,9 +215,8 @@ def _qk(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps):
     sizes, dt, wdt, rot = _qk_args(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps)
     qo, ko = torch.empty_like(q), torch.empty_like(k)
     ins, outs = (_heads(q, "q"), _heads(k, "k")), (_heads(qo, "q"), _heads(ko, "k"))
-    with _On(q) as st:
-        _lib.check(_lib.lib().sb_qk_norm_rotary(*ins, dt, _ptr(q_weight), _ptr(k_weight), wdt, eps, rot, *sizes, *outs, st),
-                   "qk_norm_rotary")
+    _call(q, "qk_norm_rotary", _lib.lib().sb_qk_norm_rotary, *ins, dt, _ptr(q_weight), _ptr(k_weight), wdt, eps, rot, *sizes,
+          *outs)
     return qo, ko
 
 
@@ -238,10 +236,8 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, coords, fr
     ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
     gs = _heads(dq_out, "dq_out"), _heads(dk_out, "dk_out")
     ins, outs = (_heads(q, "q"), _heads(k, "k")), (_heads(dq, "dq"), _heads(dk, "dk"))
-    with _On(q) as st:
-        _lib.check(lib.sb_qk_norm_rotary_backward(*gs, *ins, dt, _ptr(q_weight), _ptr(k_weight), wdt, eps, rot, *sizes, *outs,
-                                                  _ptr(dqw), _ptr(dkw), ws.data_ptr(), need.value, st),
-                   "qk_norm_rotary_backward")
+    _call(q, "qk_norm_rotary_backward", lib.sb_qk_norm_rotary_backward, *gs, *ins, dt, _ptr(q_weight), _ptr(k_weight), wdt,
+          eps, rot, *sizes, *outs, _ptr(dqw), _ptr(dkw), ws.data_ptr(), need.value)
     return dq, dk, dqw, dkw
 
 
@@ -283,8 +279,7 @@ def block_means(k, block, *, kv_lens=None):
         raise ValueError(f"block must be positive, got {block}")
     out = torch.empty(b, h, -(-s // block), d, dtype=torch.float32, device=k.device)
     lens, hk = _lens(kv_lens, "kv_lens", k), _heads(k, "k")
-    with _On(k) as st:
-        _lib.check(_lib.lib().sb_block_means(hk, _FLOATS[k.dtype], lens, b, h, s, d, block, out.data_ptr(), st), "block_means")
+    _call(k, "block_means", _lib.lib().sb_block_means, hk, _FLOATS[k.dtype], lens, b, h, s, d, block, out.data_ptr())
     return out
 
 
@@ -307,9 +302,8 @@ def block_select(q, means, topk, block, kv_rows, *, kv_lens=None, q_lens=None, k
         raise ValueError("means must be contiguous")
     out = torch.empty(b, hk, sq, topk, dtype=torch.int32, device=q.device)
     kl, ql, hq_view = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q), _heads(q, "q")
-    with _On(q) as st:
-        _lib.check(_lib.lib().sb_block_select(hq_view, _FLOATS[q.dtype], means.data_ptr(), kl, ql, b, hq, hk, sq, kv_rows, d,
-                                              block, topk, keep_first, int(keep_own), out.data_ptr(), st), "block_select")
+    _call(q, "block_select", _lib.lib().sb_block_select, hq_view, _FLOATS[q.dtype], means.data_ptr(), kl, ql, b, hq, hk, sq,
+          kv_rows, d, block, topk, keep_first, keep_own, out.data_ptr())
     return out
 
 
@@ -343,9 +337,8 @@ def _attend(q, k, v, index, block, scale, kv_lens, q_lens):
     ws, need = _attn_workspace(sizes, 0, q.device)
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
     hs, ho = (_heads(q, "q"), _heads(k, "k"), _heads(v, "v")), _heads(out, "out")
-    with _On(q) as st:
-        _lib.check(_lib.lib().sb_block_attention(*hs, dt, index.data_ptr(), kl, ql, *sizes, scale, ho, lse.data_ptr(),
-                                                 _ptr(ws), need, st), "block_attention")
+    _call(q, "block_attention", _lib.lib().sb_block_attention, *hs, dt, index.data_ptr(), kl, ql, *sizes, scale, ho,
+          lse.data_ptr(), _ptr(ws), need)
     return out, lse
 
 
@@ -366,9 +359,8 @@ def block_attention_backward(dout, q, k, v, out, lse, index, block, *, scale=Non
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
     ins = _heads(dout, "dout"), _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(out, "out")
     outs = _heads(dq, "dq"), _heads(dk, "dk"), _heads(dv, "dv")
-    with _On(q) as st:
-        _lib.check(_lib.lib().sb_block_attention_backward(*ins, lse.data_ptr(), dt, index.data_ptr(), kl, ql, *sizes, scale,
-                                                          *outs, _ptr(ws), need, st), "block_attention_backward")
+    _call(q, "block_attention_backward", _lib.lib().sb_block_attention_backward, *ins, lse.data_ptr(), dt, index.data_ptr(),
+          kl, ql, *sizes, scale, *outs, _ptr(ws), need)
     return dq, dk, dv
 
 

@@ -84,8 +84,9 @@ int fill_rotary(const char* what, const sb_rotary* r, int rows, RotArgs* a) {
 
 template <typename T, int VEC, int NI, bool ADJ, int OP>
 int launch_rotary_as(const RotArgs& a, int grid, cudaStream_t st) {
-  const int smem = kRotTableBytes + kRotMaxTile * 6 * 8 + 2 * kRotMaxDim * 4;
-  rotary_kernel<T, VEC, NI, ADJ, OP><<<grid, kRotThreads, smem, st>>>(a);
+  // gradients: queries and keys in CTAs of their own
+  const dim3 ctas((unsigned)grid, OP == ROT_NORM_BWD && a.heads[1] > 0 ? 2 : 1);
+  rotary_kernel<T, VEC, NI, ADJ, OP><<<ctas, kRotThreads, 0, st>>>(a);
   return check_launch("rotary_kernel");
 }
 template <typename T, bool ADJ, int OP>
@@ -107,7 +108,7 @@ int launch_rotary_op(const RotArgs& a, int dtype, bool adjacent, int vec, int gr
                   : launch_rotary_vec<__nv_bfloat16, false, OP>(a, vec, grid, st);
 }
 
-// Vector width, lanes, tile and grid of a call whose operands are filled in.
+// Vector width, lanes and grid of a call whose operands are filled in.
 // `vec` comes in as the widest that bases and strides allow.
 int launch_rotary(RotArgs& a, int op, int dtype, bool adjacent, int vec, cudaStream_t st, int* grid_out) {
   const int D = a.dim, P = a.pairs;
@@ -115,19 +116,22 @@ int launch_rotary(RotArgs& a, int op, int dtype, bool adjacent, int vec, cudaStr
   a.items = adjacent ? (D + 2 * vec - 1) / (2 * vec) : P / vec + ((D - 2 * P) / vec + 1) / 2;
   a.lanes_log2 = pow2_log2(a.items < 32 ? a.items : 32);
   a.inv_dim = 1.f / (float)D;
+  // heads side by side: no more than share the work of the angles or than there are
+  const int least = a.heads[1] > 0 && a.heads[1] < a.heads[0] ? a.heads[1] : a.heads[0];
+  int side = 0;
+  while (side + a.lanes_log2 < 5 && (2 << side) <= vec && (2 << side) <= least) ++side;
+  a.side_log2 = side;
   const long long tokens = (long long)a.batch * a.rows;
-  // about eight items a thread and tile, as long as every SM has a few tiles
-  const int per_token = (a.heads[0] + a.heads[1]) << a.lanes_log2;
-  long long tile = 8 * kRotThreads / per_token;
-  const long long spread = tokens / (4 * num_sms());
-  if (tile > spread) tile = spread;
-  if (P && tile > kRotTableBytes / 8 / P) tile = kRotTableBytes / 8 / P;
-  if (tile > kRotMaxTile) tile = kRotMaxTile;
-  if (tile < 1) tile = 1;
-  a.tile = (int)tile;
-  a.num_tiles = (int)cdiv(tokens, tile);
-  int grid = a.num_tiles;
-  if (op == ROT_NORM_BWD && grid > kRotMaxGrid) grid = kRotMaxGrid;
+  a.groups = (int)cdiv(tokens, 32 >> (a.lanes_log2 + side));
+  // few tokens: their heads split over warps until every SM has some (never for
+  // the gradients, whose warps go over many units)
+  a.split = 1;
+  while (op != ROT_NORM_BWD && (long long)a.groups * a.split < 8 * num_sms() && (2 << side) * a.split <= a.heads[0]) a.split *= 2;
+  a.rows_inv = a.rows > 1 ? (uint32_t)(0x100000000ull / a.rows) : 0xffffffffu;
+  a.pairs_inv = P > 1 ? (uint32_t)(0x100000000ull / P) : 0xffffffffu;
+  int grid = (int)cdiv((long long)a.groups * a.split, kRotWarps);
+  const int most = op == ROT_NORM_BWD ? kRotMaxGrid : 3 * num_sms();  // the CTAs that run at once
+  if (grid > most) grid = most;
   if (grid_out) *grid_out = grid;
   if (op == ROT_TURN) return launch_rotary_op<ROT_TURN>(a, dtype, adjacent, vec, grid, st);
   if (op == ROT_NORM) return launch_rotary_op<ROT_NORM>(a, dtype, adjacent, vec, grid, st);

@@ -6,15 +6,16 @@
 //   norm:      x^ = x rstd, rstd = (mean(x^2) + eps)^-1/2,  y = R (w x^)
 //   backward:  g = R^T dy, dw = sum g x^, dx = rstd (w g - x^ mean(w g x^))
 //
-// A CTA owns a tile of tokens. It first fills a shared table with the cos and
-// sin of every (token, pair) once, which all heads of the token then use; the
-// angle is reduced in 64 bits as turns (coord * freq / 2 pi minus its nearest
-// integer), so positions of any size keep fp32 accuracy, and only the
-// remainder goes through the 32-bit sincospi. Then its threads run over
-// (token, head, lane) items: a lane holds VEC pairs of one head (both members
-// of a pair in the same thread), L lanes make a head and sum its squares by
-// shuffles. Rows are read once and written once, in 16-byte accesses where
-// shapes and strides allow (VEC below), so the kernels are bound by HBM.
+// A warp owns a few tokens and all (or a share) of their heads. A lane holds VEC
+// pairs of one head (both members of a pair in the same thread), L lanes make a
+// head and sum its squares by shuffles, HL heads lie side by side in the warp, so
+// that a load covers whole lines of a token's heads. The warp works out the cos
+// and sin of its tokens' pairs once, each lane its share, passes them through its
+// own piece of shared memory into registers and uses them for every head; the
+// rows of the first heads are on their way meanwhile, and no warp waits for
+// another. The angle is reduced in 64 bits, so positions of any size keep fp32
+// accuracy. Rows are read once and written once, in 16-byte accesses where shapes
+// and strides allow. Bound by HBM.
 //
 // Channels: half pairing (p, P + p), adjacent pairing (2p, 2p + 1), P pairs in
 // all; channels from 2P on are not turned. Leading `prefix` rows of each
@@ -26,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/shrimp_b200.h"
 
@@ -34,9 +36,8 @@ namespace sb {
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxDim = 256;
 constexpr int kRotMaxAxes = 4;
-constexpr int kRotMaxTile = 64;         // tokens of a tile
-constexpr int kRotTableBytes = 16384;   // cos / sin pairs of a tile
-constexpr int kRotMaxGrid = 148 * 4;    // CTAs of the gradient kernel (one partial weight gradient each)
+constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kRotMaxGrid = 148 * 2;    // CTAs of the gradient kernel (one partial weight gradient each)
 
 enum RotOp { ROT_TURN = 0, ROT_NORM = 1, ROT_NORM_BWD = 2 };
 
@@ -55,9 +56,11 @@ struct RotArgs {
   long long cs[3];             // batch, row, axis
   const double* freqs;
   int axis_end[kRotMaxAxes];   // exclusive end of each axis' pairs
-  int pairs, prefix, batch, rows, dim, items, lanes_log2;
+  int pairs, prefix, batch, rows, dim, items;
+  int lanes_log2, side_log2;   // L, HL
   float sign, eps, inv_dim;
-  int tile, num_tiles;
+  int groups, split;           // token groups of a warp's size, shares of a token's heads
+  uint32_t rows_inv, pairs_inv;  // floor(2^32 / rows), floor(2^32 / pairs); 2^32 - 1 for 1
 };
 
 template <typename T>
@@ -69,6 +72,58 @@ template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) RotVec {
   T v[VEC];
 };
+
+// VEC values to and from 32 bits, 16-bit types in pairs.
+template <typename T, int VEC>
+__device__ __forceinline__ void rot_unpack(const RotVec<T, VEC>& x, float (&f)[VEC]) {
+  if constexpr (sizeof(T) == 2 && VEC >= 2) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      float2 p;
+      if constexpr (std::is_same<T, __half>::value) p = __half22float2(__halves2half2(x.v[e], x.v[e + 1]));
+      else p = __bfloat1622float2(__halves2bfloat162(x.v[e], x.v[e + 1]));
+      f[e] = p.x;
+      f[e + 1] = p.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = rot_f32(x.v[e]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ RotVec<T, VEC> rot_pack(const float (&f)[VEC]) {
+  RotVec<T, VEC> x;
+  if constexpr (sizeof(T) == 2 && VEC >= 2) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 p = __floats2half2_rn(f[e], f[e + 1]);
+        x.v[e] = p.x;
+        x.v[e + 1] = p.y;
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(f[e], f[e + 1]);
+        x.v[e] = p.x;
+        x.v[e + 1] = p.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x.v[e] = rot_cast<T>(f[e]);
+  }
+  return x;
+}
+
+// x / d and the remainder by m = floor(2^32 / d), for 0 <= x < 2^31: the product
+// falls short of the quotient by one at most.
+__device__ __forceinline__ int rot_div(int x, int d, uint32_t m, int& rest) {
+  int q = (int)__umulhi((uint32_t)x, m);
+  rest = x - q * d;
+  if (rest >= d) {
+    rest -= d;
+    ++q;
+  }
+  return q;
+}
 
 __device__ __forceinline__ double rot_coord(const void* p, int dtype, long long i) {
   switch (dtype) {
@@ -87,29 +142,46 @@ __device__ __forceinline__ float rot_weight(const void* p, int dtype, int i) {
   }
 }
 
+// cos and sin of an angle in quarter turns, reduced in 64 bits to the nearest one
+// (at most half a quarter off, whatever the position), then the Taylor series of
+// both on [-pi/4, pi/4] (to x^9 and x^8: off by under 3e-8).
+__device__ __forceinline__ float2 rot_cos_sin(double quarters) {
+  const double q = rint(quarters);
+  const float x = (float)(quarters - q) * 1.5707963267948966f, x2 = x * x;
+  const float sn = x + x * x2 * (-1.f / 6.f + x2 * (1.f / 120.f + x2 * (-1.f / 5040.f + x2 * (1.f / 362880.f))));
+  const float co = 1.f + x2 * (-0.5f + x2 * (1.f / 24.f + x2 * (-1.f / 720.f + x2 * (1.f / 40320.f))));
+  const int n = (int)(long long)q;
+  const float c = n & 1 ? sn : co, v = n & 1 ? co : sn;
+  return make_float2((n + 1) & 2 ? -c : c, n & 2 ? -v : v);
+}
+
 // Slots of one lane: NI items of two VEC-wide chunks. Item i of a head:
 //   half pairing:  i < P / VEC: chunks at i * VEC and P + i * VEC (turned);
 //                  else two chunks of the unturned rest (the second may be missing)
 //   adjacent:      channels [2 VEC i, 2 VEC (i + 1)), every pair inside.
+// The gradient kernel runs queries and keys in CTAs of their own (blockIdx.y), so
+// that a thread adds up one set of weight gradients.
 template <typename T, int VEC, int NI, bool ADJ, int OP>
-__global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
-  extern __shared__ __align__(16) char rot_smem[];
-  float2* table = reinterpret_cast<float2*>(rot_smem);                       // [tile][pairs]
-  long long* off = reinterpret_cast<long long*>(rot_smem + kRotTableBytes);  // [tile][2][3]
-  float* wsm = reinterpret_cast<float*>(off + kRotMaxTile * 6);              // [2][dim]
+__global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotary_kernel(const RotArgs a) {
+  constexpr int U = OP == ROT_NORM_BWD || NI > 1 ? 1 : 2;  // heads whose rows a lane has in flight
+  constexpr bool BWD = OP == ROT_NORM_BWD;
+  __shared__ __align__(16) float2 tables[kRotWarps][32 * VEC * NI];
+  __shared__ double freqs[kRotMaxDim / 2];         // quarter turns per coordinate step
+  __shared__ unsigned char axis[kRotMaxDim / 2];
+  __shared__ float weights[2][OP == ROT_TURN ? 1 : kRotMaxDim];
   using V = RotVec<T, VEC>;
-  const int tid = threadIdx.x;
-  const int L = 1 << a.lanes_log2, lane = tid & (L - 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int L = 1 << a.lanes_log2, HL = 1 << a.side_log2, ll = lane & (L - 1);
+  const int side = lane >> a.lanes_log2 & (HL - 1), sub = lane >> (a.lanes_log2 + a.side_log2);
+  const int TW = 32 >> (a.lanes_log2 + a.side_log2);  // tokens of a unit
   const int P = a.pairs, D = a.dim;
-  if (OP != ROT_TURN)
-    for (int i = tid; i < 2 * D; i += kRotThreads)
-      wsm[i] = rot_weight(a.w[i >= D], a.w_dtype, i >= D ? i - D : i);
+  float2* table = tables[warp];  // [TW][P]
 
   // this lane's channels and its place in the table (pair < 0: not turned)
   int ca[NI], cb[NI], pr[NI];
 #pragma unroll
   for (int k = 0; k < NI; ++k) {
-    const int i = lane + k * L;
+    const int i = ll + k * L;
     if (i >= a.items) {
       ca[k] = cb[k] = pr[k] = -1;
     } else if (ADJ) {
@@ -127,191 +199,202 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
       pr[k] = -1;
     }
   }
-  float dwa[2][NI][2 * VEC];
-  if (OP == ROT_NORM_BWD) {
+  float dwa[NI][2 * VEC];
+  if (BWD) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int k = 0; k < NI; ++k)
 #pragma unroll
-      for (int k = 0; k < NI; ++k)
-#pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) dwa[h][k][e] = 0.f;
+      for (int e = 0; e < 2 * VEC; ++e) dwa[k][e] = 0.f;
   }
-
-  const long long tokens = (long long)a.batch * a.rows;
-  for (long long tile = blockIdx.x; tile < a.num_tiles; tile += gridDim.x) {
-    const long long t0 = tile * a.tile;
-    const int nt = (int)(tokens - t0 < a.tile ? tokens - t0 : a.tile);
-    if (tile != blockIdx.x) __syncthreads();  // the table of the tile before is still being read
-    for (int i = tid; i < nt * P; i += kRotThreads) {
-      const int tk = i / P, p = i - tk * P;
-      const long long t = t0 + tk;
-      const int b = (int)(t / a.rows), s = (int)(t - (long long)b * a.rows);
-      float2 cs = make_float2(1.f, 0.f);
-      if (s >= a.prefix) {
-        int ax = 0;
-        while (p >= a.axis_end[ax]) ++ax;
-        const double c = rot_coord(a.coords, a.coord_dtype, b * a.cs[0] + (s - a.prefix) * a.cs[1] + ax * a.cs[2]);
-        const double turns = c * (a.freqs[p] * 0.15915494309189533577);  // 1 / (2 pi)
-        const float r = (float)(2.0 * (turns - rint(turns)));
-        float sn, co;
-        sincospif(r, &sn, &co);
-        cs = make_float2(co, a.sign * sn);
-      }
-      table[i] = cs;
-    }
-    for (int i = tid; i < nt * 2; i += kRotThreads) {
-      const int h = i & 1;
-      const long long t = t0 + (i >> 1);
-      const long long b = t / a.rows, s = t - b * a.rows;
-      off[i * 3] = b * a.xs[h][0] + s * a.xs[h][2];
-      off[i * 3 + 1] = b * a.ys[h][0] + s * a.ys[h][2];
-      off[i * 3 + 2] = b * a.gs[h][0] + s * a.gs[h][2];
-    }
-    __syncthreads();
+  for (int p = tid; p < P; p += kRotThreads) {
+    int ax = 0;
+    while (p >= a.axis_end[ax]) ++ax;
+    axis[p] = (unsigned char)ax;
+    freqs[p] = a.freqs[p] * 0.63661977236758134308;  // 2 / pi
+  }
+  if (OP != ROT_TURN)
+    for (int i = tid; i < 2 * D; i += kRotThreads)
+      weights[i >= D][i >= D ? i - D : i] = rot_weight(a.w[i >= D], a.w_dtype, i >= D ? i - D : i);
+  __syncthreads();
+  float w0[NI][2 * VEC];  // this lane's weights
+  auto load_weights = [&](int h) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int e = 0; e < 2 * VEC; ++e) {
+        const int c = e < VEC ? ca[k] + e : cb[k] + e - VEC;
+        w0[k][e] = (e < VEC ? ca[k] : cb[k]) >= 0 ? weights[h][c] : 0.f;
+      }
+  };
+  if (BWD) load_weights(blockIdx.y);
+  const int tokens = a.batch * a.rows;  // below 2^31
+  const int units = a.groups * a.split, stride = gridDim.x * kRotWarps;
+  for (int unit = blockIdx.x * kRotWarps + warp; unit < units; unit += stride) {
+    const int group = a.split == 1 ? unit : unit / a.split;
+    const int share = unit - group * a.split, t = group * TW + sub;
+    int s;
+    const int b = rot_div(t, a.rows, a.rows_inv, s);
+    float cs[NI][VEC], sn[NI][VEC];
+    bool made = false;
+#pragma unroll
+    for (int hh = 0; hh < (BWD ? 1 : 2); ++hh) {
+      const int h = BWD ? blockIdx.y : hh;
       const int H = a.heads[h];
       if (H == 0) continue;
-      const T* __restrict__ xp = (const T*)a.x[h];
-      const T* __restrict__ gp = (const T*)a.dy[h];
-      T* yp = (T*)a.y[h];
-      const int total = nt * H << a.lanes_log2;
+      // this share's heads, and the rows of this lane's first one
+      const int per = a.split == 1 ? H : ((H + a.split - 1) / a.split + HL - 1) & ~(HL - 1);
+      const int end = t < tokens ? min(H, (share + 1) * per) : 0;
+      int hd = share * per + side;
+      const long long xh = a.xs[h][1] << a.side_log2, yh = a.ys[h][1] << a.side_log2, gh = BWD ? a.gs[h][1] << a.side_log2 : 0;
+      const T* x = (const T*)a.x[h] + b * a.xs[h][0] + hd * a.xs[h][1] + s * a.xs[h][2];
+      const T* g = BWD ? (const T*)a.dy[h] + b * a.gs[h][0] + hd * a.gs[h][1] + s * a.gs[h][2] : nullptr;
+      T* y = (T*)a.y[h] + b * a.ys[h][0] + hd * a.ys[h][1] + s * a.ys[h][2];
+      if (OP == ROT_NORM) load_weights(h);
       // whole warps stay in the loop together: the shuffles need every lane
-      for (int base = 0; base < total; base += kRotThreads) {
-        const int row = (base + tid) >> a.lanes_log2;
-        const bool live = base + tid < total;
-        const int tk = live ? row / H : 0, hd = live ? row - tk * H : 0;
-        const long long* o = off + (tk * 2 + h) * 3;
-        float u[NI][VEC], v[NI][VEC], gu[NI][VEC], gv[NI][VEC];
+      for (int h0 = share * per; h0 < min(H, (share + 1) * per); h0 += U * HL) {
+        V xa[U][NI], xb[U][NI], ga[U][NI], gb[U][NI];
 #pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          V xa{}, xb{}, ga{}, gb{};
-          const long long xo = o[0] + hd * a.xs[h][1], go = o[2] + hd * a.gs[h][1];
-          if (live && ca[k] >= 0) {
-            xa = *reinterpret_cast<const V*>(xp + xo + ca[k]);
-            if (OP == ROT_NORM_BWD) ga = *reinterpret_cast<const V*>(gp + go + ca[k]);
-          }
-          if (live && cb[k] >= 0) {
-            xb = *reinterpret_cast<const V*>(xp + xo + cb[k]);
-            if (OP == ROT_NORM_BWD) gb = *reinterpret_cast<const V*>(gp + go + cb[k]);
-          }
+        for (int w = 0; w < U; ++w) {
+          const bool live = hd + w * HL < end;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            u[k][e] = rot_f32(xa.v[e]);
-            v[k][e] = rot_f32(xb.v[e]);
-            if (OP == ROT_NORM_BWD) {
-              gu[k][e] = rot_f32(ga.v[e]);
-              gv[k][e] = rot_f32(gb.v[e]);
+          for (int k = 0; k < NI; ++k) {
+            xa[w][k] = live && ca[k] >= 0 ? *reinterpret_cast<const V*>(x + w * xh + ca[k]) : V{};
+            xb[w][k] = live && cb[k] >= 0 ? *reinterpret_cast<const V*>(x + w * xh + cb[k]) : V{};
+            if (BWD) {
+              ga[w][k] = live && ca[k] >= 0 ? *reinterpret_cast<const V*>(g + w * gh + ca[k]) : V{};
+              gb[w][k] = live && cb[k] >= 0 ? *reinterpret_cast<const V*>(g + w * gh + cb[k]) : V{};
             }
           }
         }
-        float rstd = 1.f;
-        if (OP != ROT_TURN) {
-          float ss = 0.f;
+        if (!made) {
+          made = true;
+          __syncwarp();
+          for (int i = lane; i < TW * P; i += 32) {
+            int p, sr;
+            const int ti = rot_div(i, P, a.pairs_inv, p);
+            const int tt = t - sub + ti, tb = rot_div(tt, a.rows, a.rows_inv, sr);
+            float2 c = make_float2(1.f, 0.f);
+            if (tt < tokens && sr >= a.prefix) {
+              c = rot_cos_sin(freqs[p] * rot_coord(a.coords, a.coord_dtype,
+                                                   tb * a.cs[0] + (sr - a.prefix) * a.cs[1] + axis[p] * a.cs[2]));
+              c.y *= a.sign;
+            }
+            table[i] = c;
+          }
+          __syncwarp();
 #pragma unroll
           for (int k = 0; k < NI; ++k)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) ss += u[k][e] * u[k][e] + v[k][e] * v[k][e];
-          for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-          rstd = rsqrtf(ss * a.inv_dim + a.eps);
+            for (int e = 0; e < VEC; ++e) {
+              const float2 c = pr[k] >= 0 && (!ADJ || pr[k] + e < P) ? table[sub * P + pr[k] + e] : make_float2(1.f, 0.f);
+              cs[k][e] = c.x;
+              sn[k][e] = BWD ? -c.y : c.y;  // gradients turn back
+            }
         }
-        float c1 = 0.f;  // backward: sum of w g x^ over the head
 #pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          if (ca[k] < 0) continue;
-          float cs[VEC], sn[VEC];
-          bool turn[VEC];  // an unturned channel never meets its neighbour's infinities
+        for (int w = 0; w < U; ++w) {
+          if (w > 0 && h0 + w * HL >= min(H, (share + 1) * per)) break;  // the whole warp
+          const bool live = hd + w * HL < end;
+          float u[NI][VEC], v[NI][VEC], gu[NI][VEC], gv[NI][VEC];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            turn[e] = pr[k] >= 0 && pr[k] + e < P;
-            const float2 t = turn[e] ? table[tk * P + pr[k] + e] : make_float2(1.f, 0.f);
-            cs[e] = t.x;
-            sn[e] = t.y;
+          for (int k = 0; k < NI; ++k) {
+            rot_unpack(xa[w][k], u[k]);
+            rot_unpack(xb[w][k], v[k]);
+            if (BWD) {
+              rot_unpack(ga[w][k], gu[k]);
+              rot_unpack(gb[w][k], gv[k]);
+            }
           }
-          // the two members of pair e: (u[e], v[e]) in the half pairing,
-          // neighbours of the 2 VEC contiguous channels in the adjacent one
+          float rstd = 1.f;
+          if (OP != ROT_TURN) {
+            float ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int i0 = ADJ ? 2 * e : e, i1 = ADJ ? 2 * e + 1 : VEC + e;
-            float& x0 = i0 < VEC ? u[k][i0 % VEC] : v[k][i0 % VEC];
-            float& x1 = i1 < VEC ? u[k][i1 % VEC] : v[k][i1 % VEC];
-            const int c0 = i0 < VEC ? ca[k] + i0 : cb[k] + i0 - VEC;
-            const int c1i = i1 < VEC ? ca[k] + i1 : cb[k] + i1 - VEC;
-            const bool two = cb[k] >= 0;
-            if (OP == ROT_TURN) {
-              const float p0 = x0, p1 = x1;
-              if (turn[e]) {
-                x0 = p0 * cs[e] - p1 * sn[e];
-                x1 = p1 * cs[e] + p0 * sn[e];
+            for (int k = 0; k < NI; ++k)
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) ss += u[k][e] * u[k][e] + v[k][e] * v[k][e];
+            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            rstd = rsqrtf(ss * a.inv_dim + a.eps);
+#pragma unroll
+            for (int k = 0; k < NI; ++k)
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                u[k][e] *= BWD ? rstd : rstd * w0[k][e];
+                v[k][e] *= BWD ? rstd : rstd * w0[k][VEC + e];
               }
-            } else if (OP == ROT_NORM) {
-              const float p0 = x0 * rstd * wsm[h * D + c0], p1 = two ? x1 * rstd * wsm[h * D + c1i] : 0.f;
-              x0 = turn[e] ? p0 * cs[e] - p1 * sn[e] : p0;
-              x1 = turn[e] ? p1 * cs[e] + p0 * sn[e] : p1;
-            } else {
-              float& g0 = i0 < VEC ? gu[k][i0 % VEC] : gv[k][i0 % VEC];
-              float& g1 = i1 < VEC ? gu[k][i1 % VEC] : gv[k][i1 % VEC];
-              // turned back: the transpose of the rotation
-              const float q0 = turn[e] ? g0 * cs[e] + g1 * sn[e] : g0, q1 = turn[e] ? g1 * cs[e] - g0 * sn[e] : g1;
-              x0 *= rstd;
-              x1 *= rstd;
-              dwa[h][k][i0] += q0 * x0;
-              dwa[h][k][i1] += q1 * x1;
-              g0 = q0 * wsm[h * D + c0];
-              g1 = two ? q1 * wsm[h * D + c1i] : 0.f;
-              c1 += g0 * x0 + g1 * x1;
+          }
+#pragma unroll
+          for (int k = 0; k < NI; ++k) {
+            if (pr[k] < 0) continue;  // an unturned channel never meets its neighbour's infinities
+            float(&m0)[VEC] = BWD ? gu[k] : u[k];
+            float(&m1)[VEC] = BWD ? gv[k] : v[k];
+            // the two members of pair e: (m0[e], m1[e]) in the half pairing,
+            // neighbours of the 2 VEC contiguous channels in the adjacent one
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const int i0 = ADJ ? 2 * e : e, i1 = ADJ ? 2 * e + 1 : VEC + e;
+              float& x0 = i0 < VEC ? m0[i0 % VEC] : m1[i0 % VEC];
+              float& x1 = i1 < VEC ? m0[i1 % VEC] : m1[i1 % VEC];
+              if (ADJ && pr[k] + e >= P) continue;
+              const float p0 = x0, p1 = x1;
+              x0 = p0 * cs[k][e] - p1 * sn[k][e];
+              x1 = p1 * cs[k][e] + p0 * sn[k][e];
             }
           }
-        }
-        if (OP == ROT_NORM_BWD) {
-          for (int m = 1; m < L; m <<= 1) c1 += __shfl_xor_sync(0xffffffffu, c1, m);
-          c1 *= a.inv_dim;
-        }
+          if (BWD) {
+            float c1 = 0.f;  // sum of w g x^ over the head
 #pragma unroll
-        for (int k = 0; k < NI; ++k) {
-          V ya, yb;
+            for (int k = 0; k < NI; ++k)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (OP == ROT_NORM_BWD) {
-              ya.v[e] = rot_cast<T>(rstd * (gu[k][e] - u[k][e] * c1));
-              yb.v[e] = rot_cast<T>(rstd * (gv[k][e] - v[k][e] * c1));
-            } else {
-              ya.v[e] = rot_cast<T>(u[k][e]);
-              yb.v[e] = rot_cast<T>(v[k][e]);
-            }
+              for (int e = 0; e < VEC; ++e) {
+                dwa[k][e] += gu[k][e] * u[k][e];
+                dwa[k][VEC + e] += gv[k][e] * v[k][e];
+                gu[k][e] *= w0[k][e];
+                gv[k][e] *= w0[k][VEC + e];
+                c1 += gu[k][e] * u[k][e] + gv[k][e] * v[k][e];
+              }
+            for (int m = 1; m < L; m <<= 1) c1 += __shfl_xor_sync(0xffffffffu, c1, m);
+            c1 *= a.inv_dim;
+#pragma unroll
+            for (int k = 0; k < NI; ++k)
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                u[k][e] = rstd * (gu[k][e] - u[k][e] * c1);
+                v[k][e] = rstd * (gv[k][e] - v[k][e] * c1);
+              }
           }
-          const long long yo = o[1] + hd * a.ys[h][1];
-          if (live && ca[k] >= 0) *reinterpret_cast<V*>(yp + yo + ca[k]) = ya;
-          if (live && cb[k] >= 0) *reinterpret_cast<V*>(yp + yo + cb[k]) = yb;
+#pragma unroll
+          for (int k = 0; k < NI; ++k) {
+            if (live && ca[k] >= 0) *reinterpret_cast<V*>(y + w * yh + ca[k]) = rot_pack<T, VEC>(u[k]);
+            if (live && cb[k] >= 0) *reinterpret_cast<V*>(y + w * yh + cb[k]) = rot_pack<T, VEC>(v[k]);
+          }
         }
+        hd += U * HL;
+        x += U * xh;
+        y += U * yh;
+        if (BWD) g += U * gh;
       }
     }
   }
 
-  if (OP == ROT_NORM_BWD) {
-    // CTA sum of the weight gradients in a fixed order: threads with the same
-    // lane hold the same channels; each adds in turn of its group
-    float* red = reinterpret_cast<float*>(rot_smem);  // [groups][dim], over the table
-    for (int h = 0; h < 2; ++h) {
-      if (a.heads[h] == 0) continue;
-      // groups of a warp first (shuffles), then the warps through shared memory
-      __syncthreads();
+  if (BWD) {
+    // CTA sum of the weight gradients in a fixed order: the heads of a warp first
+    // (threads of one lane hold the same channels), then the warps
+    __shared__ float red[kRotWarps][kRotMaxDim];
 #pragma unroll
-      for (int k = 0; k < NI; ++k)
+    for (int k = 0; k < NI; ++k)
 #pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) {
-          float s = dwa[h][k][e];
-          for (int m = L; m < 32; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-          const int c = e < VEC ? ca[k] + e : cb[k] + e - VEC;
-          const bool have = e < VEC ? ca[k] >= 0 : cb[k] >= 0;
-          if (have && (tid & 31) < L) red[(tid >> 5) * D + c] = s;
-        }
-      __syncthreads();
-      for (int c = tid; c < D; c += kRotThreads) {
-        float s = 0.f;
-        for (int g = 0; g < kRotThreads / 32; ++g) s += red[g * D + c];
-        a.dw_part[((long long)blockIdx.x * 2 + h) * D + c] = s;
+      for (int e = 0; e < 2 * VEC; ++e) {
+        float s = dwa[k][e];
+        for (int m = L; m < 32; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        const int c = e < VEC ? ca[k] + e : cb[k] + e - VEC;
+        const bool have = e < VEC ? ca[k] >= 0 : cb[k] >= 0;
+        if (have && lane < L) red[warp][c] = s;
       }
+    __syncthreads();
+    for (int c = tid; c < D; c += kRotThreads) {
+      float s = 0.f;
+      for (int g = 0; g < kRotWarps; ++g) s += red[g][c];
+      a.dw_part[((long long)blockIdx.x * 2 + blockIdx.y) * D + c] = s;
     }
   }
 }
@@ -325,6 +408,7 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float* __restrict
   void* dw = h ? dw1 : dw0;
   double s = 0.0;
   if (c < dim && (h ? heads1 : heads0) > 0)
+#pragma unroll 8
     for (int g = threadIdx.y; g < grid; g += 32) s += (double)part[((long long)g * 2 + h) * dim + c];
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
