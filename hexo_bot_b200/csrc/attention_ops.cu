@@ -116,10 +116,13 @@ int launch_rotary(RotArgs& a, int op, int dtype, bool adjacent, int vec, cudaStr
   a.items = adjacent ? (D + 2 * vec - 1) / (2 * vec) : P / vec + ((D - 2 * P) / vec + 1) / 2;
   a.lanes_log2 = pow2_log2(a.items < 32 ? a.items : 32);
   a.inv_dim = 1.f / (float)D;
-  // heads side by side: no more than share the work of the angles or than there are
+  // heads side by side: no more than share the work of the angles, and half of
+  // them at most, so that a lane's angles serve two heads or more (4096 x 69 rows,
+  // 8 heads of 16: 47 us with all side by side, 35 with half, 35 with a quarter,
+  // 53 with an eighth, where loads touch too many lines)
   const int least = a.heads[1] > 0 && a.heads[1] < a.heads[0] ? a.heads[1] : a.heads[0];
   int side = 0;
-  while (side + a.lanes_log2 < 5 && (2 << side) <= vec && (2 << side) <= least) ++side;
+  while (side + a.lanes_log2 < 5 && (2 << side) <= vec && 2 * (2 << side) <= a.heads[0] && (2 << side) <= least) ++side;
   a.side_log2 = side;
   const long long tokens = (long long)a.batch * a.rows;
   a.groups = (int)cdiv(tokens, 32 >> (a.lanes_log2 + side));
@@ -336,9 +339,29 @@ struct LaunchFew {
   cudaStream_t st;
   template <typename T, int DP, int BK>
   int operator()() const {
-    const long long grid = (long long)a.batch * a.kv_heads * a.q_rows * ((a.group + 15) / 16);
-    return launch_ba(block_attn_few_kernel<T, DP, BK>, "block_attn_few_kernel", grid, ba_few_warps<DP, BK>() * 32,
-                     ba_few_smem<DP, BK>(), a, st);
+    constexpr int W = ba_few_warps<DP, BK>();
+    const long long rows = (long long)a.batch * a.kv_heads * a.q_rows * ((a.group + 15) / 16);
+    // CTAs of a row: as many as have a block for every warp and run at once (64
+    // rows of 32 blocks, D = 128: 29 us with one CTA a row, 17 with two, 21 with
+    // four, 37 with eight, which take turns)
+    int cluster = 1;
+    while (cluster < kBaFewCluster && cluster * W < a.topk && 2 * rows * cluster <= num_sms()) cluster *= 2;
+    if (rows * cluster > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "block_attention: too many rows for one launch");
+    auto kern = block_attn_few_kernel<T, DP, BK>;
+    if (int s = ensure_smem(reinterpret_cast<const void*>(kern), ba_few_smem<DP, BK>())) return s;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = (unsigned)(rows * cluster);
+    cfg.blockDim = W * 32;
+    cfg.dynamicSmemBytes = ba_few_smem<DP, BK>();
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, a);  // errors surface in check_launch
+    return check_launch("block_attn_few_kernel");
   }
 };
 struct LaunchFwd {

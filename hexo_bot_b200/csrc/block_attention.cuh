@@ -276,12 +276,12 @@ __device__ __forceinline__ int ba_div_group(const BaArgs& a, int x) {
 // rows, 2 (lane % 4) and + 1 the columns of each 8-wide tile).
 template <typename T, int DP, int BK>
 struct BaTile {
-  float o[DP / 8][4];
+  float s[BK / 8][4], o[DP / 8][4];
   float m[2], l[2];
 
-  __device__ __forceinline__ void run(uint32_t q, uint32_t k, uint32_t v, int live_keys, float scale_log2) {
+  // weights, row maxima and sums; the keys are free afterwards
+  __device__ __forceinline__ void scores(uint32_t q, uint32_t k, int live_keys, float scale_log2) {
     const int lane = threadIdx.x & 31;
-    float s[BK / 8][4];
 #pragma unroll
     for (int n = 0; n < BK / 8; ++n)
 #pragma unroll
@@ -339,6 +339,9 @@ struct BaTile {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
+  }
+  __device__ __forceinline__ void output(uint32_t v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
@@ -776,17 +779,22 @@ __global__ __launch_bounds__(kBaJoinThreads) void block_attn_join_kernel(const B
 }
 
 // ---- forward, few queries --------------------------------------------------------
-// One CTA per (batch, kv head, query): its warps take the row's blocks in turn,
-// each with a key block of its own in shared memory, and keep running maxima,
-// sums and output rows; the warps' results are joined in shared memory. The
-// group's heads are the rows of the 16-row tile.
+// A cluster of CTAs per (batch, kv head, query): their warps take the row's blocks
+// in turn, each with a key block of its own in shared memory, and keep running
+// maxima, sums and output rows; the results are joined over a CTA's warps in
+// shared memory, then over the cluster's CTAs in distributed shared memory, each
+// CTA a share of the channels. The group's heads are the rows of the 16-row tile.
+// Bound by the read of the chosen keys and values (8 x 8 rows, 4 heads of 128, 32
+// blocks of 64: 30 us with one CTA a row, whose warps took 8 blocks one after
+// another).
+constexpr int kBaFewCluster = 8;
 template <int DP, int BK>
 constexpr int ba_few_warps() {
   return DP * BK >= 16384 ? 2 : DP * BK >= 8192 ? 4 : 8;
 }
 template <int DP, int BK>
 constexpr int ba_few_smem() {
-  return ba_few_warps<DP, BK>() * (2 * BK * DP * 2) + 16 * DP * 2;
+  return ba_few_warps<DP, BK>() * (2 * BK * DP * 2) + 16 * DP * 2 + 16 * DP * 4;
 }
 
 template <typename T, int DP, int BK>
@@ -800,8 +808,12 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
   __shared__ int chosen[kBaMaxTopk];
   __shared__ int num;
   __shared__ float2 sml[W][16];
+  __shared__ float2 cml[16];  // the CTA's maxima and sums
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int G = a.group, gt = (G + 15) / 16;
-  const long long u = blockIdx.x;
+  const long long u = blockIdx.x / C;
   const int gi = (int)(u % gt);
   const int i = (int)(u / gt % a.q_rows);
   const int bh = (int)(u / gt / a.q_rows), b = bh / a.kv_heads, h = bh - b * a.kv_heads;
@@ -837,18 +849,32 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
   for (int x = 0; x < DP / 8; ++x)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
-  for (int c = warp; c < n; c += W) {
-    const int j = chosen[c];
-    const int have = min(BK, kv - j * BK);
-    const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s;
-    const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s;
-    ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, lane, 32);
-    ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, lane, 32);
-    cp_async_wait_all();
-    __syncwarp();
+  // the next block's keys load while this one's values are used, its values
+  // while the next scores are computed
+  const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h;
+  auto load = [&](uint32_t to, const T* src, long long stride, int c) {
+    if (c < n) {
+      const int j = chosen[c];
+      ba_load_rows<T, DP>(to, src + (long long)j * BK * stride, stride, BK, min(BK, kv - j * BK), a.dim, lane, 32);
+    }
+    cp_async_commit();
+  };
+  load(ks, kp, a.k.s, rank * W + warp);
+  load(vs, vp, a.v.s, rank * W + warp);
+  for (int c = rank * W + warp; c < n; c += C * W) {
+    const int have = min(BK, kv - chosen[c] * BK);
     BaTile<T, DP, BK> tile;
-    tile.run(qs, ks, vs, have, a.scale_log2);
+    cp_async_wait<1>();
     __syncwarp();
+    tile.scores(qs, ks, have, a.scale_log2);
+    __syncwarp();
+    load(ks, kp, a.k.s, c + C * W);
+    cp_async_wait<1>();
+    __syncwarp();
+    tile.output(vs);
+    __syncwarp();
+    load(vs, vp, a.v.s, c + C * W);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float t = fmaxf(top[r], tile.m[r]);
@@ -864,6 +890,7 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
     }
   }
   // join over the warps: parts in the key buffers (16 x DP fp32 each)
+  cp_async_wait_all();
   __syncthreads();
   float* mine = reinterpret_cast<float*>(ba_smem) + warp * (16 * DP);
 #pragma unroll
@@ -876,6 +903,7 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
   }
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(ba_smem);
+  float* cta = reinterpret_cast<float*>(ba_smem + W * (2 * BK * DP * 2) + 16 * DP * 2);  // [16][dim], the CTA's rows
   for (int x = threadIdx.x; x < rows * a.dim; x += W * 32) {
     const int row = x / a.dim, d = x - row * a.dim;
     float t = -INFINITY;
@@ -887,10 +915,35 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
       s += f * sml[w][row].y;
       acc += f * all[w * (16 * DP) + row * DP + d];
     }
+    cta[x] = acc;
+    if (d == 0) cml[row] = make_float2(t, s);
+  }
+  cluster.sync();
+  for (int x = rank * W * 32 + threadIdx.x; x < rows * a.dim; x += C * W * 32) {
+    const int row = x / a.dim, d = x - row * a.dim;
+    float2 p[kBaFewCluster];
+    float o[kBaFewCluster], t = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kBaFewCluster; ++c)
+      if (c < C) {
+        p[c] = cluster.map_shared_rank(cml, c)[row];
+        o[c] = cluster.map_shared_rank(cta, c)[x];
+        t = fmaxf(t, p[c].x);
+      }
+    const float ref = t == -INFINITY ? 0.f : t;
+    float acc = 0.f, s = 0.f;
+#pragma unroll
+    for (int c = 0; c < kBaFewCluster; ++c)
+      if (c < C) {
+        const float f = ba_exp2(p[c].x - ref);
+        s += f * p[c].y;
+        acc += f * o[c];
+      }
     const int hq = h * G + gi * 16 + row;
     ((T*)a.o.p)[b * a.o.b + hq * a.o.h + i * a.o.s + d] = rot_cast<T>(s == 0.f ? 0.f : acc / s);
     if (d == 0) a.lse[((long long)b * a.kv_heads * G + hq) * a.q_rows + i] = (ref + log2f(s)) * kLn2;
   }
+  cluster.sync();  // a CTA's shared memory stays until the others have read it
 }
 
 // ---- backward --------------------------------------------------------------------
