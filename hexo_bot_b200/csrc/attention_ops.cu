@@ -217,9 +217,10 @@ constexpr long long kBaWindowBytes = 1ll << 30;
 constexpr int kBaFewRows = 16;      // up to so many queries take the few-query kernel
 // Work items an SM and window, and the listed rows that an item may hold: fewer
 // items leave SMs idle behind popular blocks (8192 rows, 8 heads of 64, 16 of 128
-// blocks, forward: 211 us with 8 an SM, 201 with 16 to 32; backward 404 / 410 /
-// 423 us with 8 / 16 / 24), smaller ones repeat the listing and the key loads.
-constexpr int kBaItems = 16, kBaMinTarget = 256, kBaMaxTarget = 1024;
+// blocks, forward: 211 us with 8 an SM, 201 with 16 to 32; backward, where every
+// segment of a block leaves a part of dk and dv: 338 / 335 / 326 / 326 / 334 us
+// with 4 / 6 / 8 / 12 / 16), smaller ones repeat the listing and the key loads.
+constexpr int kBaItems = 16, kBaBwdItems = 8, kBaMinTarget = 256, kBaMaxTarget = 1024;
 
 // Segments of `seg` list groups over all windows of wq rows.
 int ba_segments(int q_rows, int wq, int seg) {
@@ -250,8 +251,9 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   // a segment: as many groups as give a work item its target of listed rows on
   // average (several items a CTA, to even out popular blocks), evenly split
   const long long pairs = (long long)p.bh_step * p.wq * topk * group;
-  long long target = pairs / (kBaItems * num_sms());
-  target = target < kBaMinTarget ? kBaMinTarget : target > kBaMaxTarget ? kBaMaxTarget : target;
+  long long target = pairs / ((backward ? kBaBwdItems : kBaItems) * num_sms());
+  const int most = backward ? 2 * kBaMaxTarget : kBaMaxTarget;
+  target = target < kBaMinTarget ? kBaMinTarget : target > most ? most : target;
   const long long groups = cdiv(p.wq, kBaMark);
   long long seg = cdiv(target * nb, (long long)topk * group * kBaMark);
   seg = seg < 1 ? 1 : seg > groups ? groups : seg;
@@ -384,8 +386,10 @@ struct LaunchBwd {
   cudaStream_t st;
   template <typename T, int DP, int BK>
   int operator()() const {
-    if (int s = launch_ba(block_attn_bwd_kernel<T, DP, BK>, "block_attn_bwd_kernel", (long long)a.nbh * a.nb * a.nseg, BK * 2,
-                          ba_bwd_smem<DP, BK>(), a, st))
+    const long long items = (long long)a.nbh * a.nb * a.nseg, most = (long long)num_sms() * ba_bwd_ctas<DP, BK>();
+    if (items > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "block_attention_backward: too many blocks for one launch");
+    if (int s = launch_ba(block_attn_bwd_kernel<T, DP, BK>, "block_attn_bwd_kernel", items < most ? items : most,
+                          kBaBwdThreads, ba_bwd_smem<DP, BK>(), a, st))
       return s;
     return launch_ba(block_attn_dq_kernel<T>, "block_attn_dq_kernel",
                      cdiv((long long)a.nbh * a.wq * a.group, kBaJoinThreads >> ba_join_lanes(a.dim, a.topk)),
@@ -752,6 +756,7 @@ int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const s
   a.part = (float*)(ws + p.part);
   a.delta = (float*)(ws + p.delta);
   a.kv_part = (float*)(ws + p.kv_part);
+  a.ticket = (uint32_t*)(ws + p.ticket);
   a.nseg_all = ba_segments(q_rows, p.wq, p.seg);
   cudaStream_t st = (cudaStream_t)stream;
   if (int s = launch_list(a, st)) return s;

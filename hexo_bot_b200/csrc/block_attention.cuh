@@ -366,20 +366,6 @@ struct BaTile {
   }
 };
 
-// Writes row r (0 / 1) of an accumulator group (channels 16 n2 ... of two 8-wide
-// tiles) as 16-byte pieces: lane pairs swap halves so that even lanes hold four
-// channels of the first tile, odd lanes of the second.
-__device__ __forceinline__ void ba_store16(float* p, const float (&t0)[4], const float (&t1)[4], int r, int n2, int dim,
-                                           bool ok) {
-  const int lane = threadIdx.x & 31;
-  const bool odd = lane & 1;
-  const float s0 = odd ? t0[2 * r] : t1[2 * r], s1 = odd ? t0[2 * r + 1] : t1[2 * r + 1];
-  const float g0 = __shfl_xor_sync(0xffffffffu, s0, 1), g1 = __shfl_xor_sync(0xffffffffu, s1, 1);
-  const int c = 16 * n2 + (odd ? 8 : 0) + 2 * (lane & 2);
-  const float4 v = odd ? make_float4(g0, g1, t1[2 * r], t1[2 * r + 1]) : make_float4(t0[2 * r], t0[2 * r + 1], g0, g1);
-  if (ok && c < dim) *reinterpret_cast<float4*>(p + c) = v;
-}
-
 // ---- forward, many queries -----------------------------------------------------
 // Tiles of 128 listed rows on the fifth-generation tensor cores, one row a
 // thread: S = Q K^T into TMEM; each thread reads its row of S, takes maximum,
@@ -975,235 +961,288 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
   if (row < rows && c == 0) a.delta[row] = s;
 }
 
-// One CTA per (segment, key block): BK / 16 warps, each owning 16 keys and
-// their dk, dv rows in registers over all listed rows. Row tiles of TR rows
-// pass through shared memory; scores are computed transposed (keys x rows), so
-// that p and ds are the left operands of dv += p do and dk += ds q without
-// leaving the registers; ds also goes through shared memory, from where the
-// warps form dq = ds k, a part of each (row, block) pair as in the forward.
-template <int DP>
-constexpr int ba_bwd_rows() {
-  return DP == 128 ? 32 : 64;
+// Work items as in the forward: one key block and a segment of the queries that
+// chose it, tiles of 128 listed rows, a row a thread. Five products a tile on the
+// tensor cores, all from shared memory:
+//   S = Q K^T, dP = dO V^T                     128 rows x BK keys, into TMEM
+//   p = 2^(S - lse), ds = p (dP - delta)       by the row's thread, to 16 bits
+//   [dV; .] += [P | dS]^T dO, [.; dK] += [P | dS]^T Q   over the item's tiles, in TMEM
+//   dQ = dS K                                  128 rows, a part of each pair
+// P and dS are written [row][key] and read as M-major operands; for blocks of up
+// to 64 keys both go through one 128-row operand (half of each result is not
+// used), for 128 keys each is one. dQ lies over S and dP, which are done with.
+// An mma.sync form, 64 rows a tile, took 310 us where this one takes @@ (8192
+// rows, 8 heads of 64, 16 of 128 blocks).
+constexpr int kBaBwdThreads = 128;
+
+template <int DP, int BK>
+constexpr int ba_bwd_tmem() {
+  constexpr int n = (2 * BK > DP ? 2 * BK : DP) + 2 * DP;
+  return n <= 128 ? 128 : n <= 256 ? 256 : 512;
 }
 template <int DP, int BK>
 constexpr int ba_bwd_smem() {
-  constexpr int TR = ba_bwd_rows<DP>();
-  return 2 * BK * DP * 2 + 2 * 2 * TR * DP * 2 + BK * TR * 2 + 2 * TR * 16 + kBaChunk * 4;
+  constexpr int keys = BK > 64 ? 2 : 1;  // 64-key panels of P and dS
+  constexpr int need = 1024 + ba_panels(DP) * (2 * BK + 2 * kBaFwdRows) * 128 + 2 * keys * kBaFwdRows * 128 + kBaChunk * 4 +
+                       kBaFwdRows * 20;
+  constexpr int least = 232448 / (512 / ba_bwd_tmem<DP, BK>() + 1) + 1;
+  return need > least ? need : least;
 }
+template <int DP, int BK>
+constexpr int ba_bwd_ctas() {
+  constexpr int t = 512 / ba_bwd_tmem<DP, BK>(), m = 233472 / (ba_bwd_smem<DP, BK>() + 2048);
+  return t < m ? t : m;
+}
+constexpr uint32_t kIdescAMn = 1u << 15;  // left operand M-major
 
 template <typename T, int DP, int BK>
-__global__ __launch_bounds__(BK * 2) void block_attn_bwd_kernel(const BaArgs a) {
-  constexpr int NW = BK / 16, THREADS = NW * 32, TR = ba_bwd_rows<DP>();
-  constexpr int TILE = TR * DP * 2;
-  extern __shared__ __align__(128) char ba_smem[];
-  const uint32_t ks = smem_u32(ba_smem), vs = ks + BK * DP * 2;
-  const uint32_t qs = vs + BK * DP * 2;        // [2][TR][DP]
-  const uint32_t gs = qs + 2 * TILE;           // [2][TR][DP]
-  const uint32_t ds = gs + 2 * TILE;           // [BK][TR]
-  char* tail = ba_smem + 2 * BK * DP * 2 + 4 * TILE + BK * TR * 2;
-  // per row of a tile: (lse in log2 units, delta) and where its dq part goes
-  float2* stat = reinterpret_cast<float2*>(tail);                    // [2][TR]
-  int* dst = reinterpret_cast<int*>(tail + 2 * TR * 8);              // [2][TR]
-  uint32_t* list = reinterpret_cast<uint32_t*>(tail + 2 * TR * 16);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t u = blockIdx.x;
-  const int sg = (int)(u % (uint32_t)a.nseg);
-  const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
-  const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  int first_group = a.w0 / kBaMark + sg * a.seg;
-  const int end = min(first_group + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
+__global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_attn_bwd_kernel(const BaArgs a) {
+  constexpr int PAN = ba_panels(DP), CH = DP / 8, ROWS = kBaFwdRows, PK = BK > 64 ? 2 : 1;
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t KB = PAN * BK * 128, QB = PAN * ROWS * 128, PB = PK * ROWS * 128;
+  constexpr int OW = DP < 32 ? DP : 32;  // channels staged at a time
+  extern __shared__ char ba_smem_raw[];
+  char* ba_smem = ba_smem_raw + (1024 - (smem_u32(ba_smem_raw) & 1023)) % 1024;
+  const uint32_t ks = smem_u32(ba_smem), vs = ks + KB, qs = vs + KB, gs = qs + QB, ps = gs + QB, dss = ps + PB;
+  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB + 2 * PB);
+  long long* qoff = reinterpret_cast<long long*>(list + kBaChunk);  // [128] rows of the tile being loaded: q
+  long long* goff = qoff + ROWS;                                     // [128] and dout
+  int* dst = reinterpret_cast<int*>(goff + ROWS);                    // [128]: parts of the tile being stored
+  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ uint32_t tmem_slot, next_item;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t items = (uint32_t)a.nbh * (uint32_t)a.nb * (uint32_t)a.nseg;
   const int G = a.group;
-  const int have = max(0, min(BK, ba_kv_len(a, b) - j * BK));
-  int rows = 0;  // of the chunk at hand
-  const T* kp = (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s;
-  const T* vp = (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s;
-  const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
-  const T* gp = (const T*)a.go.p + b * a.go.b + (long long)h * G * a.go.h;
-  constexpr int CH = DP / 8;
-  auto load_tile = [&](int t, int buf) {
-    for (int x = threadIdx.x; x < TR * CH; x += THREADS) {
-      const int r = x / CH, c = x - r * CH;
-      const int row = t * TR + r;
-      const bool ok = row < rows && c * 8 < a.dim;
-      const T *sq = qp, *sgr = gp;
-      if (ok) {
-        const int li = ba_div_group(a, row), g = row - li * G;
-        const long long i = list[li] >> 6;
-        sq = qp + g * a.q.h + i * a.q.s + c * 8;
-        sgr = gp + g * a.go.h + i * a.go.s + c * 8;
-      }
-      cp_async16(ba_at<DP>(qs + buf * TILE, r, c), sq, ok ? 16 : 0);
-      cp_async16(ba_at<DP>(gs + buf * TILE, r, c), sgr, ok ? 16 : 0);
-    }
-    for (int r = threadIdx.x; r < TR; r += THREADS) {
-      const int row = t * TR + r;
-      float2 st = make_float2(INFINITY, 0.f);  // rows that are not there: weight 0
-      int to = -1;
-      if (row < rows) {
-        const int li = ba_div_group(a, row), g = row - li * G;
-        const uint32_t e = list[li];
-        const int i = (int)(e >> 6);
-        const long long qrow = (long long)bh * a.q_rows + i;
-        // a row all of whose scores are -inf has no weights
-        const float l = a.lse[((long long)b * a.kv_heads * G + h * G + g) * a.q_rows + i];
-        st = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, a.delta[qrow * G + g]);
-        to = ((lbh * a.wq + (i - a.w0)) * G + g) * a.topk + (int)(e & 63);
-      }
-      stat[buf * TR + r] = st;
-      dst[buf * TR + r] = to;
-    }
-  };
-  float dk[DP / 8][4], dv[DP / 8][4];
-#pragma unroll
-  for (int x = 0; x < DP / 8; ++x)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dk[x][e] = dv[x][e] = 0.f;
-  const int k0 = warp * 16;
-  const bool live0 = k0 + (lane >> 2) < have, live1 = k0 + (lane >> 2) + 8 < have;
-  bool loaded = false;
-  for (int gq = have > 0 ? first_group : end; gq < end;) {
-    rows = ba_fill<THREADS>(a, bh, j, gq, end, list) * G;
-    if (rows == 0) continue;
-    if (!loaded) {
-      ba_load_rows<T, DP>(ks, kp, a.k.s, BK, have, a.dim, threadIdx.x, THREADS);
-      ba_load_rows<T, DP>(vs, vp, a.v.s, BK, have, a.dim, threadIdx.x, THREADS);
-      loaded = true;
-    }
-    const int tiles = (rows + TR - 1) / TR;
-    load_tile(0, 0);
-    cp_async_commit();
-    for (int t = 0; t < tiles; ++t) {
-      const int buf = t & 1;
-      if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
-      cp_async_commit();
-      cp_async_wait<1>();
-      __syncthreads();
-      const uint32_t qt = qs + buf * TILE, gt = gs + buf * TILE;
-      float s[TR / 8][4], dp[TR / 8][4];
-#pragma unroll
-      for (int x = 0; x < TR / 8; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][e] = dp[x][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        uint32_t fk[4], fv[4];
-        ldmatrix_x4(fk, ba_at<DP>(ks, k0 + (lane & 15), 2 * kk + (lane >> 4)));
-        ldmatrix_x4(fv, ba_at<DP>(vs, k0 + (lane & 15), 2 * kk + (lane >> 4)));
-#pragma unroll
-        for (int x = 0; x < TR / 16; ++x) {
-          uint32_t f[4];
-          ldmatrix_x4(f, ba_at<DP>(qt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-          const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
-          MmaTraits<T>::mma(s[2 * x], fk, b0);
-          MmaTraits<T>::mma(s[2 * x + 1], fk, b1);
-          ldmatrix_x4(f, ba_at<DP>(gt, 16 * x + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-          const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
-          MmaTraits<T>::mma(dp[2 * x], fv, c0);
-          MmaTraits<T>::mma(dp[2 * x + 1], fv, c1);
-        }
-      }
-      // p = 2^(s - lse), ds = p (dp - delta): columns are rows of the tile
-#pragma unroll
-      for (int x = 0; x < TR / 8; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 st = stat[buf * TR + 8 * x + 2 * (lane & 3) + (e & 1)];
-          const bool live = e >> 1 ? live1 : live0;
-          s[x][e] = live ? ba_exp2(fmaf(s[x][e], a.scale_log2, -st.x)) : 0.f;
-          dp[x][e] = live ? s[x][e] * (dp[x][e] - st.y) : 0.f;
-        }
-      // p and ds are rounded to the inputs' type for the matrix unit (as the
-      // forward rounds p); their products are added in 32 bits
-      uint32_t fp[TR / 16][4], fd[TR / 16][4];
-#pragma unroll
-      for (int x = 0; x < TR / 16; ++x) {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          fp[x][2 * hf] = MmaTraits<T>::pack(s[2 * x + hf][0], s[2 * x + hf][1]);
-          fp[x][2 * hf + 1] = MmaTraits<T>::pack(s[2 * x + hf][2], s[2 * x + hf][3]);
-          fd[x][2 * hf] = MmaTraits<T>::pack(dp[2 * x + hf][0], dp[2 * x + hf][1]);
-          fd[x][2 * hf + 1] = MmaTraits<T>::pack(dp[2 * x + hf][2], dp[2 * x + hf][3]);
-          // ds to shared memory as [key][row]
-          const uint32_t a0 = ba_at<TR>(ds, k0 + (lane >> 2), 2 * x + hf) + 4 * (lane & 3);
-          const uint32_t a1 = ba_at<TR>(ds, k0 + (lane >> 2) + 8, 2 * x + hf) + 4 * (lane & 3);
-          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a0), "r"(fd[x][2 * hf]) : "memory");
-          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(a1), "r"(fd[x][2 * hf + 1]) : "memory");
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < TR / 16; ++x)
-#pragma unroll
-        for (int nn = 0; nn < DP / 16; ++nn) {
-          uint32_t f[4];
-          ldmatrix_x4_trans(f, ba_at<DP>(gt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
-          const uint32_t b0[2] = {f[0], f[1]}, b1[2] = {f[2], f[3]};
-          MmaTraits<T>::mma(dv[2 * nn], fp[x], b0);
-          MmaTraits<T>::mma(dv[2 * nn + 1], fp[x], b1);
-          ldmatrix_x4_trans(f, ba_at<DP>(qt, 16 * x + (lane & 15), 2 * nn + (lane >> 4)));
-          const uint32_t c0[2] = {f[0], f[1]}, c1[2] = {f[2], f[3]};
-          MmaTraits<T>::mma(dk[2 * nn], fd[x], c0);
-          MmaTraits<T>::mma(dk[2 * nn + 1], fd[x], c1);
-        }
-      __syncthreads();
-      // dq parts: units of 16 rows x 16 channels, spread over the warps
-      for (int unit = warp; unit < (TR / 16) * (DP / 16); unit += NW) {
-        const int mt = unit % (TR / 16), nt = unit / (TR / 16);
-        if (nt * 16 >= a.dim || t * TR + mt * 16 >= rows) continue;
-        float acc[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[x][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-          uint32_t fa[4], fb[4];
-          ldmatrix_x4_trans(fa, ba_at<TR>(ds, 16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * mt + ((lane >> 3) & 1)));
-          ldmatrix_x4_trans(fb, ba_at<DP>(ks, 16 * kk + (lane & 15), 2 * nt + (lane >> 4)));
-          const uint32_t b0[2] = {fb[0], fb[1]}, b1[2] = {fb[2], fb[3]};
-          MmaTraits<T>::mma(acc[0], fa, b0);
-          MmaTraits<T>::mma(acc[1], fa, b1);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int to = dst[buf * TR + mt * 16 + (lane >> 2) + 8 * r];
-          ba_store16(a.part + (long long)to * a.dim, acc[0], acc[1], r, nt, a.dim, to >= 0);
-        }
-      }
-      __syncthreads();  // ds, the tile and its stats are written over from here on
-    }
+  const uint32_t bar_s = smem_u32(&bars[0]), bar_o = smem_u32(&bars[1]);
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), ba_bwd_tmem<DP, BK>());
+    tmem_relinquish();
   }
-  cp_async_wait_all();
-  // keys of this block: final rows, or this segment's part
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int key = k0 + (lane >> 2) + 8 * r;
-    if (a.nseg_all > 1) {
-      float* p = a.kv_part + ((((long long)bh * a.nb + j) * a.nseg_all + a.seg0 + sg) * 2 * BK + key) * a.dim;
-#pragma unroll
-      for (int x = 0; x < DP / 8; ++x)
-        if (x * 8 < a.dim) {
-          *reinterpret_cast<float2*>(p + x * 8 + 2 * (lane & 3)) = make_float2(dk[x][2 * r], dk[x][2 * r + 1]);
-          *reinterpret_cast<float2*>(p + (long long)BK * a.dim + x * 8 + 2 * (lane & 3)) =
-              make_float2(dv[x][2 * r], dv[x][2 * r + 1]);
-        }
-    } else if (j * BK + key < a.kv_rows) {
-      T* pk = (T*)a.dk.p + b * a.dk.b + h * a.dk.h + (long long)(j * BK + key) * a.dk.s;
-      T* pv = (T*)a.dv.p + b * a.dv.b + h * a.dv.h + (long long)(j * BK + key) * a.dv.s;
-#pragma unroll
-      for (int x = 0; x < DP / 8; ++x)
-        if (x * 8 < a.dim) {
-          *reinterpret_cast<uint32_t*>(pk + x * 8 + 2 * (lane & 3)) =
-              MmaTraits<T>::pack(dk[x][2 * r] * a.scale, dk[x][2 * r + 1] * a.scale);
-          *reinterpret_cast<uint32_t*>(pv + x * 8 + 2 * (lane & 3)) = MmaTraits<T>::pack(dv[x][2 * r], dv[x][2 * r + 1]);
-        }
-    }
+  if (tid == 0) {
+    mbar_init(bar_s, 1);
+    mbar_init(bar_o, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, lanes = (uint32_t)(warp * 32) << 16;
+  const uint32_t s_tm = tmem, dp_tm = tmem + BK, dq_tm = tmem;
+  const uint32_t dv_tm = tmem + (2 * BK > DP ? 2 * BK : DP), dk_tm = dv_tm + DP;
+  bool ok = true;
+  uint32_t phase = 0;
+  for (uint32_t u = blockIdx.x; u < items;) {
+    const int sg = (int)(u % (uint32_t)a.nseg);
+    const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
+    const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
+    const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+    int g = a.w0 / kBaMark + sg * a.seg;
+    const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
+    const int have = max(0, min(BK, ba_kv_len(a, b) - j * BK));
+    tc_fence_before();
+    __syncthreads();  // the item before is done with the keys and with dv, dk
+    if (tid == 0) next_item = gridDim.x + atomicAdd(a.ticket, 1u);
+    if (have == 0) g = end;
+    const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
+    const T* gp = (const T*)a.go.p + b * a.go.b + (long long)h * G * a.go.h;
+    if (have > 0) {  // on their way while the list is made
+      ba_load_panels<T, DP, BK>(ks, (const T*)a.k.p + b * a.k.b + h * a.k.h + (long long)j * BK * a.k.s, a.k.s, have, a.dim);
+      ba_load_panels<T, DP, BK>(vs, (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s, a.v.s, have, a.dim);
+    }
+    bool any = false;  // dv, dk hold something of this item
+    while (g < end) {
+      const int n = ba_fill<kBaBwdThreads>(a, bh, j, g, end, list);
+      if (n == 0) continue;
+      const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
+      float lse = INFINITY, delta = 0.f;  // of this thread's row of the next tile
+      int at = -1;
+      // a warp loads the 32 rows whose offsets its lanes worked out
+      auto load_tile = [&](int tile) {
+        const int row = tile * ROWS + tid;
+        long long off = -1, og = 0;
+        lse = INFINITY;  // rows that are not there: weight 0
+        delta = 0.f;
+        at = -1;
+        if (row < rows) {
+          const int li = ba_div_group(a, row), gr = row - li * G;
+          const uint32_t e = list[li];
+          const int i = (int)(e >> 6);
+          off = gr * a.q.h + (long long)i * a.q.s;
+          og = gr * a.go.h + (long long)i * a.go.s;
+          // a row all of whose scores are -inf has no weights
+          const float l = a.lse[((long long)b * a.kv_heads * G + h * G + gr) * a.q_rows + i];
+          lse = l == -INFINITY ? INFINITY : l * kLog2e;
+          delta = a.delta[((long long)bh * a.q_rows + i) * G + gr];
+          // where its dq part goes (a window's parts number less than 2^31)
+          at = ((lbh * a.wq + (i - a.w0)) * G + gr) * a.topk + (int)(e & 63);
+        }
+        qoff[tid] = off;
+        goff[tid] = og;
+        __syncwarp();
+#pragma unroll
+        for (int x0 = 0; x0 < 32 * CH; x0 += 32) {
+          const int r = warp * 32 + (x0 + lane) / CH, c = (x0 + lane) % CH;
+          const long long o = qoff[r];
+          const bool in = o >= 0 && c * 8 < a.dim;
+          cp_async16(ba_panel_at(qs, ROWS, r, c), in ? qp + o + c * 8 : qp, in ? 16 : 0);
+          cp_async16(ba_panel_at(gs, ROWS, r, c), in ? gp + goff[r] + c * 8 : gp, in ? 16 : 0);
+        }
+        __syncwarp();
+      };
+      load_tile(0);
+      for (int t = 0; t < tiles; ++t) {
+        const float lse_t = lse, delta_t = delta;
+        dst[tid] = at;
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();  // the tile is there; every thread has read the dq of the one before
+        tc_fence_after();
+        if (tid == 0) {
+          constexpr uint32_t id = mma_idesc(BK, BF);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            tc_mma_f16(s_tm, sw128_desc(qs + kk / 4 * ROWS * 128 + kk % 4 * 32),
+                       sw128_desc(ks + kk / 4 * BK * 128 + kk % 4 * 32), id, kk > 0);
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            tc_mma_f16(dp_tm, sw128_desc(gs + kk / 4 * ROWS * 128 + kk % 4 * 32),
+                       sw128_desc(vs + kk / 4 * BK * 128 + kk % 4 * 32), id, kk > 0);
+          tc_commit(bar_s);
+        }
+        ok = ok && mbar_wait(bar_s, phase);
+        tc_fence_after();
+        // p and ds are rounded to the inputs' type for the matrix unit (as the
+        // forward rounds p); their products are added in 32 bits
+#pragma unroll
+        for (int c0 = 0; c0 < BK; c0 += 32) {
+          float s[32], dp[32];
+          ba_tmem_ld<32>(s_tm + lanes + c0, s);
+          ba_tmem_ld<32>(dp_tm + lanes + c0, dp);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            s[x] = ba_exp2(fmaf(s[x], a.scale_log2, -lse_t));
+            dp[x] = s[x] * (dp[x] - delta_t);
+          }
+          if (c0 + 32 > have) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (c0 + x >= have) s[x] = dp[x] = 0.f;
+          }
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            const uint32_t to = ba_panel_at(0, ROWS, tid, (c0 + x) / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(ps + to), "r"(MmaTraits<T>::pack(s[x], s[x + 1])),
+                         "r"(MmaTraits<T>::pack(s[x + 2], s[x + 3])), "r"(MmaTraits<T>::pack(s[x + 4], s[x + 5])),
+                         "r"(MmaTraits<T>::pack(s[x + 6], s[x + 7]))
+                         : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dss + to),
+                         "r"(MmaTraits<T>::pack(dp[x], dp[x + 1])), "r"(MmaTraits<T>::pack(dp[x + 2], dp[x + 3])),
+                         "r"(MmaTraits<T>::pack(dp[x + 4], dp[x + 5])), "r"(MmaTraits<T>::pack(dp[x + 6], dp[x + 7]))
+                         : "memory");
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          constexpr uint32_t id_kv = mma_idesc(DP, BF) | kIdescAMn | kIdescBMn, id_q = mma_idesc(DP, BF) | kIdescBMn;
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            tc_mma_f16(dq_tm, sw128_desc(dss + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
+                       kk > 0);
+          // [P | dS]: the panel after P's first is dS for up to 64 keys, P's second for 128
+#pragma unroll
+          for (int kk = 0; kk < ROWS / 16; ++kk)
+            tc_mma_f16(dv_tm, ba_mn_desc(ps + kk * 2048, ROWS * 128), ba_mn_desc(gs + kk * 2048, ROWS * 128), id_kv,
+                       any || kk > 0);
+#pragma unroll
+          for (int kk = 0; kk < ROWS / 16; ++kk)
+            tc_mma_f16(dk_tm, ba_mn_desc((BK > 64 ? dss : ps) + kk * 2048, ROWS * 128), ba_mn_desc(qs + kk * 2048, ROWS * 128),
+                       id_kv, any || kk > 0);
+          tc_commit(bar_o);
+        }
+        any = true;
+        ok = ok && mbar_wait(bar_o, phase);
+        phase ^= 1;
+        tc_fence_after();
+        if (t + 1 < tiles) load_tile(t + 1);
+        // dq to its parts: a warp's 32 rows through P's bytes, which are done with
+        const uint32_t stage = ps + warp * 32 * 128;
+#pragma unroll
+        for (int c0 = 0; c0 < DP; c0 += OW) {
+          float o[OW];
+          ba_tmem_ld<OW>(dq_tm + lanes + c0, o);
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < OW; x += 4)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(stage + lane * 128 + (((x / 4) ^ (lane & 7)) << 4)),
+                         "f"(o[x]), "f"(o[x + 1]), "f"(o[x + 2]), "f"(o[x + 3])
+                         : "memory");
+          __syncwarp();
+          constexpr int LR = OW / 4;  // lanes of a row
+#pragma unroll
+          for (int x = 0; x < LR; ++x) {
+            const int r = x * (32 / LR) + lane / LR, c = lane % LR;
+            const uint4 v = lds128(stage + r * 128 + ((c ^ (r & 7)) << 4));
+            const int to = dst[warp * 32 + r];
+            if (to >= 0 && c0 + c * 4 < a.dim)
+              *reinterpret_cast<uint4*>(a.part + (long long)to * a.dim + c0 + c * 4) = v;
+          }
+        }
+        __syncwarp();  // dst is written over by the next tile
+      }
+    }
+    cp_async_wait_all();  // keys of an item that nobody chose
+    // the item's keys: final rows, or this segment's part; a lane of TMEM a key
+#pragma unroll
+    for (int w = 0; w < (BK > 64 ? 2 : 1); ++w) {
+      const bool is_v = BK > 64 ? w == 0 : tid < 64;  // this warp's half: dv or dk
+      const int key = BK > 64 ? tid : tid & 63;
+      const float f = !ok ? __int_as_float(0x7fc00000) : is_v ? 1.f : a.scale;  // a wait that gave up leaves no number
+#pragma unroll
+      for (int c0 = 0; c0 < DP; c0 += 16) {
+        float o[16];
+        ba_tmem_ld<16>((is_v ? dv_tm : dk_tm) + lanes + c0, o);
+        if (!any || key >= have) {  // dead keys: zeros, whatever the rows hold
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[x] = 0.f;
+        }
+        if (key >= BK) continue;
+#pragma unroll
+        for (int x = 0; x < 16; x += 8) {
+          if (c0 + x >= a.dim) continue;
+          if (a.nseg_all > 1) {
+            float4* p = reinterpret_cast<float4*>(
+                a.kv_part + ((((long long)bh * a.nb + j) * a.nseg_all + a.seg0 + sg) * 2 * BK + (is_v ? BK : 0) + key) * a.dim +
+                c0 + x);
+            // the sum over the segments scales
+            const float one = ok ? 1.f : f;
+            p[0] = make_float4(o[x] * one, o[x + 1] * one, o[x + 2] * one, o[x + 3] * one);
+            p[1] = make_float4(o[x + 4] * one, o[x + 5] * one, o[x + 6] * one, o[x + 7] * one);
+          } else if (j * BK + key < a.kv_rows) {
+            const HeadsView& d = is_v ? a.dv : a.dk;
+            T* p = (T*)d.p + b * d.b + h * d.h + (long long)(j * BK + key) * d.s + c0 + x;
+            *reinterpret_cast<uint4*>(p) =
+                make_uint4(MmaTraits<T>::pack(o[x] * f, o[x + 1] * f), MmaTraits<T>::pack(o[x + 2] * f, o[x + 3] * f),
+                           MmaTraits<T>::pack(o[x + 4] * f, o[x + 5] * f), MmaTraits<T>::pack(o[x + 6] * f, o[x + 7] * f));
+          }
+        }
+      }
+    }
+    __syncthreads();
+    u = next_item;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, ba_bwd_tmem<DP, BK>());
 }
 
 // dq of the window: the sum of each row's parts.
 template <typename T>
 __global__ __launch_bounds__(kBaJoinThreads) void block_attn_dq_kernel(const BaArgs a) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;  // for the next window
   const BaRow r(a);
   const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
   const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
