@@ -169,19 +169,19 @@ void put(RotArgs* a, int slot, const sb_heads* x, const sb_heads* dy, const sb_h
 // ---- block selection ----------------------------------------------------------
 constexpr int kSelFewRows = 8;  // up to so many queries of a sequence take the few-query kernel
 
-template <typename T, int PER>
+template <typename T, int PER, int LPR>
 int launch_select_per(const SelArgs& a, unsigned grid, cudaStream_t st) {
   const int smem = sel_smem_bytes(a.tile, a.nb, a.dim);
-  if (int s = ensure_smem(reinterpret_cast<const void*>(block_select_kernel<T, PER>), smem)) return s;
-  block_select_kernel<T, PER><<<grid, kSelThreads, smem, st>>>(a);
+  if (int s = ensure_smem(reinterpret_cast<const void*>(block_select_kernel<T, PER, LPR>), smem)) return s;
+  block_select_kernel<T, PER, LPR><<<grid, kSelThreads, smem, st>>>(a);
   return check_launch("block_select_kernel");
 }
 template <typename T>
 int launch_select(const SelArgs& a, unsigned grid, cudaStream_t st) {
-  if (a.nb <= 40) return launch_select_per<T, 5>(a, grid, st);
-  if (a.nb <= 64) return launch_select_per<T, 8>(a, grid, st);
-  if (a.nb <= 128) return launch_select_per<T, 16>(a, grid, st);
-  return launch_select_per<T, 0>(a, grid, st);
+  if (a.nb <= 40) return launch_select_per<T, 20, 2>(a, grid, st);
+  if (a.nb <= 64) return launch_select_per<T, 32, 2>(a, grid, st);
+  if (a.nb <= 128) return launch_select_per<T, 32, 4>(a, grid, st);
+  return launch_select_per<T, 0, 32>(a, grid, st);
 }
 template <typename T, int PER>
 int launch_select_few_per(const SelArgs& a, unsigned rows, int cluster, cudaStream_t st) {

@@ -1054,7 +1054,7 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
       const int n = ba_fill<kBaBwdThreads>(a, bh, j, g, end, list);
       if (n == 0) continue;
       const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
-      float lse = INFINITY, delta = 0.f;  // of this thread's row of the next tile
+      float lse = INFINITY, delta = 0.f;  // of this thread's row of the next tile, as loaded
       int at = -1;
       // a warp loads the 32 rows whose offsets its lanes worked out
       auto load_tile = [&](int tile) {
@@ -1069,9 +1069,7 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
           const int i = (int)(e >> 6);
           off = gr * a.q.h + (long long)i * a.q.s;
           og = gr * a.go.h + (long long)i * a.go.s;
-          // a row all of whose scores are -inf has no weights
-          const float l = a.lse[((long long)b * a.kv_heads * G + h * G + gr) * a.q_rows + i];
-          lse = l == -INFINITY ? INFINITY : l * kLog2e;
+          lse = a.lse[((long long)b * a.kv_heads * G + h * G + gr) * a.q_rows + i];
           delta = a.delta[((long long)bh * a.q_rows + i) * G + gr];
           // where its dq part goes (a window's parts number less than 2^31)
           at = ((lbh * a.wq + (i - a.w0)) * G + gr) * a.topk + (int)(e & 63);
@@ -1091,7 +1089,8 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
       };
       load_tile(0);
       for (int t = 0; t < tiles; ++t) {
-        const float lse_t = lse, delta_t = delta;
+        // a row all of whose scores are -inf has no weights
+        const float lse_t = lse == -INFINITY ? INFINITY : lse * kLog2e, delta_t = delta;
         dst[tid] = at;
         cp_async_wait_all();
         fence_proxy_async_smem();

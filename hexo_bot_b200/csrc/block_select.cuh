@@ -446,20 +446,21 @@ __device__ __forceinline__ bool sel_row_fast(const SelArgs& a, const float* s, c
   return true;
 }
 
-// Four rows by a warp, eight lanes a row, scores in registers (live <= 8 PER).
+// 32 / LPR rows by a warp, LPR lanes a row, scores in registers (live <= LPR PER).
 // Lanes of a row whose 32-bit scores settle it write it; returns whether this
 // lane's row is settled. `on`: this lane's row exists. The border is looked for
 // by halving the range of the scores until as many as wanted lie above.
-template <int PER>
-__device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, float err, bool on, int* out) {
-  const int lane = threadIdx.x & 31, id = lane & 7, shift = lane & 24;
+template <int PER, int LPR>
+__device__ __forceinline__ bool sel_rows(const float* s, const SelRow& r, float err, bool on, int* out) {
+  const int lane = threadIdx.x & 31, id = lane & (LPR - 1), shift = lane & ~(LPR - 1);
+  constexpr uint32_t kRow = (1u << LPR) - 1u;  // a row's lanes in a ballot
   const int want = r.want();
   float v[PER];
   float most = -INFINITY, least = INFINITY;
   bool odd = !(err < INFINITY);
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
-    const int j = id + 8 * x;
+    const int j = id + LPR * x;
     v[x] = -INFINITY;  // blocks that do not compete are never above the border
     if (j < r.live && !r.is_forced(j)) {
       v[x] = s[j];
@@ -468,9 +469,9 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
       least = fminf(least, v[x]);
     }
   }
-  odd = (__ballot_sync(0xffffffffu, odd) >> shift & 0xffu) != 0;
+  odd = (__ballot_sync(0xffffffffu, odd) >> shift & kRow) != 0;
 #pragma unroll
-  for (int m = 1; m < 8; m <<= 1) {
+  for (int m = 1; m < LPR; m <<= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
     least = fminf(least, __shfl_xor_sync(0xffffffffu, least, m));
   }
@@ -485,7 +486,7 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
 #pragma unroll
     for (int x = 0; x < PER; ++x) c += v[x] >= mid;
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) c += __shfl_xor_sync(0xffffffffu, c, m);
+    for (int m = 1; m < LPR; m <<= 1) c += __shfl_xor_sync(0xffffffffu, c, m);
     if (busy) {
       if (c == want) {
         exact = true;
@@ -505,7 +506,7 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
     dropped = in ? dropped : fmaxf(dropped, v[x]);
   }
 #pragma unroll
-  for (int m = 1; m < 8; m <<= 1) {
+  for (int m = 1; m < LPR; m <<= 1) {
     kept = fminf(kept, __shfl_xor_sync(0xffffffffu, kept, m));
     dropped = fmaxf(dropped, __shfl_xor_sync(0xffffffffu, dropped, m));
   }
@@ -514,15 +515,15 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
   int n = 0;
 #pragma unroll
   for (int x = 0; x < PER; ++x) {
-    const int j = id + 8 * x;
+    const int j = id + LPR * x;
     const bool in = j < r.live && (all || r.is_forced(j) || (search && v[x] >= t));
-    const uint32_t m = __ballot_sync(0xffffffffu, in) >> shift & 0xffu;
+    const uint32_t m = __ballot_sync(0xffffffffu, in) >> shift & kRow;
     const int at = n + __popc(m & ((1u << id) - 1u));
     if (write && in && at < r.topk) out[at] = j;
     n += __popc(m);
   }
   if (write)
-    for (int x = n + id; x < r.topk; x += 8) out[x] = -1;
+    for (int x = n + id; x < r.topk; x += LPR) out[x] = -1;
   return settled;
 }
 
@@ -531,7 +532,7 @@ __device__ __forceinline__ bool sel_rows_oct(const float* s, const SelRow& r, fl
 //   summed queries [2][tile][dp + 8] and a chunk of means [2][64][dp + 8] as
 //   bf16 pairs (x = hi + mid + rest, |rest| <= 2^-18 |x|), the rows' squares
 //   two lists of rows left to do
-// stride: an odd multiple of 8 (four rows' octets meet distinct banks); rows of
+// stride: an odd multiple of 8 (neighbouring rows meet distinct banks); rows of
 // dp + 8: an odd number of 16-byte chunks, so ldmatrix meets every bank once.
 __host__ __device__ inline int sel_stride(int nb) { return ((nb + 7) / 8 | 1) * 8; }
 __host__ __device__ inline int sel_dp(int dim) { return (dim + 15) / 16 * 16; }
@@ -563,8 +564,9 @@ __device__ __forceinline__ void sel_split8(const float (&x)[8], __nv_bfloat16* h
   *reinterpret_cast<RotVec<__nv_bfloat16, 8>*>(mid) = m;
 }
 
-// PER > 0: rows of up to 8 PER blocks, settled four a warp; 0: a warp a row.
-template <typename T, int PER>
+// PER > 0: rows of up to LPR PER blocks, LPR lanes a row (the fewer, the fewer
+// instructions a row: 16 x 2440 rows, 8 heads, 39 blocks 102 us with eight, 89 with two); 0: a warp a row.
+template <typename T, int PER, int LPR>
 __global__ __launch_bounds__(kSelThreads, 3) void block_select_kernel(const SelArgs a) {
   extern __shared__ __align__(16) char sel_smem[];
   const int D = a.dim, DP = sel_dp(D), RS = DP + 8, NBS = sel_stride(a.nb), TQ = a.tile, TQ16 = max(TQ, 16);
@@ -743,13 +745,13 @@ __global__ __launch_bounds__(kSelThreads, 3) void block_select_kernel(const SelA
     return unit * q + 1e-34f * (mmax + q) + 1e-40f;
   };
   if (PER > 0) {
-    for (int r0 = warp * 4; r0 < nl; r0 += kSelWarps * 4) {
-      const int r = r0 + (lane >> 3);
+    for (int r0 = warp * (32 / LPR); r0 < nl; r0 += kSelThreads / LPR) {
+      const int r = r0 + lane / LPR;
       const bool on = r < nl;
       const int rr = on ? r : 0;
       const SelRow row(a, i0 + rr, live);
-      const bool done = sel_rows_oct<PER ? PER : 1>(sc + rr * NBS, row, err_of(rr), on, out + (long long)rr * a.topk);
-      if (on && !done && (lane & 7) == 0) todo[atomicAdd(&todo_n, 1)] = r;
+      const bool done = sel_rows<PER ? PER : 1, LPR>(sc + rr * NBS, row, err_of(rr), on, out + (long long)rr * a.topk);
+      if (on && !done && lane % LPR == 0) todo[atomicAdd(&todo_n, 1)] = r;
     }
     __syncthreads();
   }
