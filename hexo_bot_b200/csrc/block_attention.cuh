@@ -980,11 +980,21 @@ constexpr int ba_bwd_tmem() {
   constexpr int n = (2 * BK > DP ? 2 * BK : DP) + 2 * DP;
   return n <= 128 ? 128 : n <= 256 ? 256 : 512;
 }
+// dq = dS K takes ds as a pair of 16-bit numbers. Its error from ds's rounding and
+// from that of the out which delta reads comes on top of its own rounding: 1.5 to
+// 1.7 times that in all with single ds (head_dim 16, or few keys a row), 1.1 to 1.3
+// with the pair; dk and dv, whose errors are independent over the rows, stay at 1.4
+// without. Heads of more than 64 channels with blocks of 128 have no shared memory
+// for it.
+template <int DP, int BK>
+constexpr bool ba_bwd_pair() {
+  return DP <= 64 || BK <= 64;
+}
 template <int DP, int BK>
 constexpr int ba_bwd_smem() {
   constexpr int keys = BK > 64 ? 2 : 1;  // 64-key panels of P and dS
-  constexpr int need = 1024 + ba_panels(DP) * (2 * BK + 2 * kBaFwdRows) * 128 + 2 * keys * kBaFwdRows * 128 + kBaChunk * 4 +
-                       kBaFwdRows * 20;
+  constexpr int need = 1024 + ba_panels(DP) * (2 * BK + 2 * kBaFwdRows) * 128 +
+                       (ba_bwd_pair<DP, BK>() ? 3 : 2) * keys * kBaFwdRows * 128 + kBaChunk * 4 + kBaFwdRows * 20;
   constexpr int least = 232448 / (512 / ba_bwd_tmem<DP, BK>() + 1) + 1;
   return need > least ? need : least;
 }
@@ -999,12 +1009,14 @@ template <typename T, int DP, int BK>
 __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_attn_bwd_kernel(const BaArgs a) {
   constexpr int PAN = ba_panels(DP), CH = DP / 8, ROWS = kBaFwdRows, PK = BK > 64 ? 2 : 1;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool PAIR = ba_bwd_pair<DP, BK>();
   constexpr uint32_t KB = PAN * BK * 128, QB = PAN * ROWS * 128, PB = PK * ROWS * 128;
   constexpr int OW = DP < 32 ? DP : 32;  // channels staged at a time
   extern __shared__ char ba_smem_raw[];
   char* ba_smem = ba_smem_raw + (1024 - (smem_u32(ba_smem_raw) & 1023)) % 1024;
-  const uint32_t ks = smem_u32(ba_smem), vs = ks + KB, qs = vs + KB, gs = qs + QB, ps = gs + QB, dss = ps + PB;
-  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB + 2 * PB);
+  const uint32_t ks = smem_u32(ba_smem), vs = ks + KB, qs = vs + KB, gs = qs + QB, ps = gs + QB, dss = ps + PB,
+                 dls = dss + PB;  // P, dS, and what dS's rounding left
+  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB + (PAIR ? 3 : 2) * PB);
   long long* qoff = reinterpret_cast<long long*>(list + kBaChunk);  // [128] rows of the tile being loaded: q
   long long* goff = qoff + ROWS;                                     // [128] and dout
   int* dst = reinterpret_cast<int*>(goff + ROWS);                    // [128]: parts of the tile being stored
@@ -1135,10 +1147,26 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
                          "r"(MmaTraits<T>::pack(s[x + 2], s[x + 3])), "r"(MmaTraits<T>::pack(s[x + 4], s[x + 5])),
                          "r"(MmaTraits<T>::pack(s[x + 6], s[x + 7]))
                          : "memory");
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dss + to),
-                         "r"(MmaTraits<T>::pack(dp[x], dp[x + 1])), "r"(MmaTraits<T>::pack(dp[x + 2], dp[x + 3])),
-                         "r"(MmaTraits<T>::pack(dp[x + 4], dp[x + 5])), "r"(MmaTraits<T>::pack(dp[x + 6], dp[x + 7]))
+            uint32_t hi[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) hi[y] = MmaTraits<T>::pack(dp[x + 2 * y], dp[x + 2 * y + 1]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dss + to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),
+                         "r"(hi[3])
                          : "memory");
+            if (PAIR) {
+              uint32_t lo[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                float2 h;
+                if constexpr (BF) h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi[y]));
+                else h = __half22float2(*reinterpret_cast<const __half2*>(&hi[y]));
+                // past the type's range hi is infinite, and the product says so
+                lo[y] = MmaTraits<T>::pack(isinf(h.x) ? 0.f : dp[x + 2 * y] - h.x, isinf(h.y) ? 0.f : dp[x + 2 * y + 1] - h.y);
+              }
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dls + to), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]),
+                           "r"(lo[3])
+                           : "memory");
+            }
           }
         }
         fence_proxy_async_smem();
@@ -1148,9 +1176,13 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
           tc_fence_after();
           constexpr uint32_t id_kv = mma_idesc(DP, BF) | kIdescAMn | kIdescBMn, id_q = mma_idesc(DP, BF) | kIdescBMn;
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
+          for (int kk = 0; kk < BK / 16; ++kk) {
             tc_mma_f16(dq_tm, sw128_desc(dss + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
                        kk > 0);
+            if (PAIR)
+              tc_mma_f16(dq_tm, sw128_desc(dls + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
+                         1);
+          }
           // [P | dS]: the panel after P's first is dS for up to 64 keys, P's second for 128
 #pragma unroll
           for (int kk = 0; kk < ROWS / 16; ++kk)
