@@ -33,6 +33,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+_MOST = 2**31 - 1
 _FLOATS = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 _COORDS = {torch.int64: _lib.DT_I64, torch.int32: _lib.DT_I32, torch.int16: _lib.DT_I16, torch.float32: _lib.DT_F32}
 
@@ -57,7 +58,16 @@ def _first(t: torch.Tensor, name: str) -> torch.Tensor:
         raise RuntimeError(f"{name} is on {t.device}: the kernels need CUDA tensors (no CPU fallback)")
     if t.dtype not in _FLOATS:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if max(t.shape) > _MOST:
+        raise ValueError(f"{name} has an axis of more than 2^31 - 1 elements")
     return t
+
+
+def _int(n: int, name: str, least: int) -> int:
+    """A size that the C side takes as a 32-bit integer."""
+    if not least <= n <= _MOST:
+        raise ValueError(f"{name} must lie in {least} to 2^31 - 1, got {n}")
+    return n
 
 
 def _heads(t: torch.Tensor, name: str) -> _lib.Heads:
@@ -275,8 +285,7 @@ def block_means(k, block, *, kv_lens=None):
 
     _first(k, "k")
     b, h, s, d = k.shape
-    if block < 1:
-        raise ValueError(f"block must be positive, got {block}")
+    _int(block, "block", 1)
     out = torch.empty(b, h, -(-s // block), d, dtype=torch.float32, device=k.device)
     lens, hk = _lens(kv_lens, "kv_lens", k), _heads(k, "k")
     _call(k, "block_means", _lib.lib().sb_block_means, hk, _FLOATS[k.dtype], lens, b, h, s, d, block, out.data_ptr())
@@ -294,8 +303,7 @@ def block_select(q, means, topk, block, kv_rows, *, kv_lens=None, q_lens=None, k
     b, hq, sq, d = q.shape
     if not isinstance(means, torch.Tensor) or means.dim() != 4:
         raise ValueError("means must be a (batch, kv heads, blocks, head_dim) tensor")
-    if block < 1 or kv_rows < 0:
-        raise ValueError(f"bad block {block} or kv_rows {kv_rows}")
+    _int(block, "block", 1), _int(kv_rows, "kv_rows", 0), _int(topk, "topk", 1), _int(keep_first, "keep_first", 0)
     hk = means.shape[1]
     _check(means, "means", q, (b, hk, -(-kv_rows // block), d), torch.float32)
     if not means.is_contiguous():
@@ -317,6 +325,7 @@ def _attn_args(q, k, v, index, block, scale):
     if not isinstance(index, torch.Tensor) or index.dim() != 4:
         raise ValueError("index must be a (batch, kv heads, rows, topk) tensor")
     topk = index.shape[3]
+    _int(block, "block", 1)
     _check(index, "index", q, (b, hk, sq, topk), torch.int32)
     if not index.is_contiguous():
         raise ValueError("index must be contiguous")

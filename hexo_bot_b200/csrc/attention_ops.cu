@@ -145,7 +145,8 @@ int check_rotary_shape(const char* what, int dtype, int batch, int heads, int ro
   if (!float_dtype(dtype)) return fail(SB_ERR_UNSUPPORTED, "%s: dtype %d (f32, f16, bf16)", what, dtype);
   if (batch < 0 || rows < 0 || heads < 1 || heads > 65535) return fail(SB_ERR_INVALID_ARG, "%s: bad sizes", what);
   if (dim < 1 || dim > kRotMaxDim) return fail(SB_ERR_UNSUPPORTED, "%s: head_dim %d (1 to %d)", what, dim, kRotMaxDim);
-  if ((long long)batch * rows > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", what);
+  // row numbers, rounded up to a warp's or a launch's next, stay below 2^31
+  if ((long long)batch * rows > 0x7fff0000ll) return fail(SB_ERR_UNSUPPORTED, "%s: more than 2^31 - 2^16 rows", what);
   return SB_OK;
 }
 
@@ -289,6 +290,7 @@ int check_ba(const char* what, int dtype, int batch, int q_heads, int kv_heads, 
   if (batch < 0 || q_rows < 0 || kv_rows < 0 || q_heads < 1 || kv_heads < 1)
     return fail(SB_ERR_INVALID_ARG, "%s: bad sizes", what);
   if (q_heads % kv_heads) return fail(SB_ERR_INVALID_ARG, "%s: %d query heads over %d key heads", what, q_heads, kv_heads);
+  if (kv_rows > 0x7fff0000) return fail(SB_ERR_UNSUPPORTED, "%s: %d key rows (at most 2^31 - 2^16)", what, kv_rows);
   if (q_rows > 1 << 26) return fail(SB_ERR_UNSUPPORTED, "%s: %d rows (at most 2^26)", what, q_rows);
   if (q_heads > 65535 || q_heads / kv_heads > 1024 || (long long)batch * kv_heads > 0x7fffffffll)
     return fail(SB_ERR_UNSUPPORTED, "%s: too many heads", what);
@@ -555,6 +557,7 @@ int sb_block_means(const sb_heads* k, int dtype, const int32_t* kv_lens, int bat
   const char* what = "block_means";
   if (!float_dtype(dtype)) return fail(SB_ERR_UNSUPPORTED, "%s: dtype %d (f32, f16, bf16)", what, dtype);
   if (batch < 0 || kv_heads < 1 || kv_rows < 0 || block < 1) return fail(SB_ERR_INVALID_ARG, "%s: bad sizes", what);
+  if ((long long)kv_rows + block > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "%s: rows and block exceed 2^31", what);
   if (head_dim < 1 || head_dim > kSelMaxDim)
     return fail(SB_ERR_UNSUPPORTED, "%s: head_dim %d (1 to %d)", what, head_dim, kSelMaxDim);
   if (batch == 0 || kv_rows == 0) return SB_OK;
@@ -597,6 +600,7 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
   if (!float_dtype(dtype)) return fail(SB_ERR_UNSUPPORTED, "%s: dtype %d (f32, f16, bf16)", what, dtype);
   if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_rows < 0 || kv_rows < 0 || block < 1)
     return fail(SB_ERR_INVALID_ARG, "%s: bad sizes", what);
+  if ((long long)kv_rows + block > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "%s: rows and block exceed 2^31", what);
   if (q_heads % kv_heads) return fail(SB_ERR_INVALID_ARG, "%s: %d query heads over %d key heads", what, q_heads, kv_heads);
   if (head_dim < 1 || head_dim > kSelMaxDim)
     return fail(SB_ERR_UNSUPPORTED, "%s: head_dim %d (1 to %d)", what, head_dim, kSelMaxDim);

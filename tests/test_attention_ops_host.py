@@ -46,6 +46,7 @@ def turn(x=None, dtype=_lib.DT_F16, rot=None, b=1, h=2, s=4, d=64, out=None):
         (dict(h=0), 1, "sizes"),
         (dict(b=-1), 1, "sizes"),
         (dict(b=1 << 16, s=1 << 16), 2, "2^31"),
+        (dict(b=1, s=2**31 - 1), 2, "2^31"),  # a warp's rows would pass 32 bits
         (dict(x=heads(data=None)), 1, "NULL"),
         (dict(x=heads(data=A16 + 1)), 1, "aligned"),
         (dict(out=heads(data=None)), 1, "NULL"),
@@ -112,6 +113,9 @@ def select(dtype=1, b=1, hq=4, hk=2, sq=8, sk=1000, d=64, block=64, topk=4, firs
     [
         (lambda: means(dtype=4), 2, "dtype"),
         (lambda: means(block=0), 1, "sizes"),
+        (lambda: means(s=2**31 - 1), 2, "2^31"),
+        (lambda: means(s=9, block=2**31 - 1), 2, "2^31"),
+        (lambda: select(sk=2**31 - 9, block=2**30), 2, "2^31"),
         (lambda: means(d=300), 2, "head_dim"),
         (lambda: means(out=None), 1, "means"),
         (lambda: means(lens=A16 + 1), 1, "misaligned"),
@@ -154,6 +158,8 @@ def attend(backward=False, q=None, dtype=1, b=1, hq=4, hk=2, sq=100, sk=1000, d=
         (dict(d=136), 2, "head_dim"),
         (dict(d=20), 2, "head_dim"),
         (dict(block=16), 2, "block"),
+        (dict(sk=2**31 - 1), 2, "key rows"),
+        (dict(sq=2**26 + 1), 2, "rows"),
         (dict(topk=0), 2, "topk"),
         (dict(topk=65), 2, "topk"),
         (dict(scale=float("inf")), 1, "scale"),

@@ -699,6 +699,11 @@ def test_python_refusals_on_the_gpu():
         lambda: ops.qk_norm_rotary(x, x, torch.ones(16, device=DEV), torch.ones(16, device=DEV, dtype=F16)),
         lambda: ops.qk_norm_rotary(x, x, None, None, eps=-1.0),
         lambda: ops.block_means(x, 0),
+        lambda: ops.block_means(x, 2**32 + 64),  # a size that would wrap into another
+        lambda: ops.block_select(x, torch.zeros(1, 2, 1, 16, device=DEV), 4, 2**32 + 64, 20),
+        lambda: ops.block_select(x, torch.zeros(1, 2, 1, 16, device=DEV), 4, 64, 20, keep_first=2**32 + 1),
+        lambda: ops.block_attention(x, x, x, index, 2**32 + 64),
+        lambda: ops.block_means(x[:, :, :1].expand(1, 2, 2**31 + 20, 16), 64),
     ]
     for call in bad:
         with pytest.raises((ValueError, RuntimeError)):
