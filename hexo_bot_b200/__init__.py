@@ -6,6 +6,8 @@ sm_100a kernels behind a C ABI (include/shrimp_b200.h). Public API:
 - ShrimpNet (hexo_bot_b200.model): the reference module tree; forward_policy_value
   runs natively on CUDA tensors.
 - ShrimpEvaluator (hexo_bot_b200.evaluator): the serve-side wire-ABI evaluator.
+- attention_ops: rotary positions, query / key norm and block-sparse attention
+  for long supports, with gradients.
 - featurize / positions: host-side input builders.
 """
 
