@@ -168,7 +168,10 @@ void put(RotArgs* a, int slot, const sb_heads* x, const sb_heads* dy, const sb_h
 }
 
 // ---- block selection ----------------------------------------------------------
-constexpr int kSelFewRows = 8;  // up to so many queries of a sequence take the few-query kernel
+// Up to so many queries of a sequence take the few-query kernel (few / many, us,
+// 8 heads of 64 over 128 blocks: 6 / 13 at 2 rows, 7 / 14 at 8, 11 / 14 at 16,
+// 14 / 23 at 32; 8 x 8 heads of 128: 14 / 26, 17 / 34, 32 / 35, 47 / 37).
+constexpr int kSelFewRows = 16;
 
 template <typename T, int PER, int LPR>
 int launch_select_per(const SelArgs& a, unsigned grid, cudaStream_t st) {
@@ -182,7 +185,7 @@ int launch_select(const SelArgs& a, unsigned grid, cudaStream_t st) {
   if (a.nb <= 40) return launch_select_per<T, 20, 2>(a, grid, st);
   if (a.nb <= 64) return launch_select_per<T, 32, 2>(a, grid, st);
   if (a.nb <= 128) return launch_select_per<T, 32, 4>(a, grid, st);
-  return launch_select_per<T, 0, 32>(a, grid, st);
+  return launch_select_per<T, 0, 8>(a, grid, st);
 }
 template <typename T, int PER>
 int launch_select_few_per(const SelArgs& a, unsigned rows, int cluster, cudaStream_t st) {
@@ -215,7 +218,10 @@ int launch_select_few(const SelArgs& a, unsigned rows, int cluster, cudaStream_t
 // 8192 rows, 8 heads of 64, 16 of 128 blocks, forward: 335 us with windows of
 // 64 MB, 278 with 100, 255 with 200, 234 with one of 277 MB.
 constexpr long long kBaWindowBytes = 1ll << 30;
-constexpr int kBaFewRows = 16;      // up to so many queries take the few-query kernel
+// Up to so many queries take the few-query kernel (few / many, us, 8 heads of 64,
+// 16 blocks: 8 / 19 at 2 rows, 10 / 21 at 16, 20 / 21 at 32, 39 / 21 at 64; 8 x 8
+// groups of 4 heads of 128: 17 / 99 at 2, 116 / 143 at 16, 230 / 163 at 32).
+constexpr int kBaFewRows = 16;
 // Work items an SM and window, and the listed rows that an item may hold: fewer
 // items leave SMs idle behind popular blocks (8192 rows, 8 heads of 64, 16 of 128
 // blocks, forward: 211 us with 8 an SM, 201 with 16 to 32; backward, where every

@@ -7,16 +7,16 @@
 //
 // Neighbouring queries choose different blocks, so a tile of queries shares no
 // key block and a query alone fills one row of a matrix instruction. The work
-// is turned round: a CTA owns one key block (in shared memory) and a segment
-// of the queries, lists the queries that chose the block, and runs them 16
-// rows at a time through mma.sync. Each (query, block) pair leaves a partial
+// is turned round: a work item is one key block (in shared memory) and a segment
+// of the queries; its CTA lists the queries that chose the block and runs them in
+// tiles of 128 rows through the tensor cores. Each (query, block) pair leaves a partial
 // result (max, sum and unnormalised output row in fp32) at the place of the
 // block in the query's list; a second kernel joins a row's parts. Nothing is
 // added up in an order that varies: results are the same from run to run.
 //
 // A part is written and read once: 8 D bytes a pair against 4 D block flops,
-// which at D = 64 and block 64 is as long at HBM's rate as the products at that
-// of mma.sync.
+// five times as long at HBM's rate as the products at the tensor cores' (D = 64,
+// block 64): the parts and the chain of a tile's steps bound the kernels.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -47,7 +47,7 @@ struct BaArgs {
   const int* q_lens;
   uint16_t* entries;      // (B Hkv, marks, kBaMark topk): per group, by block: place in the row's list << 8 | query
   uint32_t* spans;        // (B Hkv, nb, marks): first entry of the group's queries that chose the block | count << 16
-  uint32_t* ticket;       // work items of the forward's CTAs that have been taken; 0 before each launch
+  uint32_t* ticket;       // work items that the persistent CTAs have taken; 0 before each launch
   unsigned long long* slots;  // (B Hkv, Sq): bit s = entry s of the row's list counts
   float* part;            // window's parts: [row][topk][dim], row = (local bh * wq + local i) * group + g
   float2* ml;             // forward: [row][topk] (max in log2 units, sum)

@@ -744,13 +744,13 @@ __global__ __launch_bounds__(kSelThreads, 3) void block_select_kernel(const SelA
     const float q = sqrtf(qn[r]);
     return unit * q + 1e-34f * (mmax + q) + 1e-40f;
   };
-  if (PER > 0) {
+  if constexpr (PER > 0) {
     for (int r0 = warp * (32 / LPR); r0 < nl; r0 += kSelThreads / LPR) {
       const int r = r0 + lane / LPR;
       const bool on = r < nl;
       const int rr = on ? r : 0;
       const SelRow row(a, i0 + rr, live);
-      const bool done = sel_rows<PER ? PER : 1, LPR>(sc + rr * NBS, row, err_of(rr), on, out + (long long)rr * a.topk);
+      const bool done = sel_rows<PER, LPR>(sc + rr * NBS, row, err_of(rr), on, out + (long long)rr * a.topk);
       if (on && !done && lane % LPR == 0) todo[atomicAdd(&todo_n, 1)] = r;
     }
     __syncthreads();

@@ -285,6 +285,9 @@ SELECT = [
     (2, 2, 1, 1, 5000, 256, 64, 2, 1, True, None, None),
     (1, 2, 2, 300, 300, 16, 64, 1, 0, True, None, None),  # the forced block alone
     (1, 1, 1, 2, 40000, 16, 4, 24, 0, False, None, None),  # 10000 blocks
+    (1, 4, 2, 21, 9000, 33, 8, 64, 1, True, (8999,), (20,)),  # many blocks, many queries
+    (1, 1, 1, 19, 35000, 16, 4, 24, 0, False, None, None),
+    (1, 2, 1, 150, 7000, 24, 64, 12, 0, False, None, None),  # 110 blocks
 ]
 
 
