@@ -629,6 +629,25 @@ def test_backward_functions_captured_beside_an_eager_graph():
     replay_and_compare(graphs, results, leaves, (ins, chain_inputs(seed=78)), step)
 
 
+def test_single_tokens_captured_beside_one_another():
+    """The serving form (means kept, one query row) captured twice, replayed at once on new inputs."""
+    g = gen(79)
+    k, v = (randn(g, 2, 2, 900, 64, dtype=BF16) for _ in range(2))
+    lens = torch.tensor([900, 333], dtype=torch.int32, device=DEV)
+    means = ops.block_means(k, 64, kv_lens=lens)
+    q = randn(g, 2, 8, 1, 64, dtype=BF16)
+
+    def step():
+        index = ops.block_select(q, means, 5, 64, 900, kv_lens=lens, keep_first=1)
+        return (index, *ops.block_attention(q, k, v, index, 64, kv_lens=lens))
+
+    graphs, results = capture_twice(step)
+    sources = [(q.clone(),), (randn(g, 2, 8, 1, 64, dtype=BF16),)]
+    replay_and_compare(graphs, results, (q,), sources, step)
+    found, bound = O.attention(q, k, v, results[0][0], 64, None, lens)
+    within(results[0][1], found["out"], bound["out"])
+
+
 def test_rows_past_two_to_the_32():
     """Strides that pass 32 bits: a cache whose rows lie 2^27 elements apart."""
     rows, d, step = 40, 16, 2**27
