@@ -267,6 +267,19 @@ __device__ __forceinline__ float ba_exp2(float x) {  // 2^x, relative error 2^-2
   return y;
 }
 
+// What rounding two values to the packed 16-bit pair `hi` left of them, packed
+// the same way: hi + rest holds a value to u^2 (u one rounding of the type).
+template <typename T>
+__device__ __forceinline__ float2 ba_unpack(uint32_t v) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t ba_rest(float a, float b, uint32_t hi) {
+  const float2 h = ba_unpack<T>(hi);
+  return MmaTraits<T>::pack(a - h.x, b - h.y);
+}
+
 __device__ __forceinline__ int ba_div_group(const BaArgs& a, int x) {
   return a.group_magic ? (int)__umulhi((uint32_t)x, a.group_magic) : x;
 }
@@ -346,19 +359,24 @@ struct BaTile {
     for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    // weights go to the matrix unit in the inputs' 16-bit type (half a step of
-    // rounding each, averaged over the keys); their sum l stays in 32 bits
+    // weights go to the matrix unit as pairs of the inputs' 16-bit type, so that
+    // the result is rounded once; their sum l is one of 32-bit weights
 #pragma unroll
     for (int kk = 0; kk < BK / 16; ++kk) {
-      const uint32_t fa[4] = {MmaTraits<T>::pack(s[2 * kk][0], s[2 * kk][1]),
-                              MmaTraits<T>::pack(s[2 * kk][2], s[2 * kk][3]),
-                              MmaTraits<T>::pack(s[2 * kk + 1][0], s[2 * kk + 1][1]),
-                              MmaTraits<T>::pack(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+      uint32_t fa[4], fr[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float* w = &s[2 * kk + (x >> 1)][2 * (x & 1)];
+        fa[x] = MmaTraits<T>::pack(w[0], w[1]);
+        fr[x] = ba_rest<T>(w[0], w[1], fa[x]);
+      }
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) {
         uint32_t fb[4];
         ldmatrix_x4_trans(fb, ba_at<DP>(v, 16 * kk + (lane & 15), 2 * n + (lane >> 4)));
         const uint32_t b0[2] = {fb[0], fb[1]}, b1[2] = {fb[2], fb[3]};
+        MmaTraits<T>::mma(o[2 * n], fr, b0);
+        MmaTraits<T>::mma(o[2 * n + 1], fr, b1);
         MmaTraits<T>::mma(o[2 * n], fa, b0);
         MmaTraits<T>::mma(o[2 * n + 1], fa, b1);
       }
@@ -369,8 +387,8 @@ struct BaTile {
 // ---- forward, many queries -----------------------------------------------------
 // Tiles of 128 listed rows on the fifth-generation tensor cores, one row a
 // thread: S = Q K^T into TMEM; each thread reads its row of S, takes maximum,
-// exponentials and sum without any exchange and writes the 16-bit weights back
-// over S; O = P V with P as the TMEM operand; O leaves through the tile's own Q
+// exponentials and sum without any exchange and writes the weights back over S as
+// pairs of 16-bit numbers; O = P V with P as the TMEM operand; O leaves through the tile's own Q
 // buffer (transposed there, so that a part goes out in whole 128-byte lines).
 // Four CTAs an SM (128 TMEM columns each at D = 64) cover one another's waits.
 // An mma.sync form of this kernel, 16 rows a warp, took 134 us where this one
@@ -595,19 +613,28 @@ __global__ __launch_bounds__(kBaFwdThreads, ba_fwd_ctas<DP, BK>()) void block_at
 #pragma unroll
         for (int c0 = 0; c0 < BK; c0 += SH) {
           if (BK > SH) load_s(c0);
-          // weights go to the matrix unit in the inputs' 16-bit type (half a step of
-          // rounding each, averaged over the keys); their sum l stays in 32 bits
+          // weights go to the matrix unit as pairs of the inputs' 16-bit type, so that
+          // the result is rounded once (what rounding leaves of SH scores lies in the
+          // columns behind their weights); their sum l is one of 32-bit weights
           float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < SH; c += 32) {
             uint32_t w[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-              const float p0 = ba_exp2(fmaf(s[c + 2 * x], sc, -ref)), p1 = ba_exp2(fmaf(s[c + 2 * x + 1], sc, -ref));
+              float &p0 = s[c + 2 * x], &p1 = s[c + 2 * x + 1];
+              p0 = ba_exp2(fmaf(p0, sc, -ref));
+              p1 = ba_exp2(fmaf(p1, sc, -ref));
               l4[x & 3] += p0 + p1;
               w[x] = MmaTraits<T>::pack(p0, p1);
+              const float2 h = ba_unpack<T>(w[x]);
+              p0 -= h.x;
+              p1 -= h.y;
             }
-            ba_tmem_st16(s_tm + lanes + (c0 + c) / 2, w);
+            ba_tmem_st16(s_tm + lanes + c0 + c / 2, w);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) w[x] = MmaTraits<T>::pack(s[c + 2 * x], s[c + 2 * x + 1]);
+            ba_tmem_st16(s_tm + lanes + c0 + (SH + c) / 2, w);
           }
           l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         }
@@ -618,8 +645,11 @@ __global__ __launch_bounds__(kBaFwdThreads, ba_fwd_ctas<DP, BK>()) void block_at
           tc_fence_after();
           constexpr uint32_t id = mma_idesc(DP, BF) | kIdescBMn;
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            tc_mma_f16_ts(o_tm, s_tm + kk * 8, ba_mn_desc(vs + kk * 2048, BK * 128), id, kk > 0);
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const uint32_t w = s_tm + kk * 16 / SH * SH + kk * 16 % SH / 2;
+            tc_mma_f16_ts(o_tm, w + SH / 2, ba_mn_desc(vs + kk * 2048, BK * 128), id, kk > 0);
+            tc_mma_f16_ts(o_tm, w, ba_mn_desc(vs + kk * 2048, BK * 128), id, 1);
+          }
           tc_commit(bar_o);
         }
         // where this row's part goes (a window's parts number less than 2^31)

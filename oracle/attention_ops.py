@@ -90,19 +90,27 @@ def seen_keys(index, sk, block, kv_lens=None, q_lens=None):
     return seen
 
 
-def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout=None):
+def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout=None, pair=False):
     """Results in 64 bits and, beside each, a bound on the kernels' error.
 
     u = one rounding to the inputs' type. The kernels round the weights p and, backward, ds to it
     (relative u each; in f16 also 2^-25 absolute, its subnormal step) and every result once more.
     Scores are 32-bit dot products: |error of s| <= es = (D + 4) 2^-24 scale sum |q||k| and a
     32-bit exp with the same order of error, which scales p by 1 +- 2 es + 2^-20. The backward's
-    delta = do . out reads the rounded out."""
+    delta = do . out reads the rounded out.
+
+    `pair`: the bound for weights that go to the matrix unit as pairs of 16-bit numbers, hi and the
+    rest of it. They are off by u^2 (u for hi, u of what it leaves for the rest). What was
+    drowned by u counts then: matrix steps of 16 keys add in 32 bits with an error of 2^-23 of the
+    sum of magnitudes each (two products a step, 16 steps at most), the join of up to 64 parts
+    with 2^-24 each and two roundings of every part's weight: 2^-17 in all."""
 
     b, hq, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
     grp = hq // hk
     u = torch.finfo(q.dtype).eps / 2
+    if pair:
+        u = u * u + 2.0**-17
     sub = 2.0**-25 if q.dtype == torch.float16 else 0.0
     scale = 1 / math.sqrt(d) if scale is None else scale
     seen = seen_keys(index, sk, block, kv_lens, q_lens)[:, :, None]
