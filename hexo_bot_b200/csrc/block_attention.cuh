@@ -995,36 +995,31 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
 // chose it, tiles of 128 listed rows, a row a thread. Five products a tile on the
 // tensor cores, all from shared memory:
 //   S = Q K^T, dP = dO V^T                     128 rows x BK keys, into TMEM
-//   p = 2^(S - lse), ds = p (dP - delta)       by the row's thread, to 16 bits
+//   p = 2^(S - lse), ds = p (dP - delta)       by the row's thread, to pairs of 16 bits
 //   [dV; .] += [P | dS]^T dO, [.; dK] += [P | dS]^T Q   over the item's tiles, in TMEM
 //   dQ = dS K                                  128 rows, a part of each pair
 // P and dS are written [row][key] and read as M-major operands; for blocks of up
 // to 64 keys both go through one 128-row operand (half of each result is not
-// used), for 128 keys each is one. dQ lies over S and dP, which are done with.
+// used), for 128 keys each is one. Both are pairs (what rounding leaves of a
+// 16-bit number is another one), so that each gradient is rounded once; with single
+// ones dv and dk were off by 1.4 times that, dq by 1.5 to 1.7. There is no room in
+// shared memory for the second halves: they wait in TMEM over dP, from where dQ takes
+// them as its left operand, and take the first ones' place for dV and dK once those
+// are done. dQ lies over S, which is done with.
 // An mma.sync form, 64 rows a tile, took 310 us where this one takes about 260 (8192
 // rows, 8 heads of 64, 16 of 128 blocks).
 constexpr int kBaBwdThreads = 128;
 
 template <int DP, int BK>
 constexpr int ba_bwd_tmem() {
-  constexpr int n = (2 * BK > DP ? 2 * BK : DP) + 2 * DP;
+  constexpr int n = BK + (BK > DP ? BK : DP) + 2 * DP;
   return n <= 128 ? 128 : n <= 256 ? 256 : 512;
-}
-// dq = dS K takes ds as a pair of 16-bit numbers. Its error from ds's rounding and
-// from that of the out which delta reads comes on top of its own rounding: 1.5 to
-// 1.7 times that in all with single ds (head_dim 16, or few keys a row), 1.1 to 1.3
-// with the pair; dk and dv, whose errors are independent over the rows, stay at 1.4
-// without. Heads of more than 64 channels with blocks of 128 have no shared memory
-// for it.
-template <int DP, int BK>
-constexpr bool ba_bwd_pair() {
-  return DP <= 64 || BK <= 64;
 }
 template <int DP, int BK>
 constexpr int ba_bwd_smem() {
   constexpr int keys = BK > 64 ? 2 : 1;  // 64-key panels of P and dS
   constexpr int need = 1024 + ba_panels(DP) * (2 * BK + 2 * kBaFwdRows) * 128 +
-                       (ba_bwd_pair<DP, BK>() ? 3 : 2) * keys * kBaFwdRows * 128 + kBaChunk * 4 + kBaFwdRows * 20;
+                       (2 * keys + 1) * kBaFwdRows * 128 + kBaChunk * 4 + kBaFwdRows * 20;
   constexpr int least = 232448 / (512 / ba_bwd_tmem<DP, BK>() + 1) + 1;
   return need > least ? need : least;
 }
@@ -1039,23 +1034,22 @@ template <typename T, int DP, int BK>
 __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_attn_bwd_kernel(const BaArgs a) {
   constexpr int PAN = ba_panels(DP), CH = DP / 8, ROWS = kBaFwdRows, PK = BK > 64 ? 2 : 1;
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  constexpr bool PAIR = ba_bwd_pair<DP, BK>();
   constexpr uint32_t KB = PAN * BK * 128, QB = PAN * ROWS * 128, PB = PK * ROWS * 128;
   constexpr int OW = DP < 32 ? DP : 32;  // channels staged at a time
   extern __shared__ char ba_smem_raw[];
   char* ba_smem = ba_smem_raw + (1024 - (smem_u32(ba_smem_raw) & 1023)) % 1024;
   const uint32_t ks = smem_u32(ba_smem), vs = ks + KB, qs = vs + KB, gs = qs + QB, ps = gs + QB, dss = ps + PB,
-                 dls = dss + PB;  // P, dS, and what dS's rounding left
-  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB + (PAIR ? 3 : 2) * PB);
+                 stages = dss + PB;  // P, dS, and the rows of dq on their way out
+  uint32_t* list = reinterpret_cast<uint32_t*>(ba_smem + 2 * KB + 2 * QB + 2 * PB + ROWS * 128);
   long long* qoff = reinterpret_cast<long long*>(list + kBaChunk);  // [128] rows of the tile being loaded: q
   long long* goff = qoff + ROWS;                                     // [128] and dout
   int* dst = reinterpret_cast<int*>(goff + ROWS);                    // [128]: parts of the tile being stored
-  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ __align__(8) uint64_t bars[3];
   __shared__ uint32_t tmem_slot, next_item;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t items = (uint32_t)a.nbh * (uint32_t)a.nb * (uint32_t)a.nseg;
   const int G = a.group;
-  const uint32_t bar_s = smem_u32(&bars[0]), bar_o = smem_u32(&bars[1]);
+  const uint32_t bar_s = smem_u32(&bars[0]), bar_o = smem_u32(&bars[1]), bar_r = smem_u32(&bars[2]);
   if (warp == 0) {
     tmem_alloc(smem_u32(&tmem_slot), ba_bwd_tmem<DP, BK>());
     tmem_relinquish();
@@ -1063,14 +1057,16 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
   if (tid == 0) {
     mbar_init(bar_s, 1);
     mbar_init(bar_o, 1);
+    mbar_init(bar_r, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot, lanes = (uint32_t)(warp * 32) << 16;
-  const uint32_t s_tm = tmem, dp_tm = tmem + BK, dq_tm = tmem;
-  const uint32_t dv_tm = tmem + (2 * BK > DP ? 2 * BK : DP), dk_tm = dv_tm + DP;
+  // dP and, 32 keys a piece, the rests of P and of dS (16 columns each); S and dQ
+  const uint32_t dp_tm = tmem, s_tm = tmem + BK, dq_tm = s_tm;
+  const uint32_t dv_tm = s_tm + (BK > DP ? BK : DP), dk_tm = dv_tm + DP;
   bool ok = true;
   uint32_t phase = 0;
   for (uint32_t u = blockIdx.x; u < items;) {
@@ -1129,6 +1125,17 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
         }
         __syncwarp();
       };
+      // [P | dS]: the panel after P's first is dS for up to 64 keys, P's second for 128
+      auto products = [&](bool add) {
+        constexpr uint32_t id = mma_idesc(DP, BF) | kIdescAMn | kIdescBMn;
+#pragma unroll
+        for (int kk = 0; kk < ROWS / 16; ++kk)
+          tc_mma_f16(dv_tm, ba_mn_desc(ps + kk * 2048, ROWS * 128), ba_mn_desc(gs + kk * 2048, ROWS * 128), id, add || kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < ROWS / 16; ++kk)
+          tc_mma_f16(dk_tm, ba_mn_desc((BK > 64 ? dss : ps) + kk * 2048, ROWS * 128), ba_mn_desc(qs + kk * 2048, ROWS * 128),
+                     id, add || kk > 0);
+      };
       load_tile(0);
       for (int t = 0; t < tiles; ++t) {
         // a row all of whose scores are -inf has no weights
@@ -1153,8 +1160,6 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
         }
         ok = ok && mbar_wait(bar_s, phase);
         tc_fence_after();
-        // p and ds are rounded to the inputs' type for the matrix unit (as the
-        // forward rounds p); their products are added in 32 bits
 #pragma unroll
         for (int c0 = 0; c0 < BK; c0 += 32) {
           float s[32], dp[32];
@@ -1170,32 +1175,60 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
             for (int x = 0; x < 32; ++x)
               if (c0 + x >= have) s[x] = dp[x] = 0.f;
           }
+          uint32_t rp[16], rd[16];
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            uint32_t wp[4], wd[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int i = x + 2 * y;
+              wp[y] = MmaTraits<T>::pack(s[i], s[i + 1]);
+              rp[x / 2 + y] = ba_rest<T>(s[i], s[i + 1], wp[y]);
+              wd[y] = MmaTraits<T>::pack(dp[i], dp[i + 1]);
+              // past the type's range wd is infinite, and the product says so
+              const float2 h = ba_unpack<T>(wd[y]);
+              rd[x / 2 + y] = MmaTraits<T>::pack(isinf(h.x) ? 0.f : dp[i] - h.x, isinf(h.y) ? 0.f : dp[i + 1] - h.y);
+            }
+            const uint32_t to = ba_panel_at(0, ROWS, tid, (c0 + x) / 8);
+            sts128(ps + to, wp);
+            sts128(dss + to, wd);
+          }
+          ba_tmem_st16(dp_tm + lanes + c0, rp);
+          ba_tmem_st16(dp_tm + lanes + c0 + 16, rd);
+        }
+        tmem_wait_st();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          constexpr uint32_t id_q = mma_idesc(DP, BF) | kIdescBMn;
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            tc_mma_f16(dq_tm, sw128_desc(dss + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
+                       kk > 0);
+            tc_mma_f16_ts(dq_tm, dp_tm + kk / 2 * 32 + 16 + kk % 2 * 8, ba_mn_desc(ks + kk * 2048, BK * 128), id_q, 1);
+          }
+          products(any);
+          tc_commit(bar_o);
+        }
+        any = true;
+        ok = ok && mbar_wait(bar_o, phase);
+        tc_fence_after();
+        // the rests take the place of P and dS
+#pragma unroll
+        for (int c0 = 0; c0 < BK; c0 += 32) {
+          float r[32];
+          ba_tmem_ld<32>(dp_tm + lanes + c0, r);
 #pragma unroll
           for (int x = 0; x < 32; x += 8) {
             const uint32_t to = ba_panel_at(0, ROWS, tid, (c0 + x) / 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(ps + to), "r"(MmaTraits<T>::pack(s[x], s[x + 1])),
-                         "r"(MmaTraits<T>::pack(s[x + 2], s[x + 3])), "r"(MmaTraits<T>::pack(s[x + 4], s[x + 5])),
-                         "r"(MmaTraits<T>::pack(s[x + 6], s[x + 7]))
-                         : "memory");
-            uint32_t hi[4];
+            uint32_t w[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) hi[y] = MmaTraits<T>::pack(dp[x + 2 * y], dp[x + 2 * y + 1]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dss + to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),
-                         "r"(hi[3])
-                         : "memory");
-            if (PAIR) {
-              uint32_t lo[4];
+            for (int z = 0; z < 2; ++z) {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                float2 h;
-                if constexpr (BF) h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi[y]));
-                else h = __half22float2(*reinterpret_cast<const __half2*>(&hi[y]));
-                // past the type's range hi is infinite, and the product says so
-                lo[y] = MmaTraits<T>::pack(isinf(h.x) ? 0.f : dp[x + 2 * y] - h.x, isinf(h.y) ? 0.f : dp[x + 2 * y + 1] - h.y);
-              }
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dls + to), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]),
-                           "r"(lo[3])
-                           : "memory");
+              for (int y = 0; y < 4; ++y) w[y] = __float_as_uint(r[16 * z + x / 2 + y]);
+              sts128((z ? dss : ps) + to, w);
             }
           }
         }
@@ -1204,33 +1237,11 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
         __syncthreads();
         if (tid == 0) {
           tc_fence_after();
-          constexpr uint32_t id_kv = mma_idesc(DP, BF) | kIdescAMn | kIdescBMn, id_q = mma_idesc(DP, BF) | kIdescBMn;
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            tc_mma_f16(dq_tm, sw128_desc(dss + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
-                       kk > 0);
-            if (PAIR)
-              tc_mma_f16(dq_tm, sw128_desc(dls + kk / 4 * ROWS * 128 + kk % 4 * 32), ba_mn_desc(ks + kk * 2048, BK * 128), id_q,
-                         1);
-          }
-          // [P | dS]: the panel after P's first is dS for up to 64 keys, P's second for 128
-#pragma unroll
-          for (int kk = 0; kk < ROWS / 16; ++kk)
-            tc_mma_f16(dv_tm, ba_mn_desc(ps + kk * 2048, ROWS * 128), ba_mn_desc(gs + kk * 2048, ROWS * 128), id_kv,
-                       any || kk > 0);
-#pragma unroll
-          for (int kk = 0; kk < ROWS / 16; ++kk)
-            tc_mma_f16(dk_tm, ba_mn_desc((BK > 64 ? dss : ps) + kk * 2048, ROWS * 128), ba_mn_desc(qs + kk * 2048, ROWS * 128),
-                       id_kv, any || kk > 0);
-          tc_commit(bar_o);
+          products(true);
+          tc_commit(bar_r);
         }
-        any = true;
-        ok = ok && mbar_wait(bar_o, phase);
-        phase ^= 1;
-        tc_fence_after();
-        if (t + 1 < tiles) load_tile(t + 1);
-        // dq to its parts: a warp's 32 rows through P's bytes, which are done with
-        const uint32_t stage = ps + warp * 32 * 128;
+        // dq to its parts, a warp's 32 rows at a time through its stage
+        const uint32_t stage = stages + warp * 32 * 128;
 #pragma unroll
         for (int c0 = 0; c0 < DP; c0 += OW) {
           float o[OW];
@@ -1252,7 +1263,13 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
             if (to >= 0 && c0 + c * 4 < a.dim)
               *reinterpret_cast<uint4*>(a.part + (long long)to * a.dim + c0 + c * 4) = v;
           }
+          if (c0 == 0) {  // q and dout are done with: the next rows load under the other channels
+            ok = ok && mbar_wait(bar_r, phase);
+            tc_fence_after();
+            if (t + 1 < tiles) load_tile(t + 1);
+          }
         }
+        phase ^= 1;
         __syncwarp();  // dst is written over by the next tile
       }
     }

@@ -103,14 +103,17 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
     rest of it. They are off by u^2 (u for hi, u of what it leaves for the rest). What was
     drowned by u counts then: matrix steps of 16 keys add in 32 bits with an error of 2^-23 of the
     sum of magnitudes each (two products a step, 16 steps at most), the join of up to 64 parts
-    with 2^-24 each and two roundings of every part's weight: 2^-17 in all."""
+    with 2^-24 each and two roundings of every part's weight: 2^-17 in all. The sums of dk and dv
+    over the rows take a step per 16 rows."""
 
     b, hq, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
     grp = hq // hk
     u = torch.finfo(q.dtype).eps / 2
+    steps = 0.0
     if pair:
         u = u * u + 2.0**-17
+        steps = 2.0**-22 * (sq * grp / 16 + 8)
     sub = 2.0**-25 if q.dtype == torch.float16 else 0.0
     scale = 1 / math.sqrt(d) if scale is None else scale
     seen = seen_keys(index, sk, block, kv_lens, q_lens)[:, :, None]
@@ -136,7 +139,8 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
     if dout is not None:
         g = torch.where(seen.any(-1)[..., None], dout.double().view(b, hk, grp, sq, d), 0.0)
         found["dv"] = (p.transpose(-1, -2) @ g).sum(2)
-        bound["dv"] = rounding(found["dv"], q.dtype) + (((u + rel_p) * p + sub * seen).transpose(-1, -2) @ g.abs()).sum(2)
+        bound["dv"] = rounding(found["dv"], q.dtype) + (
+            ((u + steps + rel_p) * p + sub * seen).transpose(-1, -2) @ g.abs()).sum(2)
         dp = g @ v64.transpose(-1, -2)
         delta = (g * out).sum(-1, keepdim=True)
         ds = p * (dp - delta)
@@ -146,6 +150,7 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
         found["dq"] = scale * (ds @ k64)
         found["dk"] = scale * (ds.transpose(-1, -2) @ q64).sum(2)
         bound["dq"] = rounding(found["dq"], q.dtype) + abs(scale) * (e_ds @ k64.abs())
+        e_ds = e_ds + steps * ds.abs()
         bound["dk"] = rounding(found["dk"], q.dtype) + abs(scale) * (e_ds.transpose(-1, -2) @ q64.abs()).sum(2)
     for name in ("out", "lse", "dq"):
         for t in (found, bound):

@@ -44,3 +44,15 @@ def test_block_attention_output_is_rounded_once(case, dtype):
     found, bound = O.attention(q, k, v, index, block, pair=True)
     within(out, found["out"], bound["out"], "out")
     within(lse, found["lse"], bound["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", SHAPES)
+def test_block_attention_gradients_are_rounded_once(case, dtype):
+    """Softmax weights and score gradients lose nothing that dq, dk and dv could show."""
+    q, k, v, index, block, dout = tensors(case, dtype, 102)
+    out, lse = ops.block_attention(q, k, v, index, block)
+    grads = ops.block_attention_backward(dout, q, k, v, out, lse, index, block)
+    found, bound = O.attention(q, k, v, index, block, dout=dout, pair=True)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        within(got, found[name], bound[name], name)
