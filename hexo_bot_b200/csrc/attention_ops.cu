@@ -280,7 +280,7 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   p.ml = at;
   if (!backward) at += align256((size_t)rows * topk * 8);
   p.delta = at;
-  if (backward) at += align256((size_t)bh * q_rows * group * 4);
+  if (backward) at += align256((size_t)bh * q_rows * group * 8);
   p.kv_part = at;
   if (backward) {
     const long long nseg = ba_segments(q_rows, p.wq, p.seg);
@@ -764,7 +764,7 @@ int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const s
   a.spans = (uint32_t*)(ws + p.spans);
   a.slots = (unsigned long long*)(ws + p.slots);
   a.part = (float*)(ws + p.part);
-  a.delta = (float*)(ws + p.delta);
+  a.delta = (float2*)(ws + p.delta);
   a.kv_part = (float*)(ws + p.kv_part);
   a.ticket = (uint32_t*)(ws + p.ticket);
   a.nseg_all = ba_segments(q_rows, p.wq, p.seg);

@@ -51,7 +51,7 @@ struct BaArgs {
   unsigned long long* slots;  // (B Hkv, Sq): bit s = entry s of the row's list counts
   float* part;            // window's parts: [row][topk][dim], row = (local bh * wq + local i) * group + g
   float2* ml;             // forward: [row][topk] (max in log2 units, sum)
-  float* delta;           // backward: (B Hkv, Sq, group) do . out
+  float2* delta;          // backward: (B Hkv, Sq, group) do . out, and the norm of do (f16 alone reads it)
   float* kv_part;         // backward, more than one segment: [bh][nb][nseg][2][block][dim]
   int batch, kv_heads, group, q_rows, kv_rows, dim, nb, block, topk, marks;
   int bh0, nbh;           // window: first (batch, kv head) pair and their count
@@ -963,7 +963,7 @@ __global__ __launch_bounds__(ba_few_warps<DP, BK>() * 32) void block_attn_few_ke
 }
 
 // ---- backward --------------------------------------------------------------------
-// delta = do . out of every row, 8 channels a lane.
+// delta = do . out of every row and the norm of do, 8 channels a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
   const int chunks = a.dim / 8;
@@ -973,7 +973,7 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
   const long long row = x / lanes;
   const int c = (int)(x - row * lanes);
   const long long rows = (long long)a.batch * a.kv_heads * a.q_rows * a.group;
-  float s = 0.f;
+  float s = 0.f, n = 0.f;
   if (row < rows && c < chunks) {
     const long long iq = row / a.group;
     const int g = (int)(row - iq * a.group);
@@ -984,11 +984,17 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
       const RotVec<T, 8> u = *reinterpret_cast<const RotVec<T, 8>*>((const T*)a.o.p + b * a.o.b + h * a.o.h + i * a.o.s + c * 8);
       const RotVec<T, 8> v = *reinterpret_cast<const RotVec<T, 8>*>((const T*)a.go.p + b * a.go.b + h * a.go.h + i * a.go.s + c * 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += rot_f32(u.v[e]) * rot_f32(v.v[e]);
+      for (int e = 0; e < 8; ++e) {
+        s += rot_f32(u.v[e]) * rot_f32(v.v[e]);
+        n += rot_f32(v.v[e]) * rot_f32(v.v[e]);
+      }
     }
   }
-  for (int m = 1; m < lanes; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-  if (row < rows && c == 0) a.delta[row] = s;
+  for (int m = 1; m < lanes; m <<= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, m);
+    n += __shfl_xor_sync(0xffffffffu, n, m);
+  }
+  if (row < rows && c == 0) a.delta[row] = make_float2(s, sqrtf(n));
 }
 
 // Work items as in the forward: one key block and a segment of the queries that
@@ -1006,6 +1012,13 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
 // shared memory for the second halves: they wait in TMEM over dP, from where dQ takes
 // them as its left operand, and take the first ones' place for dV and dK once those
 // are done. dQ lies over S, which is done with.
+//
+// f16 keeps full precision over 2^-14 to 2^16 only. There P is taken times 2^14 (it
+// is 1 at most), and ds times a power of two that brings its bound
+//   |ds| <= |do| max |v| + |delta|
+// over the tile's rows and the block's keys below 2^15. The power holds for a work
+// item (with two octaves to spare at first); a tile that needs a smaller one
+// has the dk summed so far scaled down. Values down to 2^-39 of the bound are not lost.
 // An mma.sync form, 64 rows a tile, took 310 us where this one takes about 260 (8192
 // rows, 8 heads of 64, 16 of 128 blocks).
 constexpr int kBaBwdThreads = 128;
@@ -1029,6 +1042,8 @@ constexpr int ba_bwd_ctas() {
   return t < m ? t : m;
 }
 constexpr uint32_t kIdescAMn = 1u << 15;  // left operand M-major
+constexpr int kBaPUp = 14;                // f16: P is held times 2^14
+__device__ __forceinline__ float ba_pow2(int e) { return __int_as_float((e + 127) << 23); }  // |e| <= 126
 
 template <typename T, int DP, int BK>
 __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_attn_bwd_kernel(const BaArgs a) {
@@ -1046,6 +1061,8 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
   int* dst = reinterpret_cast<int*>(goff + ROWS);                    // [128]: parts of the tile being stored
   __shared__ __align__(8) uint64_t bars[3];
   __shared__ uint32_t tmem_slot, next_item;
+  __shared__ float row_norm[kBaBwdThreads / 32], row_delta[kBaBwdThreads / 32];  // the warps' largest of a tile
+  __shared__ uint32_t v_bits;  // the largest sum of squares over 8 channels of a value
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t items = (uint32_t)a.nbh * (uint32_t)a.nb * (uint32_t)a.nseg;
   const int G = a.group;
@@ -1079,7 +1096,10 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
     const int have = max(0, min(BK, ba_kv_len(a, b) - j * BK));
     tc_fence_before();
     __syncthreads();  // the item before is done with the keys and with dv, dk
-    if (tid == 0) next_item = gridDim.x + atomicAdd(a.ticket, 1u);
+    if (tid == 0) {
+      next_item = gridDim.x + atomicAdd(a.ticket, 1u);
+      v_bits = 0;
+    }
     if (have == 0) g = end;
     const T* qp = (const T*)a.q.p + b * a.q.b + (long long)h * G * a.q.h;
     const T* gp = (const T*)a.go.p + b * a.go.b + (long long)h * G * a.go.h;
@@ -1088,18 +1108,21 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
       ba_load_panels<T, DP, BK>(vs, (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s, a.v.s, have, a.dim);
     }
     bool any = false;  // dv, dk hold something of this item
+    int ex = 0;        // f16: ds and dk are held times 2^ex
+    float v_norm = 0.f;
     while (g < end) {
       const int n = ba_fill<kBaBwdThreads>(a, bh, j, g, end, list);
       if (n == 0) continue;
       const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
-      float lse = INFINITY, delta = 0.f;  // of this thread's row of the next tile, as loaded
+      float lse = INFINITY;  // of this thread's row of the next tile, as loaded
+      float2 delta = make_float2(0.f, 0.f);
       int at = -1;
       // a warp loads the 32 rows whose offsets its lanes worked out
       auto load_tile = [&](int tile) {
         const int row = tile * ROWS + tid;
         long long off = -1, og = 0;
         lse = INFINITY;  // rows that are not there: weight 0
-        delta = 0.f;
+        delta = make_float2(0.f, 0.f);
         at = -1;
         if (row < rows) {
           const int li = ba_div_group(a, row), gr = row - li * G;
@@ -1139,7 +1162,15 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
       load_tile(0);
       for (int t = 0; t < tiles; ++t) {
         // a row all of whose scores are -inf has no weights
-        const float lse_t = lse == -INFINITY ? INFINITY : lse * kLog2e, delta_t = delta;
+        const float lse_t = lse == -INFINITY ? INFINITY : lse * kLog2e, delta_t = delta.x;
+        if (!BF) {  // rows that hold infinities or NaN pass them on; the others' scale ignores them
+          const uint32_t n = __reduce_max_sync(0xffffffffu, delta.y < INFINITY ? __float_as_uint(delta.y) : 0u);
+          const uint32_t d = __reduce_max_sync(0xffffffffu, fabsf(delta_t) < INFINITY ? __float_as_uint(fabsf(delta_t)) : 0u);
+          if (lane == 0) {
+            row_norm[warp] = __uint_as_float(n);
+            row_delta[warp] = __uint_as_float(d);
+          }
+        }
         dst[tid] = at;
         cp_async_wait_all();
         fence_proxy_async_smem();
@@ -1158,6 +1189,47 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
                        sw128_desc(vs + kk / 4 * BK * 128 + kk % 4 * 32), id, kk > 0);
           tc_commit(bar_s);
         }
+        if (!BF) {
+          if (!any) {
+            uint32_t most = 0;
+            for (int x = tid; x < BK * CH; x += kBaBwdThreads) {
+              const uint4 w = lds128(ba_panel_at(vs, BK, x / CH, x % CH));
+              const float2 f[4] = {ba_unpack<T>(w.x), ba_unpack<T>(w.y), ba_unpack<T>(w.z), ba_unpack<T>(w.w)};
+              float n = 0.f;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) n += f[y].x * f[y].x + f[y].y * f[y].y;
+              if (n < INFINITY) most = max(most, __float_as_uint(n));
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) atomicMax(&v_bits, most);
+            __syncthreads();
+            v_norm = sqrtf((float)CH * __uint_as_float(v_bits));
+          }
+          float n = 0.f, d = 0.f;
+#pragma unroll
+          for (int w = 0; w < kBaBwdThreads / 32; ++w) {
+            n = fmaxf(n, row_norm[w]);
+            d = fmaxf(d, row_delta[w]);
+          }
+          // bound < 2^(b + 1): times 2^(14 - b) it stays below 2^15
+          const int most = 14 - ((int)(__float_as_uint(fmaxf(fmaf(n, v_norm, d), 1e-24f)) >> 23) - 127);
+          if (!any) {
+            ex = most - 2;
+          } else if (ex > most) {
+            const float f = ba_pow2(most - 2 - ex);
+            ex = most - 2;
+#pragma unroll
+            for (int c0 = 0; c0 < DP; c0 += 16) {
+              float o[16];
+              uint32_t w[16];
+              ba_tmem_ld<16>(dk_tm + lanes + c0, o);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) w[x] = __float_as_uint(o[x] * f);
+              ba_tmem_st16(dk_tm + lanes + c0, w);
+            }
+          }
+        }
+        const float p_up = BF ? 0.f : kBaPUp, g = BF ? 1.f : ba_pow2(ex - kBaPUp), ds_down = BF ? 1.f : ba_pow2(-ex);
         ok = ok && mbar_wait(bar_s, phase);
         tc_fence_after();
 #pragma unroll
@@ -1167,8 +1239,8 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
           ba_tmem_ld<32>(dp_tm + lanes + c0, dp);
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
-            s[x] = ba_exp2(fmaf(s[x], a.scale_log2, -lse_t));
-            dp[x] = s[x] * (dp[x] - delta_t);
+            s[x] = ba_exp2(fmaf(s[x], a.scale_log2, p_up - lse_t));
+            dp[x] = s[x] * (BF ? dp[x] - delta_t : fmaf(dp[x], g, -delta_t * g));
           }
           if (c0 + 32 > have) {
 #pragma unroll
@@ -1246,6 +1318,10 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
         for (int c0 = 0; c0 < DP; c0 += OW) {
           float o[OW];
           ba_tmem_ld<OW>(dq_tm + lanes + c0, o);
+          if (!BF) {
+#pragma unroll
+            for (int x = 0; x < OW; ++x) o[x] *= ds_down;
+          }
           if (!ok) o[0] = __int_as_float(0x7fc00000);  // a wait that gave up leaves no number
           __syncwarp();
 #pragma unroll
@@ -1279,7 +1355,8 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
     for (int w = 0; w < (BK > 64 ? 2 : 1); ++w) {
       const bool is_v = BK > 64 ? w == 0 : tid < 64;  // this warp's half: dv or dk
       const int key = BK > 64 ? tid : tid & 63;
-      const float f = !ok ? __int_as_float(0x7fc00000) : is_v ? 1.f : a.scale;  // a wait that gave up leaves no number
+      const float down = BF ? 1.f : ba_pow2(is_v ? -kBaPUp : -ex);
+      const float f = !ok ? __int_as_float(0x7fc00000) : is_v ? down : a.scale * down;  // a wait that gave up leaves no number
 #pragma unroll
       for (int c0 = 0; c0 < DP; c0 += 16) {
         float o[16];
@@ -1297,7 +1374,7 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
                 a.kv_part + ((((long long)bh * a.nb + j) * a.nseg_all + a.seg0 + sg) * 2 * BK + (is_v ? BK : 0) + key) * a.dim +
                 c0 + x);
             // the sum over the segments scales
-            const float one = ok ? 1.f : f;
+            const float one = ok ? down : f;
             p[0] = make_float4(o[x] * one, o[x + 1] * one, o[x + 2] * one, o[x + 3] * one);
             p[1] = make_float4(o[x + 4] * one, o[x + 5] * one, o[x + 6] * one, o[x + 7] * one);
           } else if (j * BK + key < a.kv_rows) {

@@ -104,7 +104,9 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
     drowned by u counts then: matrix steps of 16 keys add in 32 bits with an error of 2^-23 of the
     sum of magnitudes each (two products a step, 16 steps at most), the join of up to 64 parts
     with 2^-24 each and two roundings of every part's weight: 2^-17 in all. The sums of dk and dv
-    over the rows take a step per 16 rows."""
+    over the rows take a step per 16 rows. In f16 the last half step of a pair is 2^-25 of what is
+    held: p times 2^14, and ds times a power of two that leaves at least 2^12 of the bound
+    max |dout| max |v| sqrt(chunks of 8 channels) + max |delta|."""
 
     b, hq, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
@@ -140,13 +142,17 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
         g = torch.where(seen.any(-1)[..., None], dout.double().view(b, hk, grp, sq, d), 0.0)
         found["dv"] = (p.transpose(-1, -2) @ g).sum(2)
         bound["dv"] = rounding(found["dv"], q.dtype) + (
-            ((u + steps + rel_p) * p + sub * seen).transpose(-1, -2) @ g.abs()).sum(2)
+            ((u + steps + rel_p) * p + (2.0**-14 if pair else 1.0) * sub * seen).transpose(-1, -2) @ g.abs()).sum(2)
         dp = g @ v64.transpose(-1, -2)
         delta = (g * out).sum(-1, keepdim=True)
         ds = p * (dp - delta)
         e_delta = (g.abs() * (bound["out"] + rounding(out, q.dtype))).sum(-1, keepdim=True)
         e_dp = (d + 4) * 2.0**-24 * (g.abs() @ v64.abs().transpose(-1, -2))
-        e_ds = (u + rel_p) * ds.abs() + p * (e_delta + e_dp + 2.0**-22 * delta.abs()) + sub * seen
+        floor = sub * seen
+        if pair:
+            most = g.norm(dim=-1).max() * v64.norm(dim=-1).max() * math.ceil(d / 8) ** 0.5 + delta.abs().max()
+            floor = floor * 2.0**-12 * most
+        e_ds = (u + rel_p) * ds.abs() + p * (e_delta + e_dp + 2.0**-22 * delta.abs()) + floor
         found["dq"] = scale * (ds @ k64)
         found["dk"] = scale * (ds.transpose(-1, -2) @ q64).sum(2)
         bound["dq"] = rounding(found["dq"], q.dtype) + abs(scale) * (e_ds @ k64.abs())

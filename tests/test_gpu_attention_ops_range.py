@@ -56,3 +56,61 @@ def test_block_attention_gradients_are_rounded_once(case, dtype):
     found, bound = O.attention(q, k, v, index, block, dout=dout, pair=True)
     for name, got in zip(("dq", "dk", "dv"), grads):
         within(got, found[name], bound[name], name)
+
+
+def gradients_within(q, k, v, index, block, dout, **kw):
+    out, lse = ops.block_attention(q, k, v, index, block, **kw)
+    grads = ops.block_attention_backward(dout, q, k, v, out, lse, index, block, **kw)
+    found, bound = O.attention(q, k, v, index, block, dout=dout, pair=True, **kw)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        within(got, found[name], bound[name], name)
+    return grads
+
+
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-3, 1e-4, 2e-5, 1e-6])
+def test_block_attention_gradients_of_any_size_in_f16(size):
+    """Weights of 1 / 8192 times gradients of any size that f16 holds."""
+    g = gen(103)
+    q, k, v = (randn(g, 1, 1, n, 64, dtype=F16) for n in (80, 8192, 8192))
+    index = torch.arange(64, dtype=torch.int32, device=DEV).expand(1, 1, 80, 64).contiguous()
+    gradients_within(q, k, v, index, 128, randn(g, 1, 1, 80, 64, dtype=F16, scale=size))
+
+
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("rising", [False, True])
+def test_block_attention_gradients_of_mixed_sizes_in_f16(rising, d, block):
+    """Rows whose gradients grow or fall by 2^20 from the first to the last, over many tiles."""
+    g = gen(104)
+    q, dout = (randn(g, 1, 2, 900, d, dtype=torch.float32) for _ in range(2))
+    k, v = (randn(g, 1, 1, 300, d, dtype=F16) for _ in range(2))
+    size = torch.logspace(-12, 8, 900, base=2.0, device=DEV)
+    dout = (dout * (size if rising else size.flip(0))[:, None]).to(F16)
+    index = torch.randint(-1, -(-300 // block), (1, 1, 900, 4), generator=g, device=DEV, dtype=torch.int32)
+    gradients_within(q.to(F16), k, v, index, block, dout)
+
+
+def test_block_attention_large_score_gradients_in_f16():
+    """Score gradients past 65504, whose products with small keys are not."""
+    q = torch.zeros(1, 1, 20, 64, dtype=F16, device=DEV)
+    k, v = (torch.zeros(1, 1, 64, 64, dtype=F16, device=DEV) for _ in range(2))
+    k[:, :, 0, 0], k[:, :, 1, 0] = 0.125, -0.125
+    v[:, :, 0], v[:, :, 1] = 40, -40
+    index = torch.zeros(1, 1, 20, 1, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([2], dtype=torch.int32, device=DEV)
+    grads = gradients_within(q, k, v, index, 64, torch.full_like(q, 1500.0), kv_lens=lens)
+    assert all(t.isfinite().all() for t in grads)
+
+
+def test_block_attention_infinite_gradients_stay_in_their_rows():
+    """A row of dout with an infinity or NaN leaves dq of the other rows as it is."""
+    for dtype in (F16, BF16):
+        q, k, v, index, block, dout = tensors((1, 2, 2, 300, 700, 64, 64, 5), dtype, 105)
+        dout[0, 0, 7, 3], dout[0, 1, 9, 0] = float("inf"), float("nan")
+        out, lse = ops.block_attention(q, k, v, index, block)
+        dq = ops.block_attention_backward(dout, q, k, v, out, lse, index, block)[0]
+        clean = dout.nan_to_num(0.0, 0.0, 0.0)
+        want = ops.block_attention_backward(clean, q, k, v, out, lse, index, block)[0]
+        rows = torch.ones(1, 2, 300, dtype=torch.bool, device=DEV)
+        rows[0, 0, 7] = rows[0, 1, 9] = False
+        assert torch.equal(dq[rows], want[rows]) and not dq[~rows].isfinite().any()
