@@ -313,7 +313,8 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
 #pragma unroll
               for (int e = 0; e < VEC; ++e) ss += u[k][e] * u[k][e] + v[k][e] * v[k][e];
             for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            rstd = rsqrtf(ss * a.inv_dim + a.eps);
+            // a head that is not there has no norm: with eps = 0 its 0 / 0 would reach the weight gradients
+            rstd = live ? rsqrtf(ss * a.inv_dim + a.eps) : 0.f;
 #pragma unroll
             for (int k = 0; k < NI; ++k)
 #pragma unroll

@@ -9,7 +9,7 @@ import torch
 
 from hexo_bot_b200 import attention_ops as ops
 from oracle import attention_ops as O
-from test_gpu_attention_ops import BF16, DEV, F16, gen, randn, within
+from test_gpu_attention_ops import BF16, DEV, F16, F32, gen, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,26 @@ def test_block_attention_infinite_gradients_stay_in_their_rows():
         rows = torch.ones(1, 2, 300, dtype=torch.bool, device=DEV)
         rows[0, 0, 7] = rows[0, 1, 9] = False
         assert torch.equal(dq[rows], want[rows]) and not dq[~rows].isfinite().any()
+
+
+# ---- norm and rotation ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,hq,hk,d", [(BF16, 16, 4, 64), (F16, 3, 1, 16), (F32, 5, 3, 20), (F32, 12, 6, 8)])
+def test_qk_norm_gradients_without_eps(dtype, hq, hk, d):
+    """eps = 0 is allowed where no row is zero: an odd number of tokens and heads that do not fill
+    a warp leave lanes without a row, which must not reach the weight gradients."""
+    g = gen(111)
+    q, k, gq, gk = (randn(g, 1, h, 7, d, dtype=dtype) for h in (hq, hk, hq, hk))
+    w = 1 + randn(g, d, scale=0.2)
+    grads = ops.qk_norm_rotary_backward(gq, gk, q, k, w, w, None, None, (), eps=0.0)
+    for x, gy, dx, dw in zip((q, k), (gq, gk), grads[:2], grads[2:]):
+        x64, w64 = x.double().requires_grad_(), w.double().requires_grad_()
+        want = torch.autograd.grad(O.qk_norm(x64, w64, None, eps=0.0), (x64, w64), gy.double())
+        hat = (x64 * x64.square().mean(-1, keepdim=True).rsqrt()).detach()
+        back = gy.double().abs() * w64.detach().abs()
+        rstd = x64.detach().square().mean(-1, keepdim=True).rsqrt()
+        mass = rstd * (back + hat.abs() * (back * hat.abs()).mean(-1, keepdim=True))
+        within(dx, want[0], O.rounding(want[0], dtype) + (2 * d + 48) * 2.0**-24 * mass, "dx")
+        mass = (gy.double().abs() * hat.abs()).sum((0, 1, 2))
+        within(dw, want[1], O.rounding(want[1], F32) + (d + 96) * 2.0**-24 * mass, "dw")
