@@ -137,3 +137,29 @@ def test_qk_norm_gradients_without_eps(dtype, hq, hk, d):
         within(dx, want[0], O.rounding(want[0], dtype) + (2 * d + 48) * 2.0**-24 * mass, "dx")
         mass = (gy.double().abs() * hat.abs()).sum((0, 1, 2))
         within(dw, want[1], O.rounding(want[1], F32) + (d + 96) * 2.0**-24 * mass, "dw")
+
+
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_without_a_place_keep_infinities_to_themselves(dtype, adjacent):
+    """Rows before the placed ones are not turned: an infinity or NaN there stays in its channel."""
+    x = randn(gen(112), 2, 3, 6, 16, dtype=dtype)
+    x[:, :, 0, 3], x[:, :, 1, 5], x[:, :, 2, 6] = float("inf"), float("-inf"), float("nan")
+    coords = torch.ones(2, 3, 1, dtype=torch.int32, device=DEV)
+    freqs = ops.rotary_freqs((8,), device=DEV)
+    for inverse in (False, True):
+        y = ops.axes_rotary(x, coords, freqs, (8,), adjacent=adjacent, inverse=inverse)
+        assert torch.equal(y[:, :, :3].nan_to_num(5.0), x[:, :, :3].nan_to_num(5.0))
+        assert y[:, :, 3:].isfinite().all()
+    # behind the norm: x / inf is 0 beside NaN at the infinity itself, with and without places
+    turned = ops.qk_norm_rotary(x, x[:, :1], None, None, coords, freqs, (8,), adjacent=adjacent)
+    plain = ops.qk_norm_rotary(x, x[:, :1], None, None)
+    for a, c in zip(turned, plain):
+        assert torch.equal(a[:, :, :3].nan_to_num(5.0), c[:, :, :3].nan_to_num(5.0))
+        assert int(a[:, :, :2].isnan().sum()) == 2 * a.shape[0] * a.shape[1]
+    grads = ops.qk_norm_rotary_backward(x, x[:, :1], x.nan_to_num(1.0, 1.0, 1.0), x[:, :1].nan_to_num(1.0, 1.0, 1.0), None, None,
+                                        coords, freqs, (8,), adjacent=adjacent)
+    want = ops.qk_norm_rotary_backward(x, x[:, :1], x.nan_to_num(1.0, 1.0, 1.0), x[:, :1].nan_to_num(1.0, 1.0, 1.0), None, None,
+                                       None, None, ())
+    for a, c in zip(grads[:2], want[:2]):
+        assert torch.equal(a[:, :, :3].nan_to_num(5.0), c[:, :, :3].nan_to_num(5.0))
