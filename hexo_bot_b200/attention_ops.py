@@ -181,6 +181,7 @@ def axes_rotary(x, coords, freqs, sections, *, adjacent=False, inverse=False, ou
     coords (B, S - prefix, axes): the first `prefix` rows (summary tokens) have no place and stay
     as they are. sections: pairs of each axis; freqs: `rotary_freqs(sections)`. Half pairing joins
     channels (p, P + p) of the P pairs, `adjacent` (2p, 2p + 1); channels from 2P on stay.
+    Coordinates and angles up to 2^53 keep 32-bit accuracy.
     `inverse` turns back. `out` may be x (in place, not under autograd)."""
 
     _first(x, "x")

@@ -13,9 +13,9 @@
 // and sin of its tokens' pairs once, each lane its share, passes them through its
 // own piece of shared memory into registers and uses them for every head; the
 // rows of the first heads are on their way meanwhile, and no warp waits for
-// another. The angle is reduced in 64 bits, so positions of any size keep fp32
-// accuracy. Rows are read once and written once, in 16-byte accesses where shapes
-// and strides allow. Bound by HBM.
+// another. The angle is reduced in pairs of 64-bit numbers, so positions and angles
+// up to 2^53 keep fp32 accuracy. Rows are read once and written once, in 16-byte
+// accesses where shapes and strides allow. Bound by HBM.
 //
 // Channels: half pairing (p, P + p), adjacent pairing (2p, 2p + 1), P pairs in
 // all; channels from 2P on are not turned. Leading `prefix` rows of each
@@ -142,12 +142,18 @@ __device__ __forceinline__ float rot_weight(const void* p, int dtype, int i) {
   }
 }
 
-// cos and sin of an angle in quarter turns, reduced in 64 bits to the nearest one
-// (at most half a quarter off, whatever the position), then the Taylor series of
-// both on [-pi/4, pi/4] (to x^9 and x^8: off by under 3e-8).
-__device__ __forceinline__ float2 rot_cos_sin(double quarters) {
-  const double q = rint(quarters);
-  const float x = (float)(quarters - q) * 1.5707963267948966f, x2 = x * x;
+// 2 / pi as a sum of two 64-bit numbers.
+constexpr double kRotTwoPi = 0.6366197723675814, kRotTwoPiRest = -3.935735335036497e-17;
+
+// cos and sin of coord (f.x + f.y) quarter turns (f.y: what f.x's rounding left),
+// reduced to the nearest one (at most half a quarter off): the product as a pair of
+// 64-bit numbers, whose second part counts as soon as the first one's last bit does;
+// past 2^50 quarters it is itself as large as one. Then the Taylor series of both on
+// [-pi/4, pi/4] (to x^9 and x^8: off by under 3e-8).
+__device__ __forceinline__ float2 rot_cos_sin(double2 f, double coord) {
+  const double p = f.x * coord, r = fma(f.x, coord, -p) + f.y * coord;
+  const double q0 = rint(p), t = (p - q0) + r, q1 = rint(t), q = q0 + q1;
+  const float x = (float)(t - q1) * 1.5707963267948966f, x2 = x * x;
   const float sn = x + x * x2 * (-1.f / 6.f + x2 * (1.f / 120.f + x2 * (-1.f / 5040.f + x2 * (1.f / 362880.f))));
   const float co = 1.f + x2 * (-0.5f + x2 * (1.f / 24.f + x2 * (-1.f / 720.f + x2 * (1.f / 40320.f))));
   const int n = (int)(long long)q;
@@ -166,7 +172,7 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
   constexpr int U = OP == ROT_NORM_BWD || NI > 1 ? 1 : 2;  // heads whose rows a lane has in flight
   constexpr bool BWD = OP == ROT_NORM_BWD;
   __shared__ __align__(16) float2 tables[kRotWarps][32 * VEC * NI];
-  __shared__ double freqs[kRotMaxDim / 2];         // quarter turns per coordinate step
+  __shared__ double2 freqs[kRotMaxDim / 2];        // quarter turns per coordinate step
   __shared__ unsigned char axis[kRotMaxDim / 2];
   __shared__ float weights[2][OP == ROT_TURN ? 1 : kRotMaxDim];
   using V = RotVec<T, VEC>;
@@ -210,7 +216,8 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
     int ax = 0;
     while (p >= a.axis_end[ax]) ++ax;
     axis[p] = (unsigned char)ax;
-    freqs[p] = a.freqs[p] * 0.63661977236758134308;  // 2 / pi
+    const double f = a.freqs[p], q = f * kRotTwoPi;
+    freqs[p] = make_double2(q, fma(f, kRotTwoPi, -q) + f * kRotTwoPiRest);
   }
   if (OP != ROT_TURN)
     for (int i = tid; i < 2 * D; i += kRotThreads)
@@ -276,8 +283,8 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
             const int tt = t - sub + ti, tb = rot_div(tt, a.rows, a.rows_inv, sr);
             float2 c = make_float2(1.f, 0.f);
             if (tt < tokens && sr >= a.prefix) {
-              c = rot_cos_sin(freqs[p] * rot_coord(a.coords, a.coord_dtype,
-                                                   tb * a.cs[0] + (sr - a.prefix) * a.cs[1] + axis[p] * a.cs[2]));
+              c = rot_cos_sin(freqs[p], rot_coord(a.coords, a.coord_dtype,
+                                                  tb * a.cs[0] + (sr - a.prefix) * a.cs[1] + axis[p] * a.cs[2]));
               c.y *= a.sign;
             }
             table[i] = c;

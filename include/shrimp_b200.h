@@ -285,7 +285,9 @@ typedef struct {
 
 /* out = rotated x (inverse != 0: rotated back, which is also the gradient).
  * x, out (B, H, S, D) f32 / f16 / bf16, D <= 256; out may be x. Angles are
- * reduced in 64 bits, the rotation is computed in 32 and rounded once. */
+ * reduced in pairs of 64-bit numbers: coordinates and angles (in radians) up to
+ * 2^53 keep 32-bit accuracy. The rotation is computed in 32 bits and
+ * rounded once. */
 int sb_axes_rotary(const sb_heads* x, int dtype, const sb_rotary* rotary, int inverse, int batch, int heads, int rows,
                    int head_dim, const sb_heads* out, void* stream);
 /* RMS norm of every query and key head, times a weight per channel, then the

@@ -4,6 +4,9 @@ little the results lose, values of every size, sizes past one window. Against
 
 from __future__ import annotations
 
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -163,3 +166,27 @@ def test_rows_without_a_place_keep_infinities_to_themselves(dtype, adjacent):
                                        None, None, ())
     for a, c in zip(grads[:2], want[:2]):
         assert torch.equal(a[:, :, :3].nan_to_num(5.0), c[:, :, :3].nan_to_num(5.0))
+
+
+PI = Fraction(31415926535897932384626433832795028841971693993751058209749445923, 10**64)
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32, F32])
+@pytest.mark.parametrize("size", [2**20, 2**28, 2**31 - 1, 10**12, 1_700_000_000_000, 1_700_000_000_000_000, 2**52, 2**53])
+def test_coordinates_of_any_size(size, kind):
+    """cos and sin of far positions against exact arithmetic. One turn of (1, 0): the kernel's
+    reduced angle is a float of at most pi / 4 (three roundings of 2^-24), its series and their
+    roundings are off by 1e-7 at most: 2^-22 in all."""
+    if kind == torch.int32 and size >= 2**31:
+        pytest.skip("past the type")
+    places = torch.tensor([size, size - 1, -size, size // 3, size // 7 * 5, 1], dtype=torch.int64).to(kind)
+    freqs = torch.tensor([1.0, 0.7853981633974483, 1e-4, 1 / 3], dtype=torch.float64)
+    n = places.numel()
+    x = torch.zeros(1, 1, n, 8, device=DEV)
+    x[..., :4] = 1
+    y = ops.axes_rotary(x, places.view(1, n, 1).to(DEV), freqs.to(DEV), (4,)).double().cpu()
+    for i, c in enumerate(places.tolist()):
+        for p, f in enumerate(freqs.tolist()):
+            angle = float((Fraction(f) * Fraction(c)) % (2 * PI))
+            assert abs(y[0, 0, i, p].item() - math.cos(angle)) <= 2.0**-22, (c, f)
+            assert abs(y[0, 0, i, 4 + p].item() - math.sin(angle)) <= 2.0**-22, (c, f)
