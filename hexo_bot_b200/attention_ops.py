@@ -18,7 +18,8 @@ keep anything between calls, and may be captured into CUDA graphs. Gradients go
 through autograd, or through the `*_backward` functions; a capture of autograd's
 backward must not find an eager graph of the same leaves alive (torch then has
 the capture wait for the other stream and fail), the functions have no such
-limit. CUDA tensors only: there is no CPU fallback.
+limit. There is no forward-mode derivative, and traces (`torch.jit.trace`, `make_fx`) are refused;
+`torch.compile` leaves the calls outside of its graphs. CUDA tensors only: there is no CPU fallback.
 """
 
 from __future__ import annotations
@@ -29,6 +30,7 @@ from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -108,6 +110,17 @@ def _call(t: torch.Tensor, what: str, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+def _visible(*ts) -> None:
+    """Refuses calls that would lose something in silence: a trace would not see the kernel and keep
+    its outputs as memory without values, a forward-mode tangent of ts would be dropped."""
+
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("the kernels cannot be traced: leave the call outside of the traced function")
+    if forward_ad._current_level >= 0:
+        if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+            raise RuntimeError("the kernels have no forward-mode derivative")
+
+
 def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -184,6 +197,7 @@ def axes_rotary(x, coords, freqs, sections, *, adjacent=False, inverse=False, ou
     Coordinates and angles up to 2^53 keep 32-bit accuracy.
     `inverse` turns back. `out` may be x (in place, not under autograd)."""
 
+    _visible(x, coords, freqs)
     _first(x, "x")
     if _wants_grad(x):
         if out is not None:
@@ -235,6 +249,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, coords, fr
     """Gradients (dq, dk, dq_weight, dk_weight) of `qk_norm_rotary` from those of its outputs; a
     weight that is None has none."""
 
+    _visible(dq_out, dk_out, q, k, q_weight, k_weight, coords, freqs)
     sizes, dt, wdt, rot = _qk_args(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps)
     _check(dq_out, "dq_out", q, q.shape, q.dtype)
     _check(dk_out, "dk_out", q, k.shape, q.dtype)
@@ -271,6 +286,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, coords=None, freqs=None, sections=(
     """RMS norm of every head of q (B, Hq, S, D) and k (B, Hk, S, D), times a weight per channel
     ((D) or None), then the rotation of `axes_rotary` (coords None: none), in one pass."""
 
+    _visible(q, k, q_weight, k_weight, coords, freqs)
     _first(q, "q")
     if _wants_grad(q, k, q_weight, k_weight):
         return _QkNorm.apply(q, k, q_weight, k_weight, coords, freqs, tuple(sections), adjacent, eps)
@@ -284,6 +300,7 @@ def block_means(k, block, *, kv_lens=None):
     """(B, H, ceil(S / block), D) float32 means of the live keys (t < kv_lens[b]) of each block of
     k (B, H, S, D); 0 for a block without any. No gradient: the choice of blocks has none."""
 
+    _visible()
     _first(k, "k")
     b, h, s, d = k.shape
     _int(block, "block", 1)
@@ -300,6 +317,7 @@ def block_select(q, means, topk, block, kv_rows, *, kv_lens=None, q_lens=None, k
     a serving program keeps up to date). The first `keep_first` blocks, and with `keep_own` the
     block row // block, are always kept. Ties go to the lowest index."""
 
+    _visible()
     _first(q, "q")
     b, hq, sq, d = q.shape
     if not isinstance(means, torch.Tensor) or means.dim() != 4:
@@ -355,6 +373,7 @@ def _attend(q, k, v, index, block, scale, kv_lens, q_lens):
 def block_attention_backward(dout, q, k, v, out, lse, index, block, *, scale=None, kv_lens=None, q_lens=None):
     """Gradients (dq, dk, dv) of `block_attention` from that of `out` and the forward's results."""
 
+    _visible(dout, q, k, v, out, lse)
     sizes, dt, scale = _attn_args(q, k, v, index, block, scale)
     b, hq, _, sq = sizes[:4]
     _check(dout, "dout", q, q.shape, q.dtype)
@@ -400,6 +419,7 @@ def block_attention(q, k, v, index, block, *, scale=None, kv_lens=None, q_lens=N
     once), block 32, 64 or 128, scale 1 / sqrt(D) by default. lse (B, Hq, Sq) float32 is the log of
     each row's sum of exp(scores). Rows without keys and rows past q_lens give zeros and -inf."""
 
+    _visible(q, k, v)
     _first(q, "q")
     if _wants_grad(q, k, v):
         return _Attend.apply(q, k, v, index, block, scale, kv_lens, q_lens)

@@ -1,0 +1,47 @@
+"""What the long-support attention operators refuse or promise at the edges of
+their use, without a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from hexo_bot_b200 import attention_ops as ops
+
+X = torch.zeros(1, 2, 4, 16)
+W = torch.ones(16)
+COORDS = torch.zeros(1, 4, 1, dtype=torch.int32)
+FREQS = ops.rotary_freqs((8,), device="cpu")
+INDEX = torch.zeros(1, 2, 4, 1, dtype=torch.int32)
+
+CALLS = {
+    "axes_rotary": lambda x: ops.axes_rotary(x, COORDS, FREQS, (8,)),
+    "qk_norm_rotary q": lambda x: ops.qk_norm_rotary(x, X, W, W, COORDS, FREQS, (8,)),
+    "qk_norm_rotary k": lambda x: ops.qk_norm_rotary(X, x, W, W, COORDS, FREQS, (8,)),
+    "qk_norm_rotary weight": lambda x: ops.qk_norm_rotary(X, X, None, x[0, 0, 0]),
+    "qk_norm_rotary_backward": lambda x: ops.qk_norm_rotary_backward(X, x, X, X, W, W, COORDS, FREQS, (8,)),
+    "block_attention q": lambda x: ops.block_attention(x, X, X, INDEX, 64),
+    "block_attention v": lambda x: ops.block_attention(X, X, x, INDEX, 64),
+    "block_attention_backward": lambda x: ops.block_attention_backward(x, X, X, X, X, X[..., 0], INDEX, 64),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_tangents_are_refused(name):
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(1, 2, 4, 16), torch.ones(1, 2, 4, 16))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            CALLS[name](x)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):  # a level without tangents changes nothing
+            CALLS[name](X)
+
+
+@pytest.mark.parametrize("name", [*CALLS, "block_means", "block_select"])
+def test_traces_are_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    calls = dict(CALLS, block_means=lambda x: ops.block_means(x, 64), block_select=lambda x: ops.block_select(x, X, 1, 64, 4))
+    for trace in (lambda f: torch.jit.trace(f, (X,)), lambda f: make_fx(f)(X)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            trace(calls[name])

@@ -190,3 +190,17 @@ def test_coordinates_of_any_size(size, kind):
             angle = float((Fraction(f) * Fraction(c)) % (2 * PI))
             assert abs(y[0, 0, i, p].item() - math.cos(angle)) <= 2.0**-22, (c, f)
             assert abs(y[0, 0, i, 4 + p].item() - math.sin(angle)) <= 2.0**-22, (c, f)
+
+
+# ---- beside torch -----------------------------------------------------------------------------
+
+
+def test_compiled_programs_call_the_operators_as_they_are():
+    x = randn(gen(121), 1, 2, 6, 16)
+    coords = torch.ones(1, 6, 1, dtype=torch.int32, device=DEV)
+    freqs = ops.rotary_freqs((8,), device=DEV)
+
+    def step(x):
+        return ops.axes_rotary(x * 2, coords, freqs, (8,)) + 1
+
+    assert torch.equal(torch.compile(step, backend="eager")(x), step(x))
