@@ -171,6 +171,8 @@ def _turn(x, coords, freqs, sections, adjacent, inverse, out=None):
     y = torch.empty_like(x) if out is None else _check(out, "out", x, x.shape, x.dtype)
     hx, hy = _heads(x, "x"), _heads(y, "out")
     _call(x, "axes_rotary", _lib.lib().sb_axes_rotary, hx, _FLOATS[x.dtype], rot, inverse, b, h, s, d, hy)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
     return y
 
 
@@ -195,11 +197,12 @@ def axes_rotary(x, coords, freqs, sections, *, adjacent=False, inverse=False, ou
     as they are. sections: pairs of each axis; freqs: `rotary_freqs(sections)`. Half pairing joins
     channels (p, P + p) of the P pairs, `adjacent` (2p, 2p + 1); channels from 2P on stay.
     Coordinates and angles up to 2^53 keep 32-bit accuracy.
-    `inverse` turns back. `out` may be x (in place, not under autograd)."""
+    `inverse` turns back. `out` may be x; it is written without autograd's knowledge and must not
+    need a gradient, but graphs that kept it refuse their backward, as after torch's own writes."""
 
     _visible(x, coords, freqs)
     _first(x, "x")
-    if _wants_grad(x):
+    if _wants_grad(x, out):
         if out is not None:
             raise ValueError("out= is not differentiable")
         return _Turn.apply(x, coords, freqs, tuple(sections), adjacent, inverse)

@@ -204,3 +204,29 @@ def test_compiled_programs_call_the_operators_as_they_are():
         return ops.axes_rotary(x * 2, coords, freqs, (8,)) + 1
 
     assert torch.equal(torch.compile(step, backend="eager")(x), step(x))
+
+
+def test_writes_into_out_are_seen_by_autograd():
+    """A graph that kept a tensor which `out` overwrote refuses its backward; an `out` that needs a
+    gradient is refused."""
+    coords = torch.ones(1, 6, 1, dtype=torch.int32, device=DEV)
+    freqs = ops.rotary_freqs((8,), device=DEV)
+    x = randn(gen(122), 1, 2, 6, 16)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    loss = (w * x).sum()
+    ops.axes_rotary(x, coords, freqs, (8,), out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    y = x.clone()
+    kept = (w * y).sum()
+    ops.axes_rotary(x, coords, freqs, (8,), out=torch.empty_like(x))  # another tensor: nothing changes
+    kept.backward()
+    leaf = torch.empty_like(x, requires_grad=True)
+    with pytest.raises(ValueError, match="out="):
+        ops.axes_rotary(x, coords, freqs, (8,), out=leaf)
+    with torch.no_grad():
+        want = ops.axes_rotary(x, coords, freqs, (8,))
+        assert torch.equal(ops.axes_rotary(x, coords, freqs, (8,), out=leaf), want)
+    with torch.inference_mode():
+        z = x.clone()
+        assert torch.equal(ops.axes_rotary(z, coords, freqs, (8,), out=z), want)
