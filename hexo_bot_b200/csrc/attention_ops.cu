@@ -229,21 +229,13 @@ constexpr int kBaFewRows = 16;
 // with 4 / 6 / 8 / 12 / 16), smaller ones repeat the listing and the key loads.
 constexpr int kBaItems = 16, kBaBwdItems = 8, kBaMinTarget = 256, kBaMaxTarget = 1024;
 
-// Segments of `seg` list groups over all windows of wq rows.
-int ba_segments(int q_rows, int wq, int seg) {
-  long long n = 0;
-  for (long long w0 = 0; w0 < q_rows; w0 += wq) n += cdiv(cdiv(q_rows - w0 < wq ? q_rows - w0 : wq, kBaMark), seg);
-  return (int)n;
-}
-
 struct BaPlan {
-  int marks, bh_step, wq, seg;
+  int marks, bh_step, wq, seg, sums;
   size_t ticket, entries, spans, slots, part, ml, delta, kv_part, total;
 };
 
 BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, int topk, bool backward) {
   BaPlan p{};
-  p.marks = (int)cdiv(q_rows, kBaMark);
   const long long row_bytes = (long long)group * topk * (dim * 4 + (backward ? 0 : 8));
   const long long per_bh = row_bytes * q_rows;
   if (per_bh <= kBaWindowBytes) {
@@ -262,17 +254,22 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   const int most = backward ? 2 * kBaMaxTarget : kBaMaxTarget;
   target = target < kBaMinTarget ? kBaMinTarget : target > most ? most : target;
   const long long groups = cdiv(p.wq, kBaMark);
+  p.marks = (int)groups;
   long long seg = cdiv(target * nb, (long long)topk * group * kBaMark);
   seg = seg < 1 ? 1 : seg > groups ? groups : seg;
   p.seg = (int)cdiv(groups, cdiv(groups, seg));
+  // backward: sums of dk and dv that a block has, one a segment of its window; the
+  // windows of a head add to the same ones, and all heads of a step share them
+  const int nseg = (int)cdiv(groups, p.seg);
+  p.sums = backward && (nseg > 1 || p.wq < q_rows) ? nseg : 0;
   const long long rows = (long long)p.bh_step * p.wq * group;
   size_t at = 0;
   p.ticket = at;
   at += 256;
   p.entries = at;
-  at += align256((size_t)bh * p.marks * kBaMark * topk * 2);
+  at += align256((size_t)p.bh_step * p.marks * kBaMark * topk * 2);
   p.spans = at;
-  at += align256((size_t)bh * nb * p.marks * 4);
+  at += align256((size_t)p.bh_step * nb * p.marks * 4);
   p.slots = at;
   at += align256((size_t)bh * q_rows * 8);
   p.part = at;
@@ -282,10 +279,7 @@ BaPlan ba_plan(long long bh, int q_rows, int group, int dim, int nb, int block, 
   p.delta = at;
   if (backward) at += align256((size_t)bh * q_rows * group * 8);
   p.kv_part = at;
-  if (backward) {
-    const long long nseg = ba_segments(q_rows, p.wq, p.seg);
-    if (nseg > 1) at += align256((size_t)bh * nb * nseg * 2 * block * dim * 4);
-  }
+  at += align256((size_t)p.bh_step * nb * p.sums * 2 * block * dim * 4);
   p.total = at;
   return p;
 }
@@ -338,7 +332,7 @@ int launch_ba(K kern, const char* name, long long grid, int threads, int smem, c
 }
 
 int launch_list(const BaArgs& a, cudaStream_t st) {
-  const long long grid = (long long)a.batch * a.kv_heads * a.marks;
+  const long long grid = a.nbh * cdiv(a.wq, kBaMark);
   const int smem = ba_list_smem(a.nb, a.topk);
   if (a.topk <= 8) return launch_ba(block_list_kernel<8>, "block_list_kernel", grid, kBaMark, smem, a, st);
   if (a.topk <= 16) return launch_ba(block_list_kernel<16>, "block_list_kernel", grid, kBaMark, smem, a, st);
@@ -426,20 +420,20 @@ void ba_fill(BaArgs* a, const int32_t* index, const int32_t* kv_lens, const int3
   a->group_magic = magic(a->group);
 }
 
-// Runs f(args) for every window of the plan.
-template <typename F>
-int ba_windows(BaArgs& a, const BaPlan& p, F f) {
+// Lists every window of the plan and runs f() for it, and done() behind the last one of each step of heads.
+template <typename F, typename G>
+int ba_windows(BaArgs& a, const BaPlan& p, cudaStream_t st, F f, G done) {
   const int bh = a.batch * a.kv_heads;
   for (a.bh0 = 0; a.bh0 < bh; a.bh0 += p.bh_step) {
     a.nbh = bh - a.bh0 < p.bh_step ? bh - a.bh0 : p.bh_step;
-    a.seg0 = 0;
     for (a.w0 = 0; a.w0 < a.q_rows; a.w0 += p.wq) {
       a.wq = a.q_rows - a.w0 < p.wq ? a.q_rows - a.w0 : p.wq;
       a.seg = p.seg;
       a.nseg = (int)cdiv(cdiv(a.wq, kBaMark), p.seg);
+      if (int s = launch_list(a, st)) return s;
       if (int s = f()) return s;
-      a.seg0 += a.nseg;
     }
+    if (int s = done()) return s;
   }
   return SB_OK;
 }
@@ -715,8 +709,7 @@ int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, 
   a.part = (float*)(ws + p.part);
   a.ml = (float2*)(ws + p.ml);
   a.ticket = (uint32_t*)(ws + p.ticket);
-  if (int s = launch_list(a, st)) return s;
-  return ba_windows(a, p, [&] { return ba_dispatch(dtype, head_dim, block, LaunchFwd{a, st}); });
+  return ba_windows(a, p, st, [&] { return ba_dispatch(dtype, head_dim, block, LaunchFwd{a, st}); }, [] { return SB_OK; });
 }
 
 int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const sb_heads* k, const sb_heads* v,
@@ -767,20 +760,22 @@ int sb_block_attention_backward(const sb_heads* dout, const sb_heads* q, const s
   a.delta = (float2*)(ws + p.delta);
   a.kv_part = (float*)(ws + p.kv_part);
   a.ticket = (uint32_t*)(ws + p.ticket);
-  a.nseg_all = ba_segments(q_rows, p.wq, p.seg);
+  a.sums = p.sums;
   cudaStream_t st = (cudaStream_t)stream;
-  if (int s = launch_list(a, st)) return s;
   const int chunks = 1 << pow2_log2(head_dim / 8);
   const long long dgrid = cdiv(bh * q_rows * a.group * chunks, 256);
   const bool f16 = dtype == SB_F16;
   if (int s = f16 ? launch_ba(block_attn_delta_kernel<__half>, "block_attn_delta_kernel", dgrid, 256, 0, a, st)
                   : launch_ba(block_attn_delta_kernel<__nv_bfloat16>, "block_attn_delta_kernel", dgrid, 256, 0, a, st))
     return s;
-  if (int s = ba_windows(a, p, [&] { return ba_dispatch(dtype, head_dim, block, LaunchBwd{a, st}); })) return s;
-  if (a.nseg_all <= 1) return SB_OK;
-  const long long kgrid = cdiv(bh * kv_rows * (head_dim / 8), 256);
-  return f16 ? launch_ba(block_attn_dkv_kernel<__half>, "block_attn_dkv_kernel", kgrid, 256, 0, a, st)
-             : launch_ba(block_attn_dkv_kernel<__nv_bfloat16>, "block_attn_dkv_kernel", kgrid, 256, 0, a, st);
+  return ba_windows(
+      a, p, st, [&] { return ba_dispatch(dtype, head_dim, block, LaunchBwd{a, st}); },
+      [&] {
+        if (a.sums == 0) return (int)SB_OK;
+        const long long kgrid = cdiv((long long)a.nbh * kv_rows * (head_dim / 8), 256);
+        return f16 ? launch_ba(block_attn_dkv_kernel<__half>, "block_attn_dkv_kernel", kgrid, 256, 0, a, st)
+                   : launch_ba(block_attn_dkv_kernel<__nv_bfloat16>, "block_attn_dkv_kernel", kgrid, 256, 0, a, st);
+      });
 }
 
 }  // extern "C"

@@ -45,19 +45,20 @@ struct BaArgs {
   const int* idx;         // (B, Hkv, Sq, topk)
   const int* kv_lens;
   const int* q_lens;
-  uint16_t* entries;      // (B Hkv, marks, kBaMark topk): per group, by block: place in the row's list << 8 | query
-  uint32_t* spans;        // (B Hkv, nb, marks): first entry of the group's queries that chose the block | count << 16
+  uint16_t* entries;      // window's (local bh, marks, kBaMark topk): per group, by block: place in the row's list << 8 | query
+  uint32_t* spans;        // (local bh, nb, marks): first entry of the group's queries that chose the block | count << 16
   uint32_t* ticket;       // work items that the persistent CTAs have taken; 0 before each launch
   unsigned long long* slots;  // (B Hkv, Sq): bit s = entry s of the row's list counts
   float* part;            // window's parts: [row][topk][dim], row = (local bh * wq + local i) * group + g
   float2* ml;             // forward: [row][topk] (max in log2 units, sum)
   float2* delta;          // backward: (B Hkv, Sq, group) do . out, and the norm of do (f16 alone reads it)
-  float* kv_part;         // backward, more than one segment: [bh][nb][nseg][2][block][dim]
-  int batch, kv_heads, group, q_rows, kv_rows, dim, nb, block, topk, marks;
+  float* kv_part;         // backward, more than one segment or window: [local bh][nb][sums][2][block][dim]
+  int batch, kv_heads, group, q_rows, kv_rows, dim, nb, block, topk;
+  int marks;              // list groups of a full window
   int bh0, nbh;           // window: first (batch, kv head) pair and their count
   int w0, wq;             // window: first query and count (w0 a multiple of kBaMark)
   int seg, nseg;          // list groups of a segment, segments of the window
-  int seg0, nseg_all;     // backward: index of the window's first segment, segments in all
+  int sums;               // backward: sums of dk and dv that a block has, one a segment; 0: results at once
   float scale, scale_log2;
   uint32_t group_magic;   // ceil(2^32 / group), 0 for group 1
 };
@@ -72,8 +73,8 @@ __device__ __forceinline__ int ba_q_len(const BaArgs& a, int b) {
 }
 
 // ---- who chose what -----------------------------------------------------------
-// One CTA per 256 queries of a (batch, kv head) turns their lists round: for
-// every block the queries that chose it, ascending, with the place of the block
+// One CTA per 256 queries of a window's (batch, kv head) turns their lists round:
+// for every block the queries that chose it, ascending, with the place of the block
 // in each query's list. A bit per (block, query) in shared memory counts and
 // orders them (a counting sort whose result no scheduling changes) and shows
 // repeated entries: `slots` marks the entries that count.
@@ -94,10 +95,11 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
   uint16_t* sorted = offs + 8 * W;                               // [256 topk]
   __shared__ uint32_t warp_sum[kBaMark / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int bh = blockIdx.x / a.marks, mark = blockIdx.x - bh * a.marks;
+  const int marks = (a.wq + kBaMark - 1) / kBaMark;
+  const int lbh = blockIdx.x / marks, mark = blockIdx.x - lbh * marks, bh = a.bh0 + lbh;
   const int b = bh / a.kv_heads;
-  const int i = mark * kBaMark + tid;
-  const bool on = i < a.q_rows;
+  const int i = a.w0 + mark * kBaMark + tid;
+  const bool on = i < a.w0 + a.wq;
   const int* src = a.idx + ((long long)bh * a.q_rows + i) * K;
   int e[KR];
 #pragma unroll
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int j = tid * 4 + y;
-      if (j < n) a.spans[((long long)bh * a.nb + j0 + j) * a.marks + mark] = at | sum[y] << 16;
+      if (j < n) a.spans[((long long)lbh * a.nb + j0 + j) * a.marks + mark] = at | sum[y] << 16;
 #pragma unroll
       for (int w = 0; w < 8; ++w) {
         if (j < n) offs[w * W + j] = (uint16_t)at;
@@ -177,13 +179,13 @@ __global__ __launch_bounds__(kBaMark) void block_list_kernel(const BaArgs a) {
     __syncthreads();
   }
   // out in 16-byte pieces (the group's place holds 256 topk entries)
-  uint4* dst = reinterpret_cast<uint4*>(a.entries + ((long long)bh * a.marks + mark) * kBaMark * K);
+  uint4* dst = reinterpret_cast<uint4*>(a.entries + ((long long)lbh * a.marks + mark) * kBaMark * K);
   for (int x = tid; x < ((int)base + 7) / 8; x += kBaMark) dst[x] = reinterpret_cast<const uint4*>(sorted)[x];
   unsigned long long counts = 0;
 #pragma unroll
   for (int s = 0; s < KR; ++s) counts |= (unsigned long long)(e[s] >= 0) << s;
   if (on) a.slots[(long long)bh * a.q_rows + i] = counts;
-  if (blockIdx.x == 0 && tid == 0 && a.ticket) *a.ticket = 0;
+  if (blockIdx.x == 0 && tid == 0) *a.ticket = 0;
 }
 
 // ---- shared-memory tiles ---------------------------------------------------------
@@ -209,17 +211,17 @@ __device__ __forceinline__ void ba_load_rows(uint32_t dst, const T* src, long lo
   }
 }
 
-// The queries that chose block j in the list groups from g on (up to `end`), as
+// The queries that chose block j in the window's list groups from g on (up to `end`), as
 // many whole groups as fit kBaChunk: list[] gets query << 6 | place in its list,
 // ascending. Moves g past the groups taken; returns the number listed. Every
 // thread of the CTA calls it; it begins and ends with a barrier.
 template <int THREADS>
-__device__ __forceinline__ int ba_fill(const BaArgs& a, int bh, int j, int& g, int end, uint32_t* list) {
+__device__ __forceinline__ int ba_fill(const BaArgs& a, int lbh, int j, int& g, int end, uint32_t* list) {
   __shared__ uint32_t pos[THREADS + 1], first[THREADS];
   __shared__ uint32_t warp_sum[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool in = g + tid < end;
-  const uint32_t sp = in ? a.spans[((long long)bh * a.nb + j) * a.marks + g + tid] : 0u;
+  const uint32_t sp = in ? a.spans[((long long)lbh * a.nb + j) * a.marks + g + tid] : 0u;
   const uint32_t cnt = sp >> 16;
   uint32_t pre = cnt;
 #pragma unroll
@@ -236,7 +238,7 @@ __device__ __forceinline__ int ba_fill(const BaArgs& a, int bh, int j, int& g, i
   if (tid == 0) pos[0] = 0;
   const int taken = __syncthreads_count(in && pre <= kBaChunk);
   const int n = (int)pos[taken];
-  const uint16_t* entries = a.entries + ((long long)bh * a.marks + g) * kBaMark * a.topk;
+  const uint16_t* entries = a.entries + ((long long)lbh * a.marks + g) * kBaMark * a.topk;
   for (int e0 = tid; e0 < n; e0 += 4 * THREADS) {  // four entries in flight
     int lo[4];
     uint32_t x[4];
@@ -254,7 +256,7 @@ __device__ __forceinline__ int ba_fill(const BaArgs& a, int bh, int j, int& g, i
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y)
-      if (e0 + y * THREADS < n) list[e0 + y * THREADS] = (uint32_t)((g + lo[y]) * kBaMark + (x[y] & 255)) << 6 | x[y] >> 8;
+      if (e0 + y * THREADS < n) list[e0 + y * THREADS] = (uint32_t)(a.w0 + (g + lo[y]) * kBaMark + (x[y] & 255)) << 6 | x[y] >> 8;
   }
   g += taken;
   __syncthreads();
@@ -525,8 +527,8 @@ __global__ __launch_bounds__(kBaFwdThreads, ba_fwd_ctas<DP, BK>()) void block_at
     const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
     const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
     const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-    int g = a.w0 / kBaMark + sg * a.seg;
-    const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
+    int g = sg * a.seg;
+    const int end = min(g + a.seg, (a.wq + kBaMark - 1) / kBaMark);
     const int have = min(BK, ba_kv_len(a, b) - j * BK);
     __syncthreads();  // the item before is done with the keys, and its successor has been read
     if (tid == 0) next_item = gridDim.x + atomicAdd(a.ticket, 1u);
@@ -538,7 +540,7 @@ __global__ __launch_bounds__(kBaFwdThreads, ba_fwd_ctas<DP, BK>()) void block_at
     ba_load_panels<T, DP, BK>(vs, (const T*)a.v.p + b * a.v.b + h * a.v.h + (long long)j * BK * a.v.s, a.v.s, have, a.dim);
     }
     while (g < end) {
-      const int n = ba_fill<kBaFwdThreads>(a, bh, j, g, end, list);
+      const int n = ba_fill<kBaFwdThreads>(a, lbh, j, g, end, list);
       if (n == 0) continue;
       const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
       // a warp loads the 32 rows whose offsets its lanes worked out
@@ -739,7 +741,6 @@ __device__ __forceinline__ void ba_strand_sum(float (&acc)[8], const BaRow& r) {
 // Joins the parts of each row, four parts a lane in flight.
 template <typename T>
 __global__ __launch_bounds__(kBaJoinThreads) void block_attn_join_kernel(const BaArgs a) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;  // for the next window
   const BaRow r(a);
   const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
   const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
@@ -1091,8 +1092,8 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
     const int j = (int)(u / (uint32_t)a.nseg % (uint32_t)a.nb);
     const int lbh = (int)(u / (uint32_t)a.nseg / (uint32_t)a.nb), bh = a.bh0 + lbh;
     const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-    int g = a.w0 / kBaMark + sg * a.seg;
-    const int end = min(g + a.seg, (a.w0 + a.wq + kBaMark - 1) / kBaMark);
+    int g = sg * a.seg;
+    const int end = min(g + a.seg, (a.wq + kBaMark - 1) / kBaMark);
     const int have = max(0, min(BK, ba_kv_len(a, b) - j * BK));
     tc_fence_before();
     __syncthreads();  // the item before is done with the keys and with dv, dk
@@ -1111,7 +1112,7 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
     int ex = 0;        // f16: ds and dk are held times 2^ex
     float v_norm = 0.f;
     while (g < end) {
-      const int n = ba_fill<kBaBwdThreads>(a, bh, j, g, end, list);
+      const int n = ba_fill<kBaBwdThreads>(a, lbh, j, g, end, list);
       if (n == 0) continue;
       const int rows = n * G, tiles = (rows + ROWS - 1) / ROWS;
       float lse = INFINITY;  // of this thread's row of the next tile, as loaded
@@ -1369,14 +1370,18 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
 #pragma unroll
         for (int x = 0; x < 16; x += 8) {
           if (c0 + x >= a.dim) continue;
-          if (a.nseg_all > 1) {
+          if (a.sums > 0) {
             float4* p = reinterpret_cast<float4*>(
-                a.kv_part + ((((long long)bh * a.nb + j) * a.nseg_all + a.seg0 + sg) * 2 * BK + (is_v ? BK : 0) + key) * a.dim +
-                c0 + x);
-            // the sum over the segments scales
+                a.kv_part + ((((long long)lbh * a.nb + j) * a.sums + sg) * 2 * BK + (is_v ? BK : 0) + key) * a.dim + c0 + x);
+            // the sum over the segments scales; windows after the first add to what the ones before left
             const float one = ok ? down : f;
-            p[0] = make_float4(o[x] * one, o[x + 1] * one, o[x + 2] * one, o[x + 3] * one);
-            p[1] = make_float4(o[x + 4] * one, o[x + 5] * one, o[x + 6] * one, o[x + 7] * one);
+            float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+            if (a.w0 > 0) {
+              u = p[0];
+              v = p[1];
+            }
+            p[0] = make_float4(u.x + o[x] * one, u.y + o[x + 1] * one, u.z + o[x + 2] * one, u.w + o[x + 3] * one);
+            p[1] = make_float4(v.x + o[x + 4] * one, v.y + o[x + 5] * one, v.z + o[x + 6] * one, v.w + o[x + 7] * one);
           } else if (j * BK + key < a.kv_rows) {
             const HeadsView& d = is_v ? a.dv : a.dk;
             T* p = (T*)d.p + b * d.b + h * d.h + (long long)(j * BK + key) * d.s + c0 + x;
@@ -1398,7 +1403,6 @@ __global__ __launch_bounds__(kBaBwdThreads, ba_bwd_ctas<DP, BK>()) void block_at
 // dq of the window: the sum of each row's parts.
 template <typename T>
 __global__ __launch_bounds__(kBaJoinThreads) void block_attn_dq_kernel(const BaArgs a) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;  // for the next window
   const BaRow r(a);
   const bool there = r.row < (long long)a.nbh * a.wq * a.group;  // the others stay for the shuffles
   const int bh = there ? a.bh0 + r.lbh : 0, b = bh / a.kv_heads, h = (bh - b * a.kv_heads) * a.group + r.g;
@@ -1429,22 +1433,22 @@ __global__ __launch_bounds__(kBaJoinThreads) void block_attn_dq_kernel(const BaA
   *reinterpret_cast<RotVec<T, 8>*>((T*)a.dq.p + b * a.dq.b + h * a.dq.h + r.i * a.dq.s + r.c) = y;
 }
 
-// dk, dv: the sum of the segments' parts, in segment order.
+// dk, dv of a step's heads: the sum over the segments, in their order.
 template <typename T>
 __global__ __launch_bounds__(256) void block_attn_dkv_kernel(const BaArgs a) {
   const int chunks = a.dim / 8;
-  const long long total = (long long)a.batch * a.kv_heads * a.kv_rows * chunks;
+  const long long total = (long long)a.nbh * a.kv_rows * chunks;
   const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
   if (x >= total) return;
   const long long row = x / chunks;
   const int c = (int)(x - row * chunks);
-  const int bh = (int)(row / a.kv_rows), t = (int)(row - (long long)bh * a.kv_rows);
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const int lbh = (int)(row / a.kv_rows), t = (int)(row - (long long)lbh * a.kv_rows);
+  const int bh = a.bh0 + lbh, b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const int j = t / a.block, key = t - j * a.block;
   const long long step = 2ll * a.block * a.dim;
-  const float* p = a.kv_part + ((long long)bh * a.nb + j) * a.nseg_all * step + (long long)key * a.dim + c * 8;
+  const float* p = a.kv_part + ((long long)lbh * a.nb + j) * a.sums * step + (long long)key * a.dim + c * 8;
   float acc[2][8] = {};
-  for (int s = 0; s < a.nseg_all; ++s, p += step)
+  for (int s = 0; s < a.sums; ++s, p += step)
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const float4* src = reinterpret_cast<const float4*>(p + (long long)w * a.block * a.dim);

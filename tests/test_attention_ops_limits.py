@@ -3,10 +3,13 @@ their use, without a GPU."""
 
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from hexo_bot_b200 import _lib
 from hexo_bot_b200 import attention_ops as ops
 
 X = torch.zeros(1, 2, 4, 16)
@@ -45,3 +48,27 @@ def test_traces_are_refused(name):
     for trace in (lambda f: torch.jit.trace(f, (X,)), lambda f: make_fx(f)(X)):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             trace(calls[name])
+
+
+def workspace(backward, batch, q_heads, kv_heads, rows, dim, block, topk):
+    need = C.c_size_t()
+    rc = _lib.lib().sb_block_attention_workspace_bytes(batch, q_heads, kv_heads, rows, rows, dim, block, topk, backward, need)
+    assert rc == 0, _lib.last_error()
+    return need.value
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("batch", [1, 8])
+@pytest.mark.parametrize("topk", [16, 64])
+@pytest.mark.parametrize("rows", [2000, 32768, 131072, 1 << 20])
+def test_workspace_of_long_calls(rows, topk, batch, backward):
+    """At most 1 GB of parts, the lists of as many rows (entries and where a block's queries begin),
+    8 bytes a row for flags, 8 for the backward, and its sums of dk and dv: those of one head in 32
+    bits, or 400 MB for the segments of a window."""
+    q_heads, kv_heads, dim, block = 32, 8, 128, 64
+    bh = batch * kv_heads
+    marks = min(bh * (rows // 256 + 1), 2**30 // (4 * topk * dim * 4) // 256 + bh)
+    lists = marks * (2 * topk * 256 + 4 * (rows // block + 1)) + 8 * bh * rows
+    sums = max(2 * (rows + block) * dim * 4, 400 << 20)
+    most = (1 << 30) + lists + backward * (8 * batch * q_heads * rows + sums) + (1 << 20)
+    assert workspace(backward, batch, q_heads, kv_heads, rows, dim, block, topk) <= most
