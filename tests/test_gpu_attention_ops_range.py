@@ -230,3 +230,44 @@ def test_writes_into_out_are_seen_by_autograd():
     with torch.inference_mode():
         z = x.clone()
         assert torch.equal(ops.axes_rotary(z, coords, freqs, (8,), out=z), want)
+
+
+# ---- several windows ----------------------------------------------------------------------------
+
+WINDOWS = [
+    # b, hq, hk, sq, sk, d, block, topk, heads of a window (0: windows over the rows of a head)
+    (2, 8, 2, 4200, 1500, 128, 32, 40, 3),
+    (5, 6, 3, 4300, 700, 64, 64, 60, 7),
+    (1, 4, 1, 13500, 1500, 128, 32, 40, 0),
+    (1, 4, 1, 13500, 4000, 128, 128, 40, 0),
+    (2, 2, 1, 33000, 500, 64, 64, 64, 0),
+]
+
+
+@pytest.mark.parametrize("case", WINDOWS)
+def test_block_attention_over_several_windows(case):
+    """Parts past 1 GB: several launches over heads, and over the rows of one head. Against 64 bits, and
+    the forward against the same heads one at a time, bit for bit."""
+    b, hq, hk, sq, sk, d, block, topk, heads = case
+    parts = hq // hk * topk * (4 * d + 8) * sq  # of one key head, forward
+    assert b * hk * parts > 2**30 and (parts > 2**30) == (heads == 0)
+    assert heads == 2**30 // parts < b * hk or heads == 0
+    q, k, v, index, block, dout = tensors(case[:8], BF16, 131)
+    qn = torch.tensor([sq - 77 * i for i in range(b)], dtype=torch.int32, device=DEV)
+    kn = torch.tensor([sk - 99 * i for i in range(b)], dtype=torch.int32, device=DEV)
+    out, lse = ops.block_attention(q, k, v, index, block, kv_lens=kn, q_lens=qn)
+    grads = ops.block_attention_backward(dout, q, k, v, out, lse, index, block, kv_lens=kn, q_lens=qn)
+    again = ops.block_attention_backward(dout, q, k, v, out, lse, index, block, kv_lens=kn, q_lens=qn)
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))
+    grp = hq // hk
+    for i in range(b):
+        for h in range(hk):
+            at, qs = (slice(i, i + 1), slice(h, h + 1)), (slice(i, i + 1), slice(h * grp, (h + 1) * grp))
+            one = q[qs], k[at], v[at], index[at].contiguous()
+            found, bound = O.attention(*one, block, None, kn[i : i + 1], qn[i : i + 1], dout[qs], pair=True)
+            within(out[qs], found["out"], bound["out"], "out")
+            within(lse[qs], found["lse"], bound["lse"], "lse")
+            for name, got in zip(("dq", "dk", "dv"), (grads[0][qs], grads[1][at], grads[2][at])):
+                within(got, found[name], bound[name], name)
+            alone = ops.block_attention(*one, block, kv_lens=kn[i : i + 1], q_lens=qn[i : i + 1])
+            assert torch.equal(alone[0], out[qs]) and torch.equal(alone[1], lse[qs])
