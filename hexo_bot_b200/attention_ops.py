@@ -97,17 +97,21 @@ def _lens(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> Optional[
     return t.data_ptr()
 
 
-def _call(t: torch.Tensor, what: str, fn, *args) -> None:
-    """fn(*args, stream) on t's device and its current stream; raises on a refusal."""
+def _on(t: torch.Tensor, what: str, fn, *args) -> None:
+    """fn(*args) with t's device as the current one; raises on a refusal."""
     index = t.device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, stream)
+        rc = fn(*args)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, stream)
+            rc = fn(*args)
     if rc:
         _lib.check(rc, what)
+
+
+def _call(t: torch.Tensor, what: str, fn, *args) -> None:
+    """fn(*args, stream) on t's device and its current stream; raises on a refusal."""
+    _on(t, what, fn, *args, torch._C._cuda_getCurrentRawStream(t.device.index))
 
 
 def _visible(*ts) -> None:
@@ -354,10 +358,10 @@ def _attn_args(q, k, v, index, block, scale):
     return (b, hq, hk, sq, sk, d, block, topk), _FLOATS[q.dtype], 1.0 / math.sqrt(d) if scale is None else float(scale)
 
 
-def _attn_workspace(sizes, backward, device):
-    need = C.c_size_t()
-    _lib.check(_lib.lib().sb_block_attention_workspace_bytes(*sizes, backward, need), "block_attention")
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None, need.value
+def _attn_workspace(t, sizes, backward):
+    need = C.c_size_t()  # the plan counts the SMs of the device that the call runs on
+    _on(t, "block_attention", _lib.lib().sb_block_attention_workspace_bytes, *sizes, backward, need)
+    return torch.empty(need.value, dtype=torch.uint8, device=t.device) if need.value else None, need.value
 
 
 def _attend(q, k, v, index, block, scale, kv_lens, q_lens):
@@ -365,7 +369,7 @@ def _attend(q, k, v, index, block, scale, kv_lens, q_lens):
     b, hq, _, sq = sizes[:4]
     out = torch.empty_like(q)
     lse = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
-    ws, need = _attn_workspace(sizes, 0, q.device)
+    ws, need = _attn_workspace(q, sizes, 0)
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
     hs, ho = (_heads(q, "q"), _heads(k, "k"), _heads(v, "v")), _heads(out, "out")
     _call(q, "block_attention", _lib.lib().sb_block_attention, *hs, dt, index.data_ptr(), kl, ql, *sizes, scale, ho,
@@ -387,7 +391,7 @@ def block_attention_backward(dout, q, k, v, out, lse, index, block, *, scale=Non
     if sq == 0:
         return torch.empty_like(q), torch.zeros_like(k), torch.zeros_like(v)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    ws, need = _attn_workspace(sizes, 1, q.device)
+    ws, need = _attn_workspace(q, sizes, 1)
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
     ins = _heads(dout, "dout"), _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(out, "out")
     outs = _heads(dq, "dq"), _heads(dk, "dk"), _heads(dv, "dv")

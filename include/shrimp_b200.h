@@ -330,7 +330,8 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
  * without keys, or past q_lens[b], gives zeros and lse = -inf. Results do not
  * vary from run to run. Few queries (<= 16 rows) need no workspace; others at
  * most about 1 GB and 8 bytes a query row and key head; the backward 8 bytes a
- * query row and head more, and dk and dv of one key head in 32 bits or 0.4 GB. */
+ * query row and head more, and dk and dv of one key head in 32 bits or 0.4 GB.
+ * The size is that for the device which is current, like the call. */
 int sb_block_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int q_rows, int kv_rows, int head_dim, int block,
                                        int topk, int backward, size_t* bytes);
 int sb_block_attention(const sb_heads* q, const sb_heads* k, const sb_heads* v, int dtype, const int32_t* index,

@@ -72,3 +72,46 @@ def test_workspace_of_long_calls(rows, topk, batch, backward):
     sums = max(2 * (rows + block) * dim * 4, 400 << 20)
     most = (1 << 30) + lists + backward * (8 * batch * q_heads * rows + sums) + (1 << 20)
     assert workspace(backward, batch, q_heads, kv_heads, rows, dim, block, topk) <= most
+
+
+def test_workspace_is_sized_on_the_tensors_device(monkeypatch):
+    """The plan depends on the device's SMs: the size is asked for where the call will run."""
+    current, asked = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def sb_block_attention_workspace_bytes(self, *args):
+            asked.append(current[0])
+            return 0
+
+        sb_block_attention = sb_block_attention_backward = None
+
+    class OnGpu1(torch.Tensor):
+        device = torch.device("cuda:1")
+        is_cuda = True
+
+    class Memory:
+        def data_ptr(self):
+            return 0
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops._lib, "lib", Lib)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: Memory())
+    monkeypatch.setattr(torch, "empty_like", lambda t: t)
+    monkeypatch.setattr(ops, "_check", lambda t, *a: t)
+    monkeypatch.setattr(ops, "_call", lambda *a: None)  # the launch
+    x = torch.zeros(1, 1, 20, 16, dtype=torch.float16).as_subclass(OnGpu1)
+    index = torch.zeros(1, 1, 20, 1, dtype=torch.int32)
+    ops.block_attention(x, x, x, index, 64)
+    ops.block_attention_backward(x, x, x, x, x, torch.zeros(1, 1, 20), index, 64)
+    assert asked == [1, 1] and current == [0]
