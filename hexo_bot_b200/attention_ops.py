@@ -81,6 +81,13 @@ def _heads(t: torch.Tensor, name: str) -> _lib.Heads:
     return _lib.Heads(t.data_ptr(), sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else 0)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A result of t's shape with unit stride over head_dim. empty_like follows t's strides, and puts
+    another axis last where t's rows or heads lie one element apart (windows that overlap)."""
+    y = torch.empty_like(t)
+    return y if y.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _grad(t: torch.Tensor) -> torch.Tensor:
     """An incoming gradient as a view the kernels read: packed anew unless it is one already."""
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
@@ -172,7 +179,7 @@ def _rotary(x, coords, freqs, sections, adjacent) -> Optional[_lib.Rotary]:
 def _turn(x, coords, freqs, sections, adjacent, inverse, out=None):
     b, h, s, d = x.shape
     rot = _rotary(x, coords, freqs, sections, adjacent)
-    y = torch.empty_like(x) if out is None else _check(out, "out", x, x.shape, x.dtype)
+    y = _like(x) if out is None else _check(out, "out", x, x.shape, x.dtype)
     hx, hy = _heads(x, "x"), _heads(y, "out")
     _call(x, "axes_rotary", _lib.lib().sb_axes_rotary, hx, _FLOATS[x.dtype], rot, inverse, b, h, s, d, hy)
     if out is not None:
@@ -245,7 +252,7 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _qk(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps):
     sizes, dt, wdt, rot = _qk_args(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps)
-    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    qo, ko = _like(q), _like(k)
     ins, outs = (_heads(q, "q"), _heads(k, "k")), (_heads(qo, "q"), _heads(ko, "k"))
     _call(q, "qk_norm_rotary", _lib.lib().sb_qk_norm_rotary, *ins, dt, _ptr(q_weight), _ptr(k_weight), wdt, eps, rot, *sizes,
           *outs)
@@ -260,7 +267,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, coords, fr
     sizes, dt, wdt, rot = _qk_args(q, k, q_weight, k_weight, coords, freqs, sections, adjacent, eps)
     _check(dq_out, "dq_out", q, q.shape, q.dtype)
     _check(dk_out, "dk_out", q, k.shape, q.dtype)
-    dq, dk = torch.empty_like(q), torch.empty_like(k)
+    dq, dk = _like(q), _like(k)
     dqw = None if q_weight is None else torch.empty_like(q_weight)
     dkw = None if k_weight is None else torch.empty_like(k_weight)
     need = C.c_size_t()
@@ -367,7 +374,7 @@ def _attn_workspace(t, sizes, backward):
 def _attend(q, k, v, index, block, scale, kv_lens, q_lens):
     sizes, dt, scale = _attn_args(q, k, v, index, block, scale)
     b, hq, _, sq = sizes[:4]
-    out = torch.empty_like(q)
+    out = _like(q)
     lse = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
     ws, need = _attn_workspace(q, sizes, 0)
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
@@ -390,7 +397,7 @@ def block_attention_backward(dout, q, k, v, out, lse, index, block, *, scale=Non
         raise ValueError("lse must be contiguous")
     if sq == 0:
         return torch.empty_like(q), torch.zeros_like(k), torch.zeros_like(v)
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    dq, dk, dv = _like(q), _like(k), _like(v)
     ws, need = _attn_workspace(q, sizes, 1)
     kl, ql = _lens(kv_lens, "kv_lens", q), _lens(q_lens, "q_lens", q)
     ins = _heads(dout, "dout"), _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(out, "out")

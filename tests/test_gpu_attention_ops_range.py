@@ -12,7 +12,7 @@ import torch
 
 from hexo_bot_b200 import attention_ops as ops
 from oracle import attention_ops as O
-from test_gpu_attention_ops import BF16, DEV, F16, F32, gen, randn, within
+from test_gpu_attention_ops import BF16, DEV, F16, F32, gen, randn, spread, within
 
 pytestmark = pytest.mark.gpu
 
@@ -230,6 +230,30 @@ def test_writes_into_out_are_seen_by_autograd():
     with torch.inference_mode():
         z = x.clone()
         assert torch.equal(ops.axes_rotary(z, coords, freqs, (8,), out=z), want)
+
+
+def test_rows_and_heads_that_overlap():
+    """Views whose rows or heads lie one element apart (sliding windows) give what copies give."""
+    base = randn(gen(123), 4000)
+    coords = torch.randint(-9, 9, (1, 4, 1), generator=gen(124), device=DEV)
+    freqs = ops.rotary_freqs((8,), device=DEV)
+    for strides in ((0, 100, 1, 1), (0, 1, 50, 1), (0, 1, 1, 1)):
+        x = base.as_strided((1, 3, 4, 16), strides)
+        copy = x.clone(memory_format=torch.contiguous_format)
+        assert torch.equal(ops.axes_rotary(x, coords, freqs, (8,)), ops.axes_rotary(copy, coords, freqs, (8,)))
+        # behind the norm against 64 bits: narrower accesses add the squares in another order
+        ang = O.angles(coords, freqs, (8,), 4)
+        x64 = copy.double().requires_grad_()
+        want = O.qk_norm(x64, None, ang)
+        rstd = (x64.square().mean(-1, keepdim=True) + 1e-6).rsqrt().detach()
+        hat = (x64.detach() * rstd).abs()
+        for out in ops.qk_norm_rotary(x, x, None, None, coords, freqs, (8,)):
+            within(out, want.detach(), O.rounding(want.detach(), F32) + 40 * 2.0**-24 * spread(hat, ang, False))
+        (dx,) = torch.autograd.grad(want, x64, copy.double())
+        back = spread(copy.double().abs(), ang, False)
+        mass = rstd * (back + hat * (back * hat).mean(-1, keepdim=True))
+        for got in ops.qk_norm_rotary_backward(copy, copy, x, x, None, None, coords, freqs, (8,))[:2]:
+            within(got, dx, O.rounding(dx, F32) + 80 * 2.0**-24 * mass)
 
 
 # ---- several windows ----------------------------------------------------------------------------
