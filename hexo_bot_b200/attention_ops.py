@@ -36,6 +36,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _MOST = 2**31 - 1
+_PROXY = torch._C._TorchDispatchModeKey.PROXY  # the mode of make_fx
 _FLOATS = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 _COORDS = {torch.int64: _lib.DT_I64, torch.int32: _lib.DT_I32, torch.int16: _lib.DT_I16, torch.float32: _lib.DT_F32}
 
@@ -104,9 +105,12 @@ def _lens(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> Optional[
     return t.data_ptr()
 
 
-def _on(t: torch.Tensor, what: str, fn, *args) -> None:
-    """fn(*args) with t's device as the current one; raises on a refusal."""
+def _call(t: torch.Tensor, what: str, fn, *args, stream: bool = True) -> None:
+    """fn(*args) with t's device as the current one, and that device's current stream as the last
+    argument of calls that take one; raises on a refusal."""
     index = t.device.index
+    if stream:
+        args += (torch._C._cuda_getCurrentRawStream(index),)
     if index == torch._C._cuda_getDevice():
         rc = fn(*args)
     else:
@@ -116,16 +120,11 @@ def _on(t: torch.Tensor, what: str, fn, *args) -> None:
         _lib.check(rc, what)
 
 
-def _call(t: torch.Tensor, what: str, fn, *args) -> None:
-    """fn(*args, stream) on t's device and its current stream; raises on a refusal."""
-    _on(t, what, fn, *args, torch._C._cuda_getCurrentRawStream(t.device.index))
-
-
 def _visible(*ts) -> None:
     """Refuses calls that would lose something in silence: a trace would not see the kernel and keep
     its outputs as memory without values, a forward-mode tangent of ts would be dropped."""
 
-    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if torch._C._is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None:
         raise RuntimeError("the kernels cannot be traced: leave the call outside of the traced function")
     if forward_ad._current_level >= 0:
         if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
@@ -367,7 +366,7 @@ def _attn_args(q, k, v, index, block, scale):
 
 def _attn_workspace(t, sizes, backward):
     need = C.c_size_t()  # the plan counts the SMs of the device that the call runs on
-    _on(t, "block_attention", _lib.lib().sb_block_attention_workspace_bytes, *sizes, backward, need)
+    _call(t, "block_attention", _lib.lib().sb_block_attention_workspace_bytes, *sizes, backward, need, stream=False)
     return torch.empty(need.value, dtype=torch.uint8, device=t.device) if need.value else None, need.value
 
 
