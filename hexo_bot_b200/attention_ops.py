@@ -135,6 +135,12 @@ def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _frozen(coords, freqs) -> None:
+    for t, name in ((coords, "coords"), (freqs, "freqs")):
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} gets no gradient: detach it")
+
+
 # ---- rotary positions -------------------------------------------------------------------------
 
 
@@ -142,7 +148,7 @@ def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, device="cuda")
     """The usual angle table: axis a's pair j of m turns theta ** (-j / m) radians a step.
 
     float64, one entry per pair, axes in order. Any other table of that form (scaled, learned and
-    frozen) serves as well."""
+    frozen) serves as well; neither it nor the coordinates get a gradient."""
 
     table = [theta ** (-j / m) for m in sections for j in range(m)]
     return torch.tensor(table, dtype=torch.float64, device=device)
@@ -211,6 +217,7 @@ def axes_rotary(x, coords, freqs, sections, *, adjacent=False, inverse=False, ou
     need a gradient, but graphs that kept it refuse their backward, as after torch's own writes."""
 
     _visible(x, coords, freqs)
+    _frozen(coords, freqs)
     _first(x, "x")
     if _wants_grad(x, out):
         if out is not None:
@@ -300,6 +307,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, coords=None, freqs=None, sections=(
     ((D) or None), then the rotation of `axes_rotary` (coords None: none), in one pass."""
 
     _visible(q, k, q_weight, k_weight, coords, freqs)
+    _frozen(coords, freqs)
     _first(q, "q")
     if _wants_grad(q, k, q_weight, k_weight):
         return _QkNorm.apply(q, k, q_weight, k_weight, coords, freqs, tuple(sections), adjacent, eps)

@@ -118,3 +118,15 @@ def test_workspace_is_sized_on_the_tensors_device(monkeypatch):
     ops.block_attention(x, x, x, index, 64)
     ops.block_attention_backward(x, x, x, x, x, torch.zeros(1, 1, 20), index, 64)
     assert asked == [1, 1] and current == [0]
+
+
+@pytest.mark.parametrize("which", ["coords", "freqs"])
+def test_tables_that_need_a_gradient_are_refused(which):
+    """Neither coordinates nor frequencies get one: a table that is still learned would stand still."""
+    coords, freqs = torch.zeros(1, 4, 1), FREQS.clone()
+    {"coords": coords, "freqs": freqs}[which].requires_grad_()
+    for call in (lambda: ops.axes_rotary(X, coords, freqs, (8,)), lambda: ops.qk_norm_rotary(X, X, W, W, coords, freqs, (8,))):
+        with pytest.raises(ValueError, match=f"{which} gets no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
