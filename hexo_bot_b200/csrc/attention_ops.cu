@@ -513,10 +513,10 @@ static int qk_norm(const char* what, const sb_heads* q, const sb_heads* k, const
   const bool adjacent = rotary && rotary->adjacent != 0;
   int grid = 0;
   if (backward) {
-    const size_t need = (size_t)kRotMaxGrid * 2 * head_dim * 4;
+    const size_t need = (size_t)kRotMaxGrid * 2 * head_dim * 8;
     if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
       return fail(SB_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned, needed", what, need);
-    a.dw_part = (float*)workspace;
+    a.dw_part = (double*)workspace;
     if (work)
       if (int s = launch_rotary(a, ROT_NORM_BWD, dtype, adjacent, vec, st, &grid)) return s;
     if (!dqw && !dkw) return SB_OK;
@@ -538,7 +538,7 @@ int sb_qk_norm_rotary(const sb_heads* q, const sb_heads* k, int dtype, const voi
 
 int sb_qk_norm_rotary_backward_workspace_bytes(int head_dim, size_t* bytes) {
   if (!bytes || head_dim < 1 || head_dim > kRotMaxDim) return fail(SB_ERR_INVALID_ARG, "qk_norm_rotary_backward: bad args");
-  *bytes = (size_t)kRotMaxGrid * 2 * head_dim * 4;
+  *bytes = (size_t)kRotMaxGrid * 2 * head_dim * 8;
   return SB_OK;
 }
 

@@ -37,6 +37,7 @@ constexpr int kRotThreads = 256;
 constexpr int kRotMaxDim = 256;
 constexpr int kRotMaxAxes = 4;
 constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kRotAdds = 32;            // weight gradients of so many heads are summed in 32 bits before 64
 constexpr int kRotMaxGrid = 148 * 2;    // CTAs of the gradient kernel (one partial weight gradient each)
 
 enum RotOp { ROT_TURN = 0, ROT_NORM = 1, ROT_NORM_BWD = 2 };
@@ -50,7 +51,7 @@ struct RotArgs {
   int heads[2];
   const void* w[2];            // norm weights or null (= 1)
   int w_dtype;
-  float* dw_part;              // backward: [grid][2][D]
+  double* dw_part;             // backward: [grid][2][D]
   const void* coords;
   int coord_dtype, axes;
   long long cs[3];             // batch, row, axis
@@ -205,8 +206,26 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
       pr[k] = -1;
     }
   }
+  // weight gradients: a thread's own sum of a few heads, and the warp's, in 64 bits
+  // (a channel's by one lane), so that long sums lose no more than short ones
+  __shared__ double dw_sum[BWD ? kRotWarps : 1][BWD ? kRotMaxDim : 1];
   float dwa[NI][2 * VEC];
+  int adds = 0;
+  auto flush = [&] {
+    adds = 0;
+#pragma unroll
+    for (int k = 0; k < NI; ++k)
+#pragma unroll
+      for (int e = 0; e < 2 * VEC; ++e) {
+        float s = dwa[k][e];
+        dwa[k][e] = 0.f;
+        for (int m = L; m < 32; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        const int c = e < VEC ? ca[k] + e : cb[k] + e - VEC;
+        if ((e < VEC ? ca[k] : cb[k]) >= 0 && lane < L) dw_sum[warp][c] += (double)s;
+      }
+  };
   if (BWD) {
+    for (int c = tid; c < kRotWarps * kRotMaxDim; c += kRotThreads) dw_sum[c / kRotMaxDim][c % kRotMaxDim] = 0.0;
 #pragma unroll
     for (int k = 0; k < NI; ++k)
 #pragma unroll
@@ -361,6 +380,7 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
             }
           }
           if (BWD) {
+            ++adds;
             float c1 = 0.f;  // sum of w g x^ over the head
 #pragma unroll
             for (int k = 0; k < NI; ++k)
@@ -394,26 +414,16 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
         if (BWD) g += U * gh;
       }
     }
+    if (BWD && adds >= kRotAdds) flush();
   }
 
   if (BWD) {
-    // CTA sum of the weight gradients in a fixed order: the heads of a warp first
-    // (threads of one lane hold the same channels), then the warps
-    __shared__ float red[kRotWarps][kRotMaxDim];
-#pragma unroll
-    for (int k = 0; k < NI; ++k)
-#pragma unroll
-      for (int e = 0; e < 2 * VEC; ++e) {
-        float s = dwa[k][e];
-        for (int m = L; m < 32; m <<= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        const int c = e < VEC ? ca[k] + e : cb[k] + e - VEC;
-        const bool have = e < VEC ? ca[k] >= 0 : cb[k] >= 0;
-        if (have && lane < L) red[warp][c] = s;
-      }
+    // CTA sum of the weight gradients, warp after warp
+    flush();
     __syncthreads();
     for (int c = tid; c < D; c += kRotThreads) {
-      float s = 0.f;
-      for (int g = 0; g < kRotWarps; ++g) s += red[g][c];
+      double s = 0.0;
+      for (int g = 0; g < kRotWarps; ++g) s += dw_sum[g][c];
       a.dw_part[((long long)blockIdx.x * 2 + blockIdx.y) * D + c] = s;
     }
   }
@@ -421,7 +431,7 @@ __global__ __launch_bounds__(kRotThreads, OP == ROT_NORM_BWD ? 2 : 3) void rotar
 
 // Weight gradients: the sum of every CTA's part, in 64 bits and in CTA order
 // within each of 32 strands, then over the strands.
-__global__ __launch_bounds__(1024) void rotary_dw_kernel(const float* __restrict__ part, int grid, int dim, void* dw0,
+__global__ __launch_bounds__(1024) void rotary_dw_kernel(const double* __restrict__ part, int grid, int dim, void* dw0,
                                                          void* dw1, int w_dtype, int heads0, int heads1) {
   __shared__ double red[32][33];
   const int h = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
@@ -429,7 +439,7 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float* __restrict
   double s = 0.0;
   if (c < dim && (h ? heads1 : heads0) > 0)
 #pragma unroll 8
-    for (int g = threadIdx.y; g < grid; g += 32) s += (double)part[((long long)g * 2 + h) * dim + c];
+    for (int g = threadIdx.y; g < grid; g += 32) s += part[((long long)g * 2 + h) * dim + c];
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < dim && dw) {

@@ -168,6 +168,31 @@ def test_rows_without_a_place_keep_infinities_to_themselves(dtype, adjacent):
         assert torch.equal(a[:, :, :3].nan_to_num(5.0), c[:, :, :3].nan_to_num(5.0))
 
 
+@pytest.mark.parametrize("b,s,hq,hk,d,sections", [(3, 217, 12, 4, 20, (3, 5)), (8, 2440, 16, 4, 64, (16, 16)),
+                                                  (64, 500, 8, 8, 128, (64,)), (2000, 37, 3, 1, 18, (2, 3))])
+def test_weight_gradients_of_long_sums(b, s, hq, hk, d, sections):
+    """dq_weight and dk_weight err no more than 32-bit terms summed in 64 bits do (1.5 times: both
+    errors are sums of independent roundings over the channels), however many rows there are."""
+    g = gen(113)
+    q, k, gq, gk = (randn(g, b, h, s, d, scale=1.5) for h in (hq, hk, hq, hk))
+    w = 1 + randn(g, d, scale=0.2)
+    coords = torch.randint(-32, 32, (b, s, len(sections)), generator=g, device=DEV)
+    freqs = ops.rotary_freqs(sections, device=DEV)
+    ang = -O.angles(coords, freqs, sections, s)
+    grads = ops.qk_norm_rotary_backward(gq, gk, q, k, w, w, coords, freqs, sections)
+    p = sum(sections)
+    for x, gy, dw in zip((q, k), (gq, gk), grads[2:]):
+        found = []
+        for dt in (torch.float64, F32):
+            cos, sin, u, v = ang.cos().to(dt), ang.sin().to(dt), gy[..., :p].to(dt), gy[..., p : 2 * p].to(dt)
+            turned = torch.cat([u * cos - v * sin, v * cos + u * sin, gy[..., 2 * p :].to(dt)], -1)
+            hat = x.to(dt) * torch.rsqrt(x.to(dt).square().mean(-1, keepdim=True) + 1e-6)
+            found.append((turned * hat).sum((0, 1, 2), dtype=torch.float64).to(dt))
+        want, plain = found
+        off, least = ((t.double() - want).norm() for t in (dw, plain))
+        assert off <= 1.5 * least + 2.0**-24 * want.norm(), (off / want.norm(), least / want.norm())
+
+
 PI = Fraction(31415926535897932384626433832795028841971693993751058209749445923, 10**64)
 
 
