@@ -336,7 +336,10 @@ def block_select(q, means, topk, block, kv_rows, *, kv_lens=None, q_lens=None, k
 
     Score of a block: the group's query heads, summed, times its mean (`block_means`, or means that
     a serving program keeps up to date). The first `keep_first` blocks, and with `keep_own` the
-    block row // block, are always kept. Ties go to the lowest index."""
+    block row // block, are always kept. Rows count from 0 in every call, so for one query against a
+    history `keep_own` names block 0: leave it off there, choose topk - 1 blocks and put the newest
+    one behind them (`block_attention` takes any order and counts a block named twice once). Ties go
+    to the lowest index."""
 
     _visible()
     _first(q, "q")
@@ -438,7 +441,7 @@ def block_attention(q, k, v, index, block, *, scale=None, kv_lens=None, q_lens=N
     q (B, Hq, Sq, D), k and v (B, Hkv, Sk, D) float16 or bfloat16, index (B, Hkv, Sq, topk) int32
     as `block_select` gives it (any order; entries out of range are skipped, one named twice counts
     once), block 32, 64 or 128, scale 1 / sqrt(D) by default. lse (B, Hq, Sq) float32 is the log of
-    each row's sum of exp(scores). Rows without keys and rows past q_lens give zeros and -inf."""
+    each row's sum of exp(scores) and has no gradient. Rows without keys and rows past q_lens give zeros and -inf."""
 
     _visible(q, k, v)
     _first(q, "q")

@@ -315,7 +315,8 @@ int sb_block_means(const sb_heads* k, int dtype, const int32_t* kv_lens, int bat
  * heads) . mean: index (B, Hkv, Sq, topk) int32, ascending, -1 where a row has
  * fewer live blocks or is no live query (row >= q_lens[b]). The first
  * keep_first blocks, and with keep_own the block row / block, are kept before
- * the others (keep_first + keep_own <= topk). Ties go to the lowest index, NaN
+ * the others (keep_first + keep_own <= topk). Rows count from 0 in every call: for
+ * one query against a history keep_own names block 0, not the newest. Ties go to the lowest index, NaN
  * ranks below every number. The choice equals that of 64-bit scores.
  * topk <= 64, at most 16384 blocks, D <= 256. */
 int sb_block_select(const sb_heads* q, int dtype, const float* means, const int32_t* kv_lens, const int32_t* q_lens, int batch,

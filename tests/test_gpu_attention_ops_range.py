@@ -196,14 +196,14 @@ def test_weight_gradients_of_long_sums(b, s, hq, hk, d, sections):
 PI = Fraction(31415926535897932384626433832795028841971693993751058209749445923, 10**64)
 
 
-@pytest.mark.parametrize("kind", [torch.int64, torch.int32, F32])
-@pytest.mark.parametrize("size", [2**20, 2**28, 2**31 - 1, 10**12, 1_700_000_000_000, 1_700_000_000_000_000, 2**52, 2**53])
+FAR = [2**20, 2**28, 2**31 - 1, 10**12, 1_700_000_000_000, 1_700_000_000_000_000, 2**52, 2**53]
+
+
+@pytest.mark.parametrize("size,kind", [(n, t) for n in FAR for t in (torch.int64, F32)] + [(n, torch.int32) for n in FAR[:3]])
 def test_coordinates_of_any_size(size, kind):
     """cos and sin of far positions against exact arithmetic. One turn of (1, 0): the kernel's
     reduced angle is a float of at most pi / 4 (three roundings of 2^-24), its series and their
     roundings are off by 1e-7 at most: 2^-22 in all."""
-    if kind == torch.int32 and size >= 2**31:
-        pytest.skip("past the type")
     places = torch.tensor([size, size - 1, -size, size // 3, size // 7 * 5, 1], dtype=torch.int64).to(kind)
     freqs = torch.tensor([1.0, 0.7853981633974483, 1e-4, 1 / 3], dtype=torch.float64)
     n = places.numel()
@@ -279,6 +279,24 @@ def test_rows_and_heads_that_overlap():
         mass = rstd * (back + hat * (back * hat).mean(-1, keepdim=True))
         for got in ops.qk_norm_rotary_backward(copy, copy, x, x, None, None, coords, freqs, (8,))[:2]:
             within(got, dx, O.rounding(dx, F32) + 80 * 2.0**-24 * mass)
+
+
+def test_one_token_with_its_newest_block():
+    """Means kept by the program, one query, the newest block put behind the chosen ones."""
+    g = gen(125)
+    k, v = (randn(g, 3, 2, 900, 64, dtype=BF16) for _ in range(2))
+    q = randn(g, 3, 8, 1, 64, dtype=BF16)
+    lens = torch.tensor([900, 333, 64], dtype=torch.int32, device=DEV)
+    means = ops.block_means(k, 64, kv_lens=lens)
+    newest = ((lens - 1) // 64).view(3, 1, 1, 1).expand(3, 2, 1, 1)
+    index = torch.cat([ops.block_select(q, means, 4, 64, 900, kv_lens=lens, keep_first=1), newest], -1)
+    out, lse = ops.block_attention(q, k, v, index, 64, kv_lens=lens)
+    want = O.select(q, means, 4, 64, 900, lens, None, 1, False)
+    kept = torch.cat([want.to(DEV), newest], -1)
+    assert torch.equal(index, kept) and index[1, 0, 0, -1] == 5 and index[2, 0, 0].tolist() == [0, -1, -1, -1, 0]
+    found, bound = O.attention(q, k, v, kept, 64, None, lens, pair=True)
+    within(out, found["out"], bound["out"], "out")
+    within(lse, found["lse"], bound["lse"], "lse")
 
 
 # ---- several windows ----------------------------------------------------------------------------
