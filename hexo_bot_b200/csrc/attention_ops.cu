@@ -118,8 +118,8 @@ int launch_rotary(RotArgs& a, int op, int dtype, bool adjacent, int vec, cudaStr
   a.inv_dim = 1.f / (float)D;
   // heads side by side: no more than share the work of the angles, and half of
   // them at most, so that a lane's angles serve two heads or more (4096 x 69 rows,
-  // 8 heads of 16: 47 us with all side by side, 35 with half, 35 with a quarter,
-  // 53 with an eighth, where loads touch too many lines)
+  // 8 heads of 16: 49 us with all side by side, 37 with half, 37 with a quarter,
+  // 54 with an eighth, where loads touch too many lines)
   const int least = a.heads[1] > 0 && a.heads[1] < a.heads[0] ? a.heads[1] : a.heads[0];
   int side = 0;
   while (side + a.lanes_log2 < 5 && (2 << side) <= vec && 2 * (2 << side) <= a.heads[0] && (2 << side) <= least) ++side;
@@ -180,6 +180,10 @@ int launch_select_per(const SelArgs& a, unsigned grid, cudaStream_t st) {
   block_select_kernel<T, PER, LPR><<<grid, kSelThreads, smem, st>>>(a);
   return check_launch("block_select_kernel");
 }
+// The form with the fewest scores and lanes a row that holds the blocks (2 lanes of
+// 20 / 2 of 32 / 4 of 32 / a warp a row, us, 16 x 2440 rows, 8 heads of 16: 110 / 151 /
+// 237 / 383 at 39 blocks, - / 157 / 243 / 385 at 64, - / - / 302 / 577 at 128; 8192 rows,
+// 4 heads of 128: 44 / 50 / 54 / 79, - / 57 / 62 / 86, - / - / 78 / 125).
 template <typename T>
 int launch_select(const SelArgs& a, unsigned grid, cudaStream_t st) {
   if (a.nb <= 40) return launch_select_per<T, 20, 2>(a, grid, st);
@@ -215,17 +219,18 @@ int launch_select_few(const SelArgs& a, unsigned rows, int cluster, cudaStream_t
 // ---- block-sparse attention ------------------------------------------------------
 // Bytes of parts that a window of rows may hold. Windows that fit the 126 MB L2
 // keep the parts off HBM but leave the SMs short of work at every launch's end:
-// 8192 rows, 8 heads of 64, 16 of 128 blocks, forward: 335 us with windows of
-// 64 MB, 278 with 100, 255 with 200, 234 with one of 277 MB.
+// 8192 rows, 8 heads of 64, 16 of 128 blocks, forward / backward: 402 / 598 us with
+// windows of 64 MB, 276 / 557 with 100, 254 / 510 with 200, 210 / 412 with one; 16 x
+// 2440 rows, 8 heads of 16: 278 / 577, 258 / 537, 228 / 494 with 200 MB or more.
 constexpr long long kBaWindowBytes = 1ll << 30;
-// Up to so many queries take the few-query kernel (few / many, us, 8 heads of 64,
-// 16 blocks: 8 / 19 at 2 rows, 10 / 21 at 16, 20 / 21 at 32, 39 / 21 at 64; 8 x 8
-// groups of 4 heads of 128: 17 / 99 at 2, 116 / 143 at 16, 230 / 163 at 32).
+// Up to so many queries take the few-query kernel (few / many, us, 8 heads of 64, 16
+// of 128 blocks: 8 / 21 at 2 rows, 11 / 22 at 16, 21 / 22 at 32, 40 / 22 at 64; 8 x 8
+// groups of 4 heads of 128, 32 of 512: 30 / 302, 205 / 435, 408 / 488, 812 / 544).
 constexpr int kBaFewRows = 16;
 // Work items an SM and window, and the listed rows that an item may hold: fewer
 // items leave SMs idle behind popular blocks (8192 rows, 8 heads of 64, 16 of 128
-// blocks, forward: 211 us with 8 an SM, 201 with 16 to 32; backward, where every
-// segment of a block leaves a part of dk and dv: 338 / 335 / 326 / 326 / 334 us
+// blocks, forward: 212 us with 8 an SM, 200 with 16 to 32; backward, where every
+// segment of a block leaves a part of dk and dv: 431 / 429 / 397 / 402 / 403 us
 // with 4 / 6 / 8 / 12 / 16), smaller ones repeat the listing and the key loads.
 constexpr int kBaItems = 16, kBaBwdItems = 8, kBaMinTarget = 256, kBaMaxTarget = 1024;
 
@@ -346,8 +351,8 @@ struct LaunchFew {
     constexpr int W = ba_few_warps<DP, BK>();
     const long long rows = (long long)a.batch * a.kv_heads * a.q_rows * ((a.group + 15) / 16);
     // CTAs of a row: as many as have a block for every warp and run at once (64
-    // rows of 32 blocks, D = 128: 29 us with one CTA a row, 17 with two, 21 with
-    // four, 37 with eight, which take turns)
+    // rows of 32 blocks, D = 128: 30 us with one CTA a row, 19 with two, 23 with
+    // four, 39 with eight, which take turns)
     int cluster = 1;
     while (cluster < kBaFewCluster && cluster * W < a.topk && 2 * rows * cluster <= num_sms()) cluster *= 2;
     if (rows * cluster > 0x7fffffffll) return fail(SB_ERR_UNSUPPORTED, "block_attention: too many rows for one launch");
@@ -644,8 +649,11 @@ int sb_block_select(const sb_heads* q, int dtype, const float* means, const int3
     if (dtype == SB_F16) return launch_select_few<__half>(a, (unsigned)rows, cluster, st);
     return launch_select_few<__nv_bfloat16>(a, (unsigned)rows, cluster, st);
   }
-  // the widest tile whose scores leave room for two CTAs an SM (four where short
-  // rows make a row's own work small against the CTA's), no wider than the rows
+  // the widest tile that leaves the three CTAs an SM which registers allow their
+  // shared memory (16 x 2440 rows, 8 heads of 16, limits of 40 / 56 / 72 KB: 191 / 155 /
+  // 155 us at 41 blocks, 293 / 292 / 270 at 96, the same at others), or two of them
+  // where 64 rows are too many for that (112 KB, or 72: 1248 and 1039 us at 256 blocks,
+  // 3976 and 4940 at 1024), no wider than the rows
   int tile = 128;
   while (tile > 64 && (sel_smem_bytes(tile, a.nb, head_dim) > 56 * 1024 || tile / 2 >= q_rows)) tile >>= 1;
   while (tile > 2 && (sel_smem_bytes(tile, a.nb, head_dim) > 112 * 1024 || tile / 2 >= q_rows)) tile >>= 1;

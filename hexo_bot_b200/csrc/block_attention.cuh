@@ -5,8 +5,8 @@
 //   backward: dv_t += p_t do, ds_t = p_t (do . v_t - do . out),
 //             dq = scale sum ds_t k_t, dk_t += scale ds_t q
 //
-// Neighbouring queries choose different blocks, so a tile of queries shares no
-// key block and a query alone fills one row of a matrix instruction. The work
+// Neighbouring queries need not choose the same blocks: a tile of queries may share
+// no key block, and a query alone fills one row of a matrix instruction. The work
 // is turned round: a work item is one key block (in shared memory) and a segment
 // of the queries; its CTA lists the queries that chose the block and runs them in
 // tiles of 128 rows through the tensor cores. Each (query, block) pair leaves a partial
@@ -390,13 +390,13 @@ struct BaTile {
 // Tiles of 128 listed rows on the fifth-generation tensor cores, one row a
 // thread: S = Q K^T into TMEM; each thread reads its row of S, takes maximum,
 // exponentials and sum without any exchange and writes the weights back over S as
-// pairs of 16-bit numbers; O = P V with P as the TMEM operand; O leaves through the tile's own Q
-// buffer (transposed there, so that a part goes out in whole 128-byte lines).
-// Four CTAs an SM (128 TMEM columns each at D = 64) cover one another's waits.
-// An mma.sync form of this kernel, 16 rows a warp, took 134 us where this one
-// takes 118 (8192 rows, 8 heads of 64, 16 of 128 blocks): it issued 48
-// instructions a row and read every key and value fragment from shared memory
-// once per 16 rows (74 % of that pipe).
+// pairs of 16-bit numbers; O = P V with P as the TMEM operand; O leaves through the
+// tile's own Q buffer (transposed there, so that a part goes out in whole 128-byte
+// lines). Four CTAs an SM (128 TMEM columns each at D = 64) cover one another's waits.
+// 8192 rows, 8 heads of 64, 16 of 128 blocks: 129 us, 118 with single 16-bit weights;
+// an mma.sync form, 16 rows a warp, took 134 with those: it issued 48 instructions
+// a row and read every key and value fragment from shared memory once per 16 rows
+// (74 % of that pipe).
 //
 // Shared memory, rows of 128 bytes (64 channels; DP = 128: two panels) in the
 // 128-byte swizzle: K, V [panels][BK], Q [2][panels][128]. As a left or right
@@ -1019,9 +1019,10 @@ __global__ __launch_bounds__(256) void block_attn_delta_kernel(const BaArgs a) {
 //   |ds| <= |do| max |v| + |delta|
 // over the tile's rows and the block's keys below 2^15. The power holds for a work
 // item (with two octaves to spare at first); a tile that needs a smaller one
-// has the dk summed so far scaled down. Values down to 2^-39 of the bound are not lost.
-// An mma.sync form, 64 rows a tile, took 310 us where this one takes about 260 (8192
-// rows, 8 heads of 64, 16 of 128 blocks).
+// has the dk summed so far scaled down. Values down to 2^-37 of the bound are not lost.
+//
+// 8192 rows, 8 heads of 64, 16 of 128 blocks: 330 us, 266 with single 16-bit p and ds;
+// an mma.sync form, 64 rows a tile, took 310 with those.
 constexpr int kBaBwdThreads = 128;
 
 template <int DP, int BK>

@@ -565,7 +565,7 @@ __device__ __forceinline__ void sel_split8(const float (&x)[8], __nv_bfloat16* h
 }
 
 // PER > 0: rows of up to LPR PER blocks, LPR lanes a row (the fewer, the fewer
-// instructions a row: 16 x 2440 rows, 8 heads, 39 blocks 102 us with eight, 89 with two); 0: a warp a row.
+// instructions a row); 0: a warp a row.
 template <typename T, int PER, int LPR>
 __global__ __launch_bounds__(kSelThreads, 3) void block_select_kernel(const SelArgs a) {
   extern __shared__ __align__(16) char sel_smem[];
