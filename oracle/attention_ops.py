@@ -149,7 +149,7 @@ def attention(q, k, v, index, block, scale=None, kv_lens=None, q_lens=None, dout
         e_delta = (g.abs() * (bound["out"] + rounding(out, q.dtype))).sum(-1, keepdim=True)
         e_dp = (d + 4) * 2.0**-24 * (g.abs() @ v64.abs().transpose(-1, -2))
         floor = sub * seen
-        if pair:
+        if pair and sk:
             most = g.norm(dim=-1).max() * v64.norm(dim=-1).max() * math.ceil(d / 8) ** 0.5 + delta.abs().max()
             floor = floor * 2.0**-12 * most
         e_ds = (u + rel_p) * ds.abs() + p * (e_delta + e_dp + 2.0**-22 * delta.abs()) + floor
